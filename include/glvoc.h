@@ -408,6 +408,85 @@ int glv_plan_last_loop_groups(const glv_plan* plan);
 int glv_plan_drawn_phase(glv_plan* plan, uint64_t seed, int batch, int frames_stride, int64_t frame_origin,
                          float* phase_dev, void* stream);
 
+/*
+ * Operators of the acoustic model's serving path (reference TTS/Fastspeech_1.py:12-56: products
+ * with fixed weights, each followed by a norm).  They need no plan, allocate nothing and wait for
+ * nothing; they run on the current device, on which every array must lie, and may be captured
+ * into a graph.  Float arrays are of one of the types below and aligned to their elements; the
+ * last dimension is contiguous, strides are counted in elements, outputs are contiguous.
+ * Zero rows (or columns of output) are answered with GLV_OK before any pointer is looked at.
+ */
+enum {
+    GLV_F32 = 0,
+    GLV_BF16 = 1,
+    GLV_F16 = 2,
+    GLV_MXFP4 = 3 /* quantised by glv_mxfp4_quantize */
+};
+
+/*
+ * Microscaled 4-bit floating point: along the last dimension every 32 elements share a scale 2^s,
+ * s = max(floor(log2 max|x|) - 2, -127), held as the byte s + 127; an element is the E2M1 code of
+ * x / 2^s (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign bit) to the nearest, ties to the even code, 6
+ * beyond 6.  A block that holds an infinity or a NaN has the scale byte 255 and reads as NaN.
+ * With groups = ceil(cols / 128), columns beyond cols being zero:
+ *   codes_dev   (rows, groups, 64) bytes, the even column in the low half; 16-byte aligned
+ *   scales_dev  (groups, rows, 4) bytes; 4-byte aligned
+ * where rows counts batch * rows.  At most 2^24 rows and 2^18 columns.
+ *   glv_mxfp4_quantize:   x_dev (batch, rows, cols), x[b, r, :] at b * batch_stride + r * row_stride.
+ *   glv_mxfp4_dequantize: out_dev (rows, cols); exact in float32 and bfloat16, and in float16 wherever
+ *                         that type can hold the value.
+ */
+int glv_mxfp4_quantize(const void* x_dev, int x_type, int batch, int rows, int cols, int64_t batch_stride,
+                       int64_t row_stride, uint8_t* codes_dev, uint8_t* scales_dev, void* stream);
+int glv_mxfp4_dequantize(const uint8_t* codes_dev, const uint8_t* scales_dev, int rows, int cols, int out_type,
+                         void* out_dev, void* stream);
+
+/*
+ * y[b, t, n] = act(sum_{j, c} q(x)[b, t + j * dilation - left, c] * w[n, j, c] + bias[n]),
+ * left = dilation * (taps - 1) / 2, rows outside [0, rows) of a batch entry counting as zeros: a
+ * linear layer for taps = 1, else Keras' Conv1D(padding='same') over a channels-last sequence.
+ * x is quantised by the call (x_type a float type; x_scales_dev is not used) or has been
+ * (GLV_MXFP4: x_dev holds the codes of batch * rows rows, strides are not used).  Sums are float.
+ *   w_codes_dev, w_scales_dev   (n_out, taps, cols) quantised by glv_mxfp4_quantize, n_out * taps rows
+ *   bias_dev                    n_out values of bias_type, or NULL
+ *   y_dev                       (batch, rows, n_out) of y_type
+ *   workspace_dev               glv_mxfp4_product_workspace() bytes, 16-byte aligned, free to use
+ *                               until the work on the stream is done (NULL when that is 0);
+ *                               the function returns -1 for a shape that the product refuses.
+ * taps * cols and n_out are at most 2^18, n_out * taps and (taps - 1) * dilation at most 2^24.
+ */
+enum { GLV_ACT_NONE = 0, GLV_ACT_RELU = 1 };
+int64_t glv_mxfp4_product_workspace(int x_type, int batch, int rows, int cols, int n_out, int taps);
+int glv_mxfp4_product(const void* x_dev, const uint8_t* x_scales_dev, int x_type, int batch, int rows, int cols,
+                      int64_t x_batch_stride, int64_t x_row_stride, const uint8_t* w_codes_dev,
+                      const uint8_t* w_scales_dev, int n_out, int taps, int dilation, const void* bias_dev,
+                      int bias_type, int activation, void* y_dev, int y_type, void* workspace_dev,
+                      int64_t workspace_bytes, void* stream);
+
+/*
+ * The end of a block and the start of the next, row by row:
+ *     y = residual + scale * scale_vec * gate * Norm_post(u)      z = Norm_pre(y)
+ * GLV_NORM_LAYER: (x - mean) / sqrt(mean((x - mean)^2) + eps) * weight + bias;
+ * GLV_NORM_RMS: x / sqrt(mean(x^2) + eps) * weight + bias; GLV_NORM_NONE: x (as the post norm), no z
+ * (as the pre norm).  Statistics are float; z is formed from y before y is rounded.
+ *   u, gate, residual   (batch, rows, cols) of `type`, each with strides of its own; gate strides may
+ *                       be 0 (a gate that is shared by rows, entries or, gate_col_stride 0, columns);
+ *                       gate and residual may be NULL (1 and 0)
+ *   post_/pre_weight, post_/pre_bias, scale_dev   cols values of vector_type (GLV_F32 or `type`), or
+ *                       NULL (1, 0 and 1); scale multiplies on top
+ *   y_dev, z_dev        (batch, rows, cols) of `type`; y may be u, gate or residual itself when that
+ *                       is contiguous (a row is read before it is written)
+ * At most 2^24 rows and 32768 columns.
+ */
+enum { GLV_NORM_NONE = 0, GLV_NORM_LAYER = 1, GLV_NORM_RMS = 2 };
+int glv_block_norm(const void* u_dev, int type, int batch, int rows, int cols, int64_t u_batch_stride,
+                   int64_t u_row_stride, int vector_type, int post_kind, const void* post_weight_dev,
+                   const void* post_bias_dev, float post_eps, const void* gate_dev, int64_t gate_batch_stride,
+                   int64_t gate_row_stride, int gate_col_stride, const void* scale_dev, float scale,
+                   const void* residual_dev, int64_t residual_batch_stride, int64_t residual_row_stride,
+                   int pre_kind, const void* pre_weight_dev, const void* pre_bias_dev, float pre_eps, void* y_dev,
+                   void* z_dev, void* stream);
+
 const char* glv_last_error(void);
 
 #ifdef __cplusplus
