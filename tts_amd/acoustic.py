@@ -31,6 +31,8 @@ import torch
 from torch import nn
 import torch.nn.functional as F
 
+from .blocks import MXFP4Tensor, Norm, block_norm, mxfp4_conv1d, mxfp4_linear, mxfp4_quantize
+
 __all__ = ["FastSpeechAcousticModel", "synthesize"]
 
 _KERAS_EPS = 1e-3
@@ -62,17 +64,45 @@ class _MaskedBiLSTM(nn.Module):
         return torch.cat([fwd, out[..., self.units:]], dim=-1)
 
 
+class _SequenceConv(nn.Conv1d):
+    """Conv1D(padding='same') whose weight can be held in MXFP4 beside the float one.  The quantised
+    copy lies in buffers outside the state dict: it moves with the module, and checkpoints stay what
+    they were."""
+
+    def __init__(self, in_dim, out_dim, kernel, dilation=1):
+        super().__init__(in_dim, out_dim, kernel, padding="same", dilation=dilation)
+        self.register_buffer("mxfp4_codes", None, persistent=False)
+        self.register_buffer("mxfp4_scales", None, persistent=False)
+
+    def quantize(self, on):
+        q = mxfp4_quantize(self.weight.detach().permute(0, 2, 1)) if on else None
+        self.mxfp4_codes, self.mxfp4_scales = (q.codes, q.scales) if on else (None, None)
+
+    def sequence(self, x, relu=False):  # (B, T, C)
+        if self.mxfp4_codes is None:
+            y = self(x.transpose(1, 2))
+            return (F.relu(y) if relu else y).transpose(1, 2)
+        n, c, taps = self.weight.shape
+        weight = MXFP4Tensor((n, taps, c) if taps > 1 else (n, c), self.mxfp4_codes, self.mxfp4_scales)
+        activation = "relu" if relu else None
+        if taps == 1:
+            return mxfp4_linear(x, weight, self.bias, activation=activation)
+        return mxfp4_conv1d(x, weight, self.bias, dilation=self.dilation[0], activation=activation)
+
+
 class _ConvNorm(nn.Module):
     """Conv1D(padding='same', activation='relu') followed by LayerNormalization."""
 
     def __init__(self, in_dim, out_dim, kernel, dilation=1):
         super().__init__()
-        self.conv = nn.Conv1d(in_dim, out_dim, kernel, padding="same", dilation=dilation)
+        self.conv = _SequenceConv(in_dim, out_dim, kernel, dilation)
         self.norm = nn.LayerNorm(out_dim, eps=_KERAS_EPS)
 
     def forward(self, x):  # (B, T, C)
-        y = F.relu(self.conv(x.transpose(1, 2))).transpose(1, 2)
-        return self.norm(y)
+        y = self.conv.sequence(x, relu=True)
+        if self.conv.mxfp4_codes is None:
+            return self.norm(y)
+        return block_norm(y, post=Norm(self.norm.weight, self.norm.bias, eps=_KERAS_EPS))
 
 
 class Encoder(nn.Module):
@@ -141,9 +171,10 @@ class FastSpeechAcousticModel(nn.Module):
         self.embed = nn.Embedding(vocab_size, embedding_dim)
         self.encoder = Encoder(embedding_dim, hidden_dim)
         self.duration_predictor = DurationPredictor(hidden_dim)
-        self.mel_out = nn.Conv1d(hidden_dim, mel_dim, 1)
+        self.mel_out = _SequenceConv(hidden_dim, mel_dim, 1)
         self.post_net = PostNet(mel_dim)
         self.last_duration_prediction = None
+        self.register_load_state_dict_post_hook(FastSpeechAcousticModel._refresh_mxfp4)
         self.eval()
 
     @torch.no_grad()
@@ -162,8 +193,29 @@ class FastSpeechAcousticModel(nn.Module):
         x = self.encoder(x, lengths)
         self.last_duration_prediction = self.duration_predictor(x)
         x = length_regulate(x, durations)
-        mel_output = self.mel_out(x.transpose(1, 2)).transpose(1, 2)
+        mel_output = self.mel_out.sequence(x)
         return mel_output + self.post_net(mel_output)
+
+    # -- MXFP4 ------------------------------------------------------------------------
+    def use_mxfp4(self, on=True):
+        """Serves the convolutions of the encoder and the duration predictor and the mel head in MXFP4 (both
+        operands; sums, biases and norms in 32 bits): `tts_amd.mxfp4_conv1d`, `mxfp4_linear` and `block_norm`
+        in place of torch's products and norms.  The model must be on a ROCm GPU.  The LSTMs, the duration
+        predictor's last layer and the post-net, whose five applications of one layer would compound the
+        rounding, stay in the model's own type.  The float weights remain; loading weights
+        (`load_keras_weights`, `load_state_dict`) quantises them anew, after other changes to them call
+        this again.  ``use_mxfp4(False)`` returns to the float form."""
+        for layer in self._mxfp4_layers():
+            layer.quantize(on)
+        return self
+
+    def _mxfp4_layers(self):
+        return [m for m in self.modules() if isinstance(m, _SequenceConv)]
+
+    def _refresh_mxfp4(self, *unused):
+        for layer in self._mxfp4_layers():
+            if layer.mxfp4_codes is not None:
+                layer.quantize(True)
 
     # -- Keras checkpoint layout ------------------------------------------------------
     def load_keras_weights(self, w):
@@ -209,6 +261,7 @@ class FastSpeechAcousticModel(nn.Module):
             norm(self.post_net.bnorm1, "post_bn")
             self.post_net.bnorm1.running_mean.copy_(t(w["post_bn_mean"]))
             self.post_net.bnorm1.running_var.copy_(t(w["post_bn_var"]))
+        self._refresh_mxfp4()
         return self
 
 
