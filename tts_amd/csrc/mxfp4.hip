@@ -12,6 +12,8 @@
 //     codes  [row][group][64]      scales [group][row][4]
 // The scales are group-major because a matrix instruction wants, for one group, the scales of 32
 // consecutive rows in 32 lanes: that is one 128-byte line here and 32 lines in row order.
+#include <type_traits>
+
 #include "lowp.h"
 #include "status.h"
 
@@ -234,6 +236,275 @@ __global__ __launch_bounds__(WAVES * 64) void product_direct_kernel(Product p) {
 }
 
 
+// ---------------------------------------------------------------------------
+// the product, large: 256 x 256 tiles staged through LDS
+// ---------------------------------------------------------------------------
+constexpr int kTile = 256;         // rows of w and rows of x of a workgroup's tile
+constexpr int kTileThreads = 512;
+constexpr int kOperand = kTile * 128;  // bytes of one operand in a stage: 256 columns of every row
+
+// what a lane reads where a tap leaves its entry
+__device__ __align__(64) const uint32_t g_zeros[16] = {};
+
+// 16 bytes a lane from memory to LDS, lane after lane from the uniform address `dst` on.  Nothing
+// waits for these loads but the explicit s_waitcnt before the barrier that hands a stage over.  M0
+// holds the LDS address (one wait state before its use); the compiler uses that register for nothing
+// in these kernels.
+__device__ inline void to_lds(const uint8_t* base, uint32_t offset, uint32_t dst) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst), "v"(offset), "s"(base) : "memory");
+}
+__device__ inline void to_lds(const uint8_t* src, uint32_t dst) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(dst), "v"(src) : "memory");
+}
+
+// Workgroup ids go round the eight XCDs; each XCD gets a contiguous run of tiles, and a run walks
+// eight rows of tiles at a time, so that what an XCD's L2 holds is used by several of its CUs.
+struct Tile {
+    int m, n;
+};
+__device__ inline Tile tile_of(int id, int total, int m_tiles, int n_tiles) {
+    const int q = total >> 3, rem = total & 7, xcd = id & 7;
+    id = xcd * q + min(xcd, rem) + (id >> 3);
+    const int band = id / (8 * n_tiles), first = band * 8, high = min(m_tiles - first, 8);
+    id -= band * 8 * n_tiles;
+    return Tile{first + id % high, id / high};
+}
+
+struct Fragments {
+    i32x4 w[4], x[2];
+};
+
+// The wave's 32 rows (x) by 128 columns (w) of accumulators through its own 16 KB of LDS, so that
+// a row of y leaves in pieces of 16 bytes.  Lane l holds y[m = l % 32][8 * (e / 4) + 4 * (l / 32)
+// + e % 4] of every accumulator; piece q of row m lies at place q ^ m: reads and writes both
+// spread over the banks.
+template <typename T>
+__device__ inline void store_rows(const Product& p, const f32x16 (&acc)[4], uint8_t* lds, int m0, int n0, int lane) {
+    constexpr int kPieces = 128 * sizeof(T) / 16, kEach = 16 / sizeof(T);
+    const int r = lane & 31, half = lane >> 5;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            struct __attribute__((aligned(4 * sizeof(T)))) Four {
+                T v[4];
+            } four;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) four.v[e] = (T)(p.relu ? relu(acc[i][4 * q + e]) : acc[i][4 * q + e]);
+            const int at = (i * 32 + 8 * q + 4 * half) * sizeof(T);
+            *reinterpret_cast<Four*>(lds + r * (kPieces * 16) + (((at >> 4) ^ (r & (kPieces - 1))) << 4) + (at & 15)) = four;
+        }
+    constexpr int kRows = 64 / kPieces;  // rows that one instruction covers
+    const int piece = lane % kPieces, sub = lane / kPieces;
+    const int n = n0 + piece * kEach;
+#pragma unroll
+    for (int k = 0; k < 32; k += kRows) {
+        const int row = k + sub;
+        struct __attribute__((packed, aligned(sizeof(T)))) Piece {
+            T v[kEach];
+        };
+        const Piece v = *reinterpret_cast<const Piece*>(__builtin_assume_aligned(
+            lds + row * (kPieces * 16) + ((piece ^ (row & (kPieces - 1))) << 4), 16));
+        if (m0 + row >= p.rows) continue;
+        T* y = static_cast<T*>(p.y) + (int64_t)(m0 + row) * p.n + n;
+        if (n + kEach <= p.n) {
+            *reinterpret_cast<Piece*>(y) = v;
+        } else {
+#pragma unroll
+            for (int e = 0; e < kEach; ++e)
+                if (n + e < p.n) y[e] = v.v[e];
+        }
+    }
+}
+
+// Eight waves, each 128 rows of w by 64 of x (4 x 2 accumulators of 32 x 32).  A stage holds 256
+// columns of both operands: [row][8 pieces of 16 bytes], piece q of row r at place q ^ (r & 7), so
+// that the 32 rows of an operand spread over the banks.  There are two stages; the next one is on
+// its way to LDS while this one is multiplied, and the barrier between them stands before the last
+// of the four steps of a stage, whose products hide the first reads of the next stage.
+template <bool CONV>
+__global__ __launch_bounds__(kTileThreads) void product_tiled_kernel(Product p) {
+    __shared__ __align__(1024) uint8_t lds[4 * kOperand];
+    __shared__ __align__(16) float bias[kTile];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = lane & 31, half = lane >> 5;
+    const int m_tiles = (p.rows + kTile - 1) / kTile, n_tiles = (p.n + kTile - 1) / kTile;
+    const Tile tile = tile_of(blockIdx.x, gridDim.x, m_tiles, n_tiles);
+    const int n0 = tile.n * kTile, m0 = tile.m * kTile;
+    const int all = p.taps * p.groups;
+    const int chunks = (all + 1) / 2;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
+
+    // staging: load i of a wave fills rows i * 64 + wave * 8 .. + 7, lane l the place l % 8 of row l / 8
+    const int srow = wave * 8 + (lane >> 3);
+    const int piece = (lane & 7) ^ (lane >> 3);
+    const int row_bytes = all * kGroupBytes, x_bytes = p.groups * kGroupBytes;
+    const uint8_t* wbase = p.wc + (int64_t)n0 * row_bytes;
+    const uint8_t* xbase = p.xc + (int64_t)m0 * x_bytes;
+    uint32_t woff[4], xoff[4];
+    int xm[4], xt[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        woff[i] = min(i * 64 + srow, p.n - 1 - n0) * row_bytes + piece * 16;
+        const int m = min(i * 64 + srow, p.rows - 1 - m0);
+        xoff[i] = m * x_bytes + piece * 16;
+        xm[i] = m0 + m;
+        xt[i] = CONV ? xm[i] % p.T : 0;
+    }
+    int stap = 0, sgx = piece >> 2;  // CONV: tap and group of this lane's pieces in the next stage
+    if (CONV)
+        while (sgx >= p.groups) sgx -= p.groups, ++stap;
+    auto stage = [&](int c, uint32_t buffer) {
+        // behind the last group of an odd count both scales are 0, i.e. 2^-254 together, and the codes
+        // are those of the group before
+        const uint32_t back = 2 * c + 1 == all && piece >= 4 ? kGroupBytes : 0;
+        const uint32_t dst = lds0 + buffer + wave * 1024;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) to_lds(wbase + (int64_t)c * 128, woff[i] - back, dst + i * 8192);
+        if (CONV) {
+            const int shift = stap * p.dilation - p.left;
+            const bool have = stap < p.taps;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint8_t* src = p.xc + (int64_t)(xm[i] + shift) * x_bytes + sgx * kGroupBytes + (piece & 3) * 16;
+                const bool inside = have && (unsigned)(xt[i] + shift) < (unsigned)p.T;
+                to_lds(inside ? src : reinterpret_cast<const uint8_t*>(g_zeros), dst + kOperand + i * 8192);
+            }
+            sgx += 2;
+            while (sgx >= p.groups) sgx -= p.groups, ++stap;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) to_lds(xbase + (int64_t)c * 128, xoff[i] - back, dst + kOperand + i * 8192);
+        }
+    };
+
+    // scales of one stage: a dword for every 32 rows
+    const int nw = (wave & 1) * 128, mw = (wave >> 1) * 64;
+    int cn[4], cm[2], ct[2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) cn[i] = min(n0 + nw + i * 32 + r, p.n - 1);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        cm[j] = min(m0 + mw + j * 32 + r, p.rows - 1);
+        ct[j] = CONV ? cm[j] % p.T : 0;
+    }
+    int ctap = 0, cgx = half;
+    if (CONV)
+        while (cgx >= p.groups) cgx -= p.groups, ++ctap;
+    // A lane without a group, or whose row the tap leaves, loads some scale and has it masked later, where
+    // the stage is taken over: a select right here would wait for the loads, and with them for the stage.
+    struct Scales {
+        int w[4], x[2], wmask, xmask[2];
+    };
+    auto scales = [&](int c, Scales& s) {
+        const bool have = 2 * c + half < all;
+        s.wmask = s.xmask[0] = s.xmask[1] = have ? -1 : 0;
+        if (CONV) {
+            const int shift = ctap * p.dilation - p.left;
+            const int gx = have ? cgx : 0, tap = have ? ctap : 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                s.w[i] = reinterpret_cast<const int*>(p.ws)[((int64_t)gx * p.n + cn[i]) * p.taps + tap];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const bool inside = have && (unsigned)(ct[j] + shift) < (unsigned)p.T;
+                s.x[j] = reinterpret_cast<const int*>(p.xs)[(int64_t)gx * p.rows + (inside ? cm[j] + shift : cm[j])];
+                s.xmask[j] = inside ? -1 : 0;
+            }
+            cgx += 2;
+            while (cgx >= p.groups) cgx -= p.groups, ++ctap;
+        } else {
+            const uint8_t* wp = p.ws + (int64_t)c * 8 * p.n;
+            const uint8_t* xp = p.xs + (int64_t)c * 8 * p.rows;
+            const int h = have ? half : 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s.w[i] = *reinterpret_cast<const int*>(wp + (uint32_t)(h * p.n + cn[i]) * 4);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) s.x[j] = *reinterpret_cast<const int*>(xp + (uint32_t)(h * p.rows + cm[j]) * 4);
+        }
+    };
+
+    int ws[4], xs[2];
+    auto take = [&](const Scales& s) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ws[i] = s.w[i] & s.wmask;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) xs[j] = s.x[j] & s.xmask[j];
+    };
+    Scales ahead;
+    stage(0, 0);
+    scales(0, ahead);
+    take(ahead);
+    if (threadIdx.x < kTile)
+        bias[threadIdx.x] = p.bias && n0 + (int)threadIdx.x < p.n ? load_float(p.bias, p.bias_type, n0 + threadIdx.x) : 0.f;
+
+    uint32_t at[4];  // the pieces of the four steps in a row
+#pragma unroll
+    for (int k = 0; k < 4; ++k) at[k] = ((half * 4 + k) ^ (r & 7)) * 16;
+    const uint32_t wr = (nw + r) * 128, xr = kOperand + (mw + r) * 128;
+    auto fetch = [&](uint32_t buffer, int k, Fragments& f) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f.w[i] = *reinterpret_cast<const i32x4*>(lds + buffer + wr + at[k] + i * 4096);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) f.x[j] = *reinterpret_cast<const i32x4*>(lds + buffer + xr + at[k] + j * 4096);
+    };
+    f32x16 acc[4][2];
+    auto multiply = [&](auto S, const Fragments& f) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[i][j] = step<S>(f.w[i], f.x[j], ws[i], xs[j], acc[i][j]);
+    };
+
+    Fragments fa, fb;
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[i][0][e] = acc[i][1][e] = bias[nw + i * 32 + 8 * (e >> 2) + 4 * half + (e & 3)];
+    fetch(0, 0, fa);
+    uint32_t buffer = 0;
+    for (int c = 0; c < chunks; ++c) {
+        scales(min(c + 1, chunks - 1), ahead);
+        if (c + 1 < chunks) stage(c + 1, buffer ^ (2 * kOperand));
+        // a step's reads are issued before the products of the step before it
+        fetch(buffer, 1, fb);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(std::integral_constant<int, 0>{}, fa);
+        __builtin_amdgcn_sched_barrier(0);
+        fetch(buffer, 2, fa);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(std::integral_constant<int, 1>{}, fb);
+        __builtin_amdgcn_sched_barrier(0);
+        fetch(buffer, 3, fb);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(std::integral_constant<int, 2>{}, fa);
+        __builtin_amdgcn_sched_barrier(0);
+        // the next stage has arrived, and this one has been read, everywhere
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        buffer ^= 2 * kOperand;
+        fetch(buffer, 0, fa);  // after the last stage: whatever lies there, not used
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(std::integral_constant<int, 3>{}, fb);
+        __builtin_amdgcn_sched_barrier(0);
+        take(ahead);
+    }
+
+    // the last barrier stands behind every read of the stages: each wave takes 16 KB of them
+    uint8_t* own = lds + wave * 16384;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const f32x16(&part)[4] = {acc[0][j], acc[1][j], acc[2][j], acc[3][j]};
+        if (p.y_type == GLV_F32)
+            store_rows<float>(p, part, own, m0 + mw + j * 32, n0 + nw, lane);
+        else if (p.y_type == GLV_BF16)
+            store_rows<bf16>(p, part, own, m0 + mw + j * 32, n0 + nw, lane);
+        else
+            store_rows<f16>(p, part, own, m0 + mw + j * 32, n0 + nw, lane);
+        // one wave's reads and the next pass's writes of its own LDS stay in order in the LDS queue
+    }
+}
+
 // rows sixteen at a time by groups four at a time
 unsigned span_blocks(int rows, int groups) { return (unsigned)((rows + 15) / 16) * ((groups + 3) / 4); }
 
@@ -372,6 +643,14 @@ extern "C" int glv_mxfp4_product(const void* x_dev, const uint8_t* x_scales_dev,
         rc = quantise(x_dev, x_type, Rows{x_batch_stride, x_row_stride, rows}, p.rows, cols, codes, scales, st);
         if (rc != GLV_OK) return rc;
         p.xc = codes, p.xs = scales;
+    }
+    if (all * n_out >= 512 * 512) {
+        const unsigned tiles = (unsigned)(((all + kTile - 1) / kTile) * ((n_out + kTile - 1) / kTile));
+        if (taps > 1)
+            hipLaunchKernelGGL(product_tiled_kernel<true>, dim3(tiles), dim3(kTileThreads), 0, st, p);
+        else
+            hipLaunchKernelGGL(product_tiled_kernel<false>, dim3(tiles), dim3(kTileThreads), 0, st, p);
+        return launch_status("product_tiled_kernel");
     }
     const int64_t tiles = ((all + 31) / 32) * ((n_out + 31) / 32);
     if (tiles > INT32_MAX) return report(GLV_ERR_INVALID, "%s: rows x n_out too large for one call", what);
