@@ -6,6 +6,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 namespace glv {
 
 typedef __bf16 bf16;
@@ -18,32 +20,56 @@ typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef f16 f16x2 __attribute__((ext_vector_type(2)));
 
 template <typename T>
-struct __attribute__((packed, aligned(sizeof(T)))) Eight {
+struct Eight {
     T v[8];
 };
+
+// 16 bytes at the alignment of a T, in one access
+typedef int i32x4_at2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef int i32x4_at4 __attribute__((ext_vector_type(4), aligned(4)));
+template <typename T>
+using Unaligned = std::conditional_t<sizeof(T) == 2, i32x4_at2, i32x4_at4>;
+template <typename T>
+__device__ inline i32x4 load_16(const T* p) {
+    return *reinterpret_cast<const Unaligned<T>*>(p);
+}
+template <typename T>
+__device__ inline void store_16(T* p, i32x4 v) {
+    *reinterpret_cast<Unaligned<T>*>(p) = v;
+}
 
 // elements [0, valid) of p, zeros behind them; valid may be negative or beyond 8
 template <typename T>
 __device__ inline Eight<T> load_eight(const T* p, int valid) {
-    Eight<T> r;
     if (valid >= 8) {
-        r = *reinterpret_cast<const Eight<T>*>(p);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) r.v[i] = i < valid ? p[i] : T(0);
+        if constexpr (sizeof(T) == 2) {
+            return __builtin_bit_cast(Eight<T>, load_16(p));
+        } else {
+            const i32x4 a = load_16(p), b = load_16(p + 4);
+            return __builtin_bit_cast(Eight<T>, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+        }
     }
+    Eight<T> r;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r.v[i] = i < valid ? p[i] : T(0);
     return r;
 }
 
 template <typename T>
 __device__ inline void store_eight(T* p, const Eight<T>& r, int valid) {
     if (valid >= 8) {
-        *reinterpret_cast<Eight<T>*>(p) = r;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < valid) p[i] = r.v[i];
+        if constexpr (sizeof(T) == 2) {
+            store_16(p, __builtin_bit_cast(i32x4, r));
+        } else {
+            const i32x8 v = __builtin_bit_cast(i32x8, r);
+            store_16(p, __builtin_shufflevector(v, v, 0, 1, 2, 3));
+            store_16(p + 4, __builtin_shufflevector(v, v, 4, 5, 6, 7));
+        }
+        return;
     }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (i < valid) p[i] = r.v[i];
 }
 
 }  // namespace glv

@@ -151,7 +151,8 @@ struct Product {
     int rows, T, n;
     int taps, dilation, left;  // tap j of row t reads row t + j * dilation - left of its batch entry
     int groups;                // groups of one tap
-    int bias_type, y_type, relu;
+    int bias_type, y_type;
+    float least;               // 0: rectified; -infinity: as it is
 };
 
 __device__ inline float load_float(const void* p, int type, int64_t i) {
@@ -168,8 +169,8 @@ __device__ inline void store_float(void* p, int type, int64_t i, float v) {
         static_cast<f16*>(p)[i] = (f16)v;
 }
 
-// max(v, 0) that keeps a NaN
-__device__ inline float relu(float v) { return v < 0.f ? 0.f : v; }
+// max(v, least) that keeps a NaN: the rectifier with least = 0, nothing with -infinity
+__device__ inline float at_least(float v, float least) { return __builtin_elementwise_maximum(v, least); }
 
 __device__ inline i32x8 widen(i32x4 v) { return __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1); }
 
@@ -230,7 +231,7 @@ __global__ __launch_bounds__(WAVES * 64) void product_direct_kernel(Product p) {
 #pragma unroll
         for (int k = 1; k < WAVES; ++k) v += sums[k][mm][nn];
         if (p.bias) v += load_float(p.bias, p.bias_type, n0 + nn);
-        if (p.relu) v = relu(v);
+        v = at_least(v, p.least);
         store_float(p.y, p.y_type, (int64_t)(m0 + mm) * p.n + n0 + nn, v);
     }
 }
@@ -290,36 +291,45 @@ __device__ inline void store_rows(const Product& p, const f32x16 (&acc)[4], uint
                 T v[4];
             } four;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) four.v[e] = (T)(p.relu ? relu(acc[i][4 * q + e]) : acc[i][4 * q + e]);
+            for (int e = 0; e < 4; ++e) four.v[e] = (T)at_least(acc[i][4 * q + e], p.least);
             const int at = (i * 32 + 8 * q + 4 * half) * sizeof(T);
             *reinterpret_cast<Four*>(lds + r * (kPieces * 16) + (((at >> 4) ^ (r & (kPieces - 1))) << 4) + (at & 15)) = four;
         }
     constexpr int kRows = 64 / kPieces;  // rows that one instruction covers
     const int piece = lane % kPieces, sub = lane / kPieces;
     const int n = n0 + piece * kEach;
+    T* y = static_cast<T*>(p.y) + (int64_t)(m0 + sub) * p.n + n;
+    auto own = [&](int row) {
+        return *reinterpret_cast<const i32x4*>(lds + row * (kPieces * 16) + ((piece ^ (row & (kPieces - 1))) << 4));
+    };
+    if (m0 + 32 <= p.rows && n0 + 128 <= p.n) {
+        i32x4 v[32 / kRows];
 #pragma unroll
+        for (int k = 0; k < 32 / kRows; ++k) v[k] = own(k * kRows + sub);
+#pragma unroll
+        for (int k = 0; k < 32 / kRows; ++k) store_16(y + (int64_t)k * kRows * p.n, v[k]);
+        return;
+    }
+#pragma unroll 1
     for (int k = 0; k < 32; k += kRows) {
-        const int row = k + sub;
-        struct __attribute__((packed, aligned(sizeof(T)))) Piece {
+        if (m0 + k + sub >= p.rows) break;
+        struct {
             T v[kEach];
-        };
-        const Piece v = *reinterpret_cast<const Piece*>(__builtin_assume_aligned(
-            lds + row * (kPieces * 16) + ((piece ^ (row & (kPieces - 1))) << 4), 16));
-        if (m0 + row >= p.rows) continue;
-        T* y = static_cast<T*>(p.y) + (int64_t)(m0 + row) * p.n + n;
+        } v = __builtin_bit_cast(decltype(v), own(k + sub));
+        T* at = y + (int64_t)k * p.n;
         if (n + kEach <= p.n) {
-            *reinterpret_cast<Piece*>(y) = v;
+            store_16(at, __builtin_bit_cast(i32x4, v));
         } else {
 #pragma unroll
             for (int e = 0; e < kEach; ++e)
-                if (n + e < p.n) y[e] = v.v[e];
+                if (n + e < p.n) at[e] = v.v[e];
         }
     }
 }
 
 // Eight waves, each 128 rows of w by 64 of x (4 x 2 accumulators of 32 x 32).  A stage holds 256
-// columns of both operands: [row][8 pieces of 16 bytes], piece q of row r at place q ^ (r & 7), so
-// that the 32 rows of an operand spread over the banks.  There are two stages; the next one is on
+// columns of both operands: [row][8 pieces of 16 bytes], piece q of row r at place q ^ (r / 2 % 8):
+// sixteen lanes that read one piece of sixteen rows then touch each of the 64 banks once.  There are two stages; the next one is on
 // its way to LDS while this one is multiplied, and the barrier between them stands before the last
 // of the four steps of a stage, whose products hide the first reads of the next stage.
 template <bool CONV>
@@ -337,7 +347,7 @@ __global__ __launch_bounds__(kTileThreads) void product_tiled_kernel(Product p) 
 
     // staging: load i of a wave fills rows i * 64 + wave * 8 .. + 7, lane l the place l % 8 of row l / 8
     const int srow = wave * 8 + (lane >> 3);
-    const int piece = (lane & 7) ^ (lane >> 3);
+    const int piece = (lane & 7) ^ ((srow >> 1) & 7);
     const int row_bytes = all * kGroupBytes, x_bytes = p.groups * kGroupBytes;
     const uint8_t* wbase = p.wc + (int64_t)n0 * row_bytes;
     const uint8_t* xbase = p.xc + (int64_t)m0 * x_bytes;
@@ -440,7 +450,7 @@ __global__ __launch_bounds__(kTileThreads) void product_tiled_kernel(Product p) 
 
     uint32_t at[4];  // the pieces of the four steps in a row
 #pragma unroll
-    for (int k = 0; k < 4; ++k) at[k] = ((half * 4 + k) ^ (r & 7)) * 16;
+    for (int k = 0; k < 4; ++k) at[k] = ((half * 4 + k) ^ ((r >> 1) & 7)) * 16;
     const uint32_t wr = (nw + r) * 128, xr = kOperand + (mw + r) * 128;
     auto fetch = [&](uint32_t buffer, int k, Fragments& f) {
 #pragma unroll
@@ -626,7 +636,7 @@ extern "C" int glv_mxfp4_product(const void* x_dev, const uint8_t* x_scales_dev,
     p.taps = taps, p.dilation = dilation, p.left = dilation * (taps - 1) / 2;
     p.groups = (cols + kGroup - 1) / kGroup;
     p.wc = w_codes_dev, p.ws = w_scales_dev;
-    p.bias = bias_dev, p.bias_type = bias_type, p.relu = activation == GLV_ACT_RELU;
+    p.bias = bias_dev, p.bias_type = bias_type, p.least = activation == GLV_ACT_RELU ? 0.f : -__builtin_huge_valf();
     p.y = y_dev, p.y_type = y_type;
     if (x_type == GLV_MXFP4) {
         rc = check_quantised(what, x_dev, x_scales_dev);
