@@ -429,7 +429,7 @@ enum {
  * x / 2^s (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign bit) to the nearest, ties to the even code, 6
  * beyond 6.  A block that holds an infinity or a NaN has the scale byte 255 and reads as NaN.
  * With groups = ceil(cols / 128), columns beyond cols being zero:
- *   codes_dev   (rows, groups, 64) bytes, the even column in the low half; 16-byte aligned
+ *   codes_dev   (groups, rows, 64) bytes, the even column in the low half; 16-byte aligned
  *   scales_dev  (groups, rows, 4) bytes; 4-byte aligned
  * where rows counts batch * rows.  At most 2^24 rows and 2^18 columns.
  *   glv_mxfp4_quantize:   x_dev (batch, rows, cols), x[b, r, :] at b * batch_stride + r * row_stride.

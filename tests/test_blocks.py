@@ -31,7 +31,7 @@ def f64(t):
 
 def blocks_of(q):
     """codes (rows, blocks, 32) and scale bytes (rows, blocks) of an MXFP4Tensor's storage."""
-    codes = q.codes.cpu().numpy()
+    codes = q.codes.cpu().numpy().transpose(1, 0, 2)
     both = np.stack([codes & 15, codes >> 4], -1).reshape(codes.shape[0], -1, 32)
     scales = q.scales.cpu().numpy().transpose(1, 0, 2).reshape(codes.shape[0], -1)
     return both, scales
@@ -478,7 +478,7 @@ def test_other_streams_at_once_give_the_same_bits():
 # -- refusals -----------------------------------------------------------------------------
 def packed(shape, device="cpu"):
     rows, groups = int(np.prod(shape[:-1])), -(-shape[-1] // 128)
-    return MXFP4Tensor(shape, torch.zeros(rows, groups, 64, dtype=torch.uint8, device=device),
+    return MXFP4Tensor(shape, torch.zeros(groups, rows, 64, dtype=torch.uint8, device=device),
                        torch.zeros(groups, rows, 4, dtype=torch.uint8, device=device))
 
 
@@ -507,9 +507,9 @@ def test_refusals_without_gpu():
     with pytest.raises(ValueError, match="codes"):
         MXFP4Tensor((5, 40), torch.zeros(5, 64, dtype=torch.uint8), torch.zeros(1, 5, 4, dtype=torch.uint8))
     with pytest.raises(ValueError, match="scales"):
-        MXFP4Tensor((5, 40), torch.zeros(5, 1, 64, dtype=torch.uint8), torch.zeros(5, 1, 4, dtype=torch.uint8))
+        MXFP4Tensor((5, 40), torch.zeros(1, 5, 64, dtype=torch.uint8), torch.zeros(5, 1, 4, dtype=torch.uint8))
     with pytest.raises(ValueError, match="last dimension"):
-        MXFP4Tensor((5, 0), torch.zeros(5, 0, 64, dtype=torch.uint8), torch.zeros(0, 5, 4, dtype=torch.uint8))
+        MXFP4Tensor((5, 0), torch.zeros(0, 5, 64, dtype=torch.uint8), torch.zeros(0, 5, 4, dtype=torch.uint8))
     for name in ("MXFP4Tensor", "Norm", "block_norm", "mxfp4_conv1d", "mxfp4_linear", "mxfp4_quantize"):
         assert name in tts_amd.__all__
 

@@ -82,7 +82,7 @@ class MXFP4Tensor:
     and an element is a 4-bit code for 0, 0.5, 1, 1.5, 2, 3, 4 or 6 with a sign (E2M1).
 
     shape   of the tensor it stands for
-    codes   (rows, groups, 64) uint8, a group being 128 columns, two to a byte, the even one low
+    codes   (groups, rows, 64) uint8, a group being 128 columns, two to a byte, the even one low
     scales  (groups, rows, 4) uint8, biased exponents of the group's four blocks; 255 is a NaN block
     """
 
@@ -93,7 +93,7 @@ class MXFP4Tensor:
         if len(shape) < 1 or shape[-1] < 1:
             raise ValueError(f"an MXFP4 tensor needs a last dimension of at least 1, got {tuple(shape)}")
         rows, groups = shape[:-1].numel(), -(-shape[-1] // _GROUP)
-        for t, name, want in ((codes, "codes", (rows, groups, 64)), (scales, "scales", (groups, rows, 4))):
+        for t, name, want in ((codes, "codes", (groups, rows, 64)), (scales, "scales", (groups, rows, 4))):
             if t.dtype != torch.uint8 or tuple(t.shape) != want or not t.is_contiguous():
                 raise ValueError(f"{name} must be a contiguous uint8 tensor of shape {want}, got {t.dtype} "
                                  f"{tuple(t.shape)}")
@@ -117,7 +117,7 @@ class MXFP4Tensor:
         out = torch.empty(self.shape, dtype=dtype, device=self.device)
         with _on(self.device) as stream:
             _lib.check(_lib.load().glv_mxfp4_dequantize(self.codes.data_ptr(), self.scales.data_ptr(),
-                                                        self.codes.shape[0], self.shape[-1], _TYPES[dtype],
+                                                        self.codes.shape[1], self.shape[-1], _TYPES[dtype],
                                                         out.data_ptr(), stream))
         return out
 
@@ -135,7 +135,7 @@ def mxfp4_quantize(x):
         raise ValueError(f"x must have a last dimension of at least 1, got {tuple(x.shape)}")
     v = _rows(x)
     rows, groups = v.shape[0] * v.shape[1], -(-v.shape[2] // _GROUP)
-    codes = torch.empty((rows, groups, 64), dtype=torch.uint8, device=x.device)
+    codes = torch.empty((groups, rows, 64), dtype=torch.uint8, device=x.device)
     scales = torch.empty((groups, rows, 4), dtype=torch.uint8, device=x.device)
     with _on(x.device) as stream:
         _lib.check(_lib.load().glv_mxfp4_quantize(v.data_ptr(), _TYPES[x.dtype], v.shape[0], v.shape[1], v.shape[2],
@@ -155,7 +155,7 @@ def _product(x, weight, bias, taps, dilation, activation, out_dtype):
             raise ValueError(f"x is on {x.device}, not on {device}")
         kind, data, scales = _MXFP4, x.codes.data_ptr(), x.scales.data_ptr()
         rows = x.shape[-2] if len(x.shape) > 1 else 1
-        batch = x.codes.shape[0] // rows if rows else 0
+        batch = x.codes.shape[1] // rows if rows else 0
         strides = (0, 0)
     else:
         _check(x, "x", device)

@@ -8,10 +8,11 @@
 // A block with an infinity or a NaN has no such scale: its byte is 255 (NaN) and its codes are 0.
 //
 // Layout.  A group is 128 columns: 64 bytes of codes (low nibble = even column) and one dword of
-// scales.  Rows are padded with zeros to whole groups.
-//     codes  [row][group][64]      scales [group][row][4]
-// The scales are group-major because a matrix instruction wants, for one group, the scales of 32
-// consecutive rows in 32 lanes: that is one 128-byte line here and 32 lines in row order.
+// scales.  Rows are padded with zeros to whole groups, and both arrays are group-major:
+//     codes  [group][row][64]      scales [group][row][4]
+// A product walks the groups and takes, of each, a run of rows: that is one run of memory here.  (In
+// row order the codes of a stage are pieces of 64 bytes, and the scales that a matrix instruction
+// wants in 32 lanes lie in 32 lines.)
 #include <type_traits>
 
 #include "lowp.h"
@@ -107,7 +108,7 @@ __global__ __launch_bounds__(256) void quantise_kernel(const T* __restrict__ x, 
         const int col = g * kGroup + piece * 8;
         int byte;
         const uint32_t c = quantise_eight(load_eight(src + col, cols - col), &byte);
-        reinterpret_cast<uint32_t*>(codes)[((int64_t)row * groups + g) * 16 + piece] = c;
+        reinterpret_cast<uint32_t*>(codes)[((int64_t)g * rows + row) * 16 + piece] = c;
         if ((piece & 3) == 0) scales[((int64_t)g * rows + row) * 4 + (piece >> 2)] = (uint8_t)byte;
     }
 }
@@ -124,7 +125,7 @@ __global__ __launch_bounds__(256) void dequantise_kernel(const uint8_t* __restri
     for (int g = first; g < min(groups, first + 4); ++g) {
         const int col = g * kGroup + piece * 8;
         if (col >= cols) return;
-        const uint32_t c = reinterpret_cast<const uint32_t*>(codes)[((int64_t)row * groups + g) * 16 + piece];
+        const uint32_t c = reinterpret_cast<const uint32_t*>(codes)[((int64_t)g * rows + row) * 16 + piece];
         const uint32_t s = scales[((int64_t)g * rows + row) * 4 + (piece >> 2)];
         // 2^-127 is a subnormal float, 255 a NaN; the codes' own values come out of the conversion
         // exactly, and the product of the two is exact wherever T can hold it
@@ -205,16 +206,18 @@ __global__ __launch_bounds__(WAVES * 64) void product_direct_kernel(Product p) {
         i32x4 w[4] = {}, x[4] = {};
         int wscale = 0, xscale = 0;
         if (g < all) {
-            const i32x4* wp = reinterpret_cast<const i32x4*>(p.wc + ((int64_t)n * all + g) * kGroupBytes);
+            const int64_t row = ((int64_t)gx * p.n + n) * p.taps + tap;
+            const i32x4* wp = reinterpret_cast<const i32x4*>(p.wc + row * kGroupBytes);
 #pragma unroll
             for (int i = 0; i < 4; ++i) w[i] = wp[i];
-            wscale = reinterpret_cast<const int*>(p.ws)[((int64_t)gx * p.n + n) * p.taps + tap];
+            wscale = reinterpret_cast<const int*>(p.ws)[row];
         }
         if (have) {  // a tap outside the entry meets zeros
-            const i32x4* xp = reinterpret_cast<const i32x4*>(p.xc + ((int64_t)(m + shift) * p.groups + gx) * kGroupBytes);
+            const int64_t row = (int64_t)gx * p.rows + m + shift;
+            const i32x4* xp = reinterpret_cast<const i32x4*>(p.xc + row * kGroupBytes);
 #pragma unroll
             for (int i = 0; i < 4; ++i) x[i] = xp[i];
-            xscale = reinterpret_cast<const int*>(p.xs)[(int64_t)gx * p.rows + m + shift];
+            xscale = reinterpret_cast<const int*>(p.xs)[row];
         }
         acc = step<0>(w[0], x[0], wscale, xscale, acc);
         acc = step<1>(w[1], x[1], wscale, xscale, acc);
@@ -242,12 +245,14 @@ __global__ __launch_bounds__(WAVES * 64) void product_direct_kernel(Product p) {
 // ---------------------------------------------------------------------------
 constexpr int kTile = 256;         // rows of w and rows of x of a workgroup's tile
 constexpr int kTileThreads = 512;
-constexpr int kOperand = kTile * 128;  // bytes of one operand in a stage: 256 columns of every row
+constexpr int kOperand = kTile * kGroupBytes;          // codes of one operand in a stage: one group of every row
+constexpr int kStage = 2 * kOperand + 2 * kTile * 4;   // both operands' codes and scales
+constexpr int kStages = 4;
 
 // what a lane reads where a tap leaves its entry
 __device__ __align__(64) const uint32_t g_zeros[16] = {};
 
-// 16 bytes a lane from memory to LDS, lane after lane from the uniform address `dst` on.  Nothing
+// 16 (or 4) bytes a lane from memory to LDS, lane after lane from the uniform address `dst` on.  Nothing
 // waits for these loads but the explicit s_waitcnt before the barrier that hands a stage over.  M0
 // holds the LDS address (one wait state before its use); the compiler uses that register for nothing
 // in these kernels.
@@ -271,6 +276,13 @@ __device__ inline Tile tile_of(int id, int total, int m_tiles, int n_tiles) {
     return Tile{first + id % high, id / high};
 }
 
+__device__ inline void dword_to_lds(const uint8_t* base, uint32_t offset, uint32_t dst) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(dst), "v"(offset), "s"(base) : "memory");
+}
+__device__ inline void dword_to_lds(const uint8_t* src, uint32_t dst) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(dst), "v"(src) : "memory");
+}
+
 struct Fragments {
     i32x4 w[4], x[2];
 };
@@ -280,7 +292,7 @@ struct Fragments {
 // + e % 4] of every accumulator; piece q of row m lies at place q ^ m: reads and writes both
 // spread over the banks.
 template <typename T>
-__device__ inline void store_rows(const Product& p, const f32x16 (&acc)[4], uint8_t* lds, int m0, int n0, int lane) {
+__device__ inline void store_rows(const Product& p, const f32x16 (&acc)[4], const float* bias, uint8_t* lds, int m0, int n0, int lane) {
     constexpr int kPieces = 128 * sizeof(T) / 16, kEach = 16 / sizeof(T);
     const int r = lane & 31, half = lane >> 5;
 #pragma unroll
@@ -291,7 +303,8 @@ __device__ inline void store_rows(const Product& p, const f32x16 (&acc)[4], uint
                 T v[4];
             } four;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) four.v[e] = (T)at_least(acc[i][4 * q + e], p.least);
+            for (int e = 0; e < 4; ++e)
+                four.v[e] = (T)at_least(acc[i][4 * q + e] + bias[i * 32 + 8 * q + 4 * half + e], p.least);
             const int at = (i * 32 + 8 * q + 4 * half) * sizeof(T);
             *reinterpret_cast<Four*>(lds + r * (kPieces * 16) + (((at >> 4) ^ (r & (kPieces - 1))) << 4) + (at & 15)) = four;
         }
@@ -327,14 +340,14 @@ __device__ inline void store_rows(const Product& p, const f32x16 (&acc)[4], uint
     }
 }
 
-// Eight waves, each 128 rows of w by 64 of x (4 x 2 accumulators of 32 x 32).  A stage holds 256
-// columns of both operands: [row][8 pieces of 16 bytes], piece q of row r at place q ^ (r / 2 % 8):
-// sixteen lanes that read one piece of sixteen rows then touch each of the 64 banks once.  There are two stages; the next one is on
-// its way to LDS while this one is multiplied, and the barrier between them stands before the last
-// of the four steps of a stage, whose products hide the first reads of the next stage.
+// Eight waves, each 128 rows of w by 64 of x (4 x 2 accumulators of 32 x 32).  A stage holds one
+// group of both operands: [row][4 pieces of 16 bytes], piece q of row r at place q ^ (r / 4 % 4):
+// sixteen lanes that read one piece of sixteen rows then touch each of the 64 banks once.  Of the
+// four stages one is multiplied while three are on their way.  A stage is two steps; the barrier
+// stands between them, so that the products of the second hide the first reads of the next stage.
 template <bool CONV>
 __global__ __launch_bounds__(kTileThreads) void product_tiled_kernel(Product p) {
-    __shared__ __align__(1024) uint8_t lds[4 * kOperand];
+    __shared__ __align__(1024) uint8_t lds[kStages * kStage];
     __shared__ __align__(16) float bias[kTile];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 31, half = lane >> 5;
@@ -342,175 +355,186 @@ __global__ __launch_bounds__(kTileThreads) void product_tiled_kernel(Product p) 
     const Tile tile = tile_of(blockIdx.x, gridDim.x, m_tiles, n_tiles);
     const int n0 = tile.n * kTile, m0 = tile.m * kTile;
     const int all = p.taps * p.groups;
-    const int chunks = (all + 1) / 2;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
 
-    // staging: load i of a wave fills rows i * 64 + wave * 8 .. + 7, lane l the place l % 8 of row l / 8
-    const int srow = wave * 8 + (lane >> 3);
-    const int piece = (lane & 7) ^ ((srow >> 1) & 7);
-    const int row_bytes = all * kGroupBytes, x_bytes = p.groups * kGroupBytes;
-    const uint8_t* wbase = p.wc + (int64_t)n0 * row_bytes;
-    const uint8_t* xbase = p.xc + (int64_t)m0 * x_bytes;
-    uint32_t woff[4], xoff[4];
-    int xm[4], xt[4];
+    // Five loads a wave and stage: two of w and two of x (load i fills rows i * 128 + wave * 16 .. + 15, lane l
+    // the place l % 4 of row l / 4), one of scales (64 rows of w or x).  Rows behind the last repeat it.
+    const int srow = wave * 16 + (lane >> 2);
+    const int place = ((lane & 3) ^ (lane >> 4)) * 16;
+    uint32_t woff[2], xoff[2], soff;
+    int xt[2], st = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        woff[i] = min(i * 64 + srow, p.n - 1 - n0) * row_bytes + piece * 16;
-        const int m = min(i * 64 + srow, p.rows - 1 - m0);
-        xoff[i] = m * x_bytes + piece * 16;
-        xm[i] = m0 + m;
-        xt[i] = CONV ? xm[i] % p.T : 0;
+    for (int i = 0; i < 2; ++i) {
+        woff[i] = min(n0 + i * 128 + srow, p.n - 1) * p.taps * kGroupBytes + place;
+        const int m = min(m0 + i * 128 + srow, p.rows - 1);
+        xoff[i] = m * kGroupBytes + place;
+        xt[i] = CONV ? m % p.T : 0;
     }
-    int stap = 0, sgx = piece >> 2;  // CONV: tap and group of this lane's pieces in the next stage
-    if (CONV)
-        while (sgx >= p.groups) sgx -= p.groups, ++stap;
-    auto stage = [&](int c, uint32_t buffer) {
-        // behind the last group of an odd count both scales are 0, i.e. 2^-254 together, and the codes
-        // are those of the group before
-        const uint32_t back = 2 * c + 1 == all && piece >= 4 ? kGroupBytes : 0;
-        const uint32_t dst = lds0 + buffer + wave * 1024;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) to_lds(wbase + (int64_t)c * 128, woff[i] - back, dst + i * 8192);
-        if (CONV) {
-            const int shift = stap * p.dilation - p.left;
-            const bool have = stap < p.taps;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint8_t* src = p.xc + (int64_t)(xm[i] + shift) * x_bytes + sgx * kGroupBytes + (piece & 3) * 16;
-                const bool inside = have && (unsigned)(xt[i] + shift) < (unsigned)p.T;
-                to_lds(inside ? src : reinterpret_cast<const uint8_t*>(g_zeros), dst + kOperand + i * 8192);
+    const bool wscales = wave < 4;
+    if (wscales) {
+        soff = min(n0 + (int)threadIdx.x, p.n - 1) * p.taps * 4;
+    } else {
+        const int m = min(m0 + (int)threadIdx.x - kTile, p.rows - 1);
+        soff = m * 4;
+        st = CONV ? m % p.T : 0;
+    }
+    // the next stage to be loaded: tap, group, and where their rows begin (counted in rows)
+    int tap = 0, gx = 0;
+    int64_t wrow = 0, xrow = 0;
+    const int64_t wstep = (int64_t)p.n * p.taps, sstep = wscales ? wstep : p.rows;
+    const uint8_t* sbase = wscales ? p.ws : p.xs;
+    int64_t srow4 = 0;
+    // loads 0 and 1: w, 2 and 3: x, 4: scales, and on to the next group; no branches
+    auto stage_part = [&](int slot, auto part) {
+        constexpr int i = part;
+        const uint32_t dst = lds0 + slot * kStage;
+        const int shift = CONV ? tap * p.dilation - p.left : 0;
+        const uint8_t* zeros = reinterpret_cast<const uint8_t*>(g_zeros);
+        if constexpr (i < 2) {
+            to_lds(p.wc + wrow * kGroupBytes, woff[i], dst + i * 8192 + wave * 1024);
+        } else if constexpr (i < 4) {
+            const uint8_t* xbase = p.xc + xrow * kGroupBytes;
+            const uint32_t to = dst + kOperand + (i - 2) * 8192 + wave * 1024;
+            if (CONV) {
+                const bool inside = (unsigned)(xt[i - 2] + shift) < (unsigned)p.T;
+                to_lds(inside ? xbase + (int64_t)xoff[i - 2] + (int64_t)shift * kGroupBytes : zeros, to);
+            } else {
+                to_lds(xbase, xoff[i - 2], to);
             }
-            sgx += 2;
-            while (sgx >= p.groups) sgx -= p.groups, ++stap;
         } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) to_lds(xbase + (int64_t)c * 128, xoff[i] - back, dst + kOperand + i * 8192);
+            const uint32_t to = dst + 2 * kOperand + wave * 256;
+            if (CONV) {
+                // of w the tap's own scales; of x those of the shifted row
+                const int own = wscales ? tap : shift;
+                const bool inside = wscales | ((unsigned)(st + shift) < (unsigned)p.T);
+                dword_to_lds(inside ? sbase + srow4 + (int64_t)soff + (int64_t)own * 4 : zeros, to);
+                const bool last = ++gx == p.groups;
+                tap += last;
+                gx = last ? 0 : gx;
+                wrow = last ? tap : wrow + wstep;
+                xrow = last ? 0 : xrow + p.rows;
+                srow4 = last ? 0 : srow4 + sstep * 4;
+            } else {
+                dword_to_lds(sbase + srow4, soff, to);
+                wrow += wstep;
+                xrow += p.rows;
+                srow4 += sstep * 4;
+            }
         }
     };
+    auto stage = [&](int slot) {
+        stage_part(slot, std::integral_constant<int, 0>{});
+        stage_part(slot, std::integral_constant<int, 1>{});
+        stage_part(slot, std::integral_constant<int, 2>{});
+        stage_part(slot, std::integral_constant<int, 3>{});
+        stage_part(slot, std::integral_constant<int, 4>{});
+    };
 
-    // scales of one stage: a dword for every 32 rows
+#pragma unroll
+    for (int c = 0; c < kStages; ++c)
+        if (c < all) stage(c);
+    // asked for here, used behind the loop: no wait of its own
+    float own_bias = 0.f;
+    if (p.bias && n0 + (int)threadIdx.x < p.n && threadIdx.x < kTile) own_bias = load_float(p.bias, p.bias_type, n0 + threadIdx.x);
+
     const int nw = (wave & 1) * 128, mw = (wave >> 1) * 64;
-    int cn[4], cm[2], ct[2];
+    // lane l takes, of row l % 32, the blocks 2 * (l / 32) and + 1 in the two steps
+    uint32_t at[2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) cn[i] = min(n0 + nw + i * 32 + r, p.n - 1);
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        cm[j] = min(m0 + mw + j * 32 + r, p.rows - 1);
-        ct[j] = CONV ? cm[j] % p.T : 0;
-    }
-    int ctap = 0, cgx = half;
-    if (CONV)
-        while (cgx >= p.groups) cgx -= p.groups, ++ctap;
-    // A lane without a group, or whose row the tap leaves, loads some scale and has it masked later, where
-    // the stage is taken over: a select right here would wait for the loads, and with them for the stage.
-    struct Scales {
-        int w[4], x[2], wmask, xmask[2];
+    for (int k = 0; k < 2; ++k) at[k] = ((half * 2 + k) ^ ((r >> 2) & 3)) * 16;
+    const uint32_t wr = (nw + r) * kGroupBytes, xr = kOperand + (mw + r) * kGroupBytes;
+    auto fetch_w = [&](uint32_t base, int k, int i, Fragments& f) {
+        f.w[i] = *reinterpret_cast<const i32x4*>(lds + base + wr + at[k] + i * 32 * kGroupBytes);
     };
-    auto scales = [&](int c, Scales& s) {
-        const bool have = 2 * c + half < all;
-        s.wmask = s.xmask[0] = s.xmask[1] = have ? -1 : 0;
-        if (CONV) {
-            const int shift = ctap * p.dilation - p.left;
-            const int gx = have ? cgx : 0, tap = have ? ctap : 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                s.w[i] = reinterpret_cast<const int*>(p.ws)[((int64_t)gx * p.n + cn[i]) * p.taps + tap];
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const bool inside = have && (unsigned)(ct[j] + shift) < (unsigned)p.T;
-                s.x[j] = reinterpret_cast<const int*>(p.xs)[(int64_t)gx * p.rows + (inside ? cm[j] + shift : cm[j])];
-                s.xmask[j] = inside ? -1 : 0;
-            }
-            cgx += 2;
-            while (cgx >= p.groups) cgx -= p.groups, ++ctap;
-        } else {
-            const uint8_t* wp = p.ws + (int64_t)c * 8 * p.n;
-            const uint8_t* xp = p.xs + (int64_t)c * 8 * p.rows;
-            const int h = have ? half : 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s.w[i] = *reinterpret_cast<const int*>(wp + (uint32_t)(h * p.n + cn[i]) * 4);
-#pragma unroll
-            for (int j = 0; j < 2; ++j) s.x[j] = *reinterpret_cast<const int*>(xp + (uint32_t)(h * p.rows + cm[j]) * 4);
-        }
+    auto fetch_x = [&](uint32_t base, int k, int j, Fragments& f) {
+        f.x[j] = *reinterpret_cast<const i32x4*>(lds + base + xr + at[k] + j * 32 * kGroupBytes);
     };
-
     int ws[4], xs[2];
-    auto take = [&](const Scales& s) {
+    const uint32_t wsr = 2 * kOperand + (nw + r) * 4, xsr = 2 * kOperand + kTile * 4 + (mw + r) * 4;
+    auto fetch_scales = [&](uint32_t base, int (&w)[4], int (&x)[2]) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) ws[i] = s.w[i] & s.wmask;
+        for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const int*>(lds + base + wsr + i * 128);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) xs[j] = s.x[j] & s.xmask[j];
+        for (int j = 0; j < 2; ++j) x[j] = *reinterpret_cast<const int*>(lds + base + xsr + j * 128);
     };
-    Scales ahead;
-    stage(0, 0);
-    scales(0, ahead);
-    take(ahead);
-    if (threadIdx.x < kTile)
-        bias[threadIdx.x] = p.bias && n0 + (int)threadIdx.x < p.n ? load_float(p.bias, p.bias_type, n0 + threadIdx.x) : 0.f;
-
-    uint32_t at[4];  // the pieces of the four steps in a row
-#pragma unroll
-    for (int k = 0; k < 4; ++k) at[k] = ((half * 4 + k) ^ ((r >> 1) & 7)) * 16;
-    const uint32_t wr = (nw + r) * 128, xr = kOperand + (mw + r) * 128;
-    auto fetch = [&](uint32_t buffer, int k, Fragments& f) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) f.w[i] = *reinterpret_cast<const i32x4*>(lds + buffer + wr + at[k] + i * 4096);
-#pragma unroll
-        for (int j = 0; j < 2; ++j) f.x[j] = *reinterpret_cast<const i32x4*>(lds + buffer + xr + at[k] + j * 4096);
-    };
-    f32x16 acc[4][2];
-    auto multiply = [&](auto S, const Fragments& f) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[i][j] = step<S>(f.w[i], f.x[j], ws[i], xs[j], acc[i][j]);
+    f32x16 acc[4][2] = {};
+    auto multiply = [&](auto S, int i, int j, const Fragments& f) {
+        acc[i][j] = step<S>(f.w[i], f.x[j], ws[i], xs[j], acc[i][j]);
     };
 
     Fragments fa, fb;
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (all >= kStages)
+        asm volatile("s_waitcnt vmcnt(15)\n\ts_barrier" ::: "memory");
+    else
+        asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+    int wnext[4], xnext[2];
+    for (int i = 0; i < 4; ++i) fetch_w(0, 0, i, fa);
+    for (int j = 0; j < 2; ++j) fetch_x(0, 0, j, fa);
+    fetch_scales(0, wnext, xnext);
+    uint32_t base = 0;
+    auto chunk = [&](int c, auto more) {
+        // the dword holds the group's four blocks: this lane's two go to the front
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i) ws[i] = (uint32_t)wnext[i] >> (half * 16);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) acc[i][0][e] = acc[i][1][e] = bias[nw + i * 32 + 8 * (e >> 2) + 4 * half + (e & 3)];
-    fetch(0, 0, fa);
-    uint32_t buffer = 0;
-    for (int c = 0; c < chunks; ++c) {
-        scales(min(c + 1, chunks - 1), ahead);
-        if (c + 1 < chunks) stage(c + 1, buffer ^ (2 * kOperand));
-        // a step's reads are issued before the products of the step before it
-        fetch(buffer, 1, fb);
-        __builtin_amdgcn_sched_barrier(0);
-        multiply(std::integral_constant<int, 0>{}, fa);
-        __builtin_amdgcn_sched_barrier(0);
-        fetch(buffer, 2, fa);
-        __builtin_amdgcn_sched_barrier(0);
-        multiply(std::integral_constant<int, 1>{}, fb);
-        __builtin_amdgcn_sched_barrier(0);
-        fetch(buffer, 3, fb);
-        __builtin_amdgcn_sched_barrier(0);
-        multiply(std::integral_constant<int, 2>{}, fa);
-        __builtin_amdgcn_sched_barrier(0);
-        // the next stage has arrived, and this one has been read, everywhere
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        buffer ^= 2 * kOperand;
-        fetch(buffer, 0, fa);  // after the last stage: whatever lies there, not used
-        __builtin_amdgcn_sched_barrier(0);
-        multiply(std::integral_constant<int, 3>{}, fb);
-        __builtin_amdgcn_sched_barrier(0);
-        take(ahead);
-    }
+        for (int j = 0; j < 2; ++j) xs[j] = (uint32_t)xnext[j] >> (half * 16);
+        // What is not a product is issued in the shadow of one (32 cycles each): both waves of a SIMD come
+        // through here together, so nothing else would keep the matrix core busy meanwhile.
+        constexpr std::integral_constant<int, 0> first{};
+        constexpr std::integral_constant<int, 1> second{};
+#define THEN __builtin_amdgcn_sched_barrier(0)
+        THEN;
+        multiply(first, 0, 0, fa), THEN, fetch_w(base, 1, 0, fb), fetch_x(base, 1, 0, fb), THEN;
+        multiply(first, 1, 0, fa), THEN, fetch_w(base, 1, 1, fb), fetch_w(base, 1, 2, fb), THEN;
+        multiply(first, 2, 0, fa), THEN, fetch_w(base, 1, 3, fb), fetch_x(base, 1, 1, fb), THEN;
+        multiply(first, 3, 0, fa), multiply(first, 0, 1, fa), multiply(first, 1, 1, fa), THEN;
+        multiply(first, 2, 1, fa), multiply(first, 3, 1, fa), THEN;
+        multiply(second, 0, 0, fb), multiply(second, 1, 0, fb), THEN;
+        // the next stage has arrived (two more may be under way), and this one has been read, everywhere
+        if constexpr (more)
+            asm volatile("s_waitcnt vmcnt(10) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        else
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        const int slot = c & (kStages - 1);
+        base = ((c + 1) & (kStages - 1)) * kStage;
+        // after the last stage these reads bring whatever lies there, and nothing uses it
+        fetch_w(base, 0, 0, fa), fetch_x(base, 0, 0, fa), THEN;
+        multiply(second, 2, 0, fb), THEN, fetch_w(base, 0, 1, fa), fetch_w(base, 0, 2, fa), THEN;
+        multiply(second, 3, 0, fb), THEN, fetch_w(base, 0, 3, fa), fetch_x(base, 0, 1, fa), THEN;
+        multiply(second, 0, 1, fb), THEN, fetch_scales(base, wnext, xnext), THEN;
+        multiply(second, 1, 1, fb), THEN;
+        if constexpr (more) {
+            stage_part(slot, std::integral_constant<int, 0>{});
+            stage_part(slot, std::integral_constant<int, 1>{});
+        }
+        THEN, multiply(second, 2, 1, fb), THEN;
+        if constexpr (more) {
+            stage_part(slot, std::integral_constant<int, 2>{});
+            stage_part(slot, std::integral_constant<int, 3>{});
+        }
+        THEN, multiply(second, 3, 1, fb), THEN;
+        if constexpr (more) stage_part(slot, std::integral_constant<int, 4>{});
+        THEN;
+#undef THEN
+    };
+    // two loops, each without a branch inside: products stay on their side of the barrier
+    int c = 0;
+    for (; c < all - kStages; ++c) chunk(c, std::true_type{});
+    for (; c < all; ++c) chunk(c, std::false_type{});
 
-    // the last barrier stands behind every read of the stages: each wave takes 16 KB of them
+    if (threadIdx.x < kTile) bias[threadIdx.x] = own_bias;
+    __syncthreads();
+    // every read of the stages lies behind: each wave takes 16 KB of them
     uint8_t* own = lds + wave * 16384;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         const f32x16(&part)[4] = {acc[0][j], acc[1][j], acc[2][j], acc[3][j]};
         if (p.y_type == GLV_F32)
-            store_rows<float>(p, part, own, m0 + mw + j * 32, n0 + nw, lane);
+            store_rows<float>(p, part, bias + nw, own, m0 + mw + j * 32, n0 + nw, lane);
         else if (p.y_type == GLV_BF16)
-            store_rows<bf16>(p, part, own, m0 + mw + j * 32, n0 + nw, lane);
+            store_rows<bf16>(p, part, bias + nw, own, m0 + mw + j * 32, n0 + nw, lane);
         else
-            store_rows<f16>(p, part, own, m0 + mw + j * 32, n0 + nw, lane);
+            store_rows<f16>(p, part, bias + nw, own, m0 + mw + j * 32, n0 + nw, lane);
         // one wave's reads and the next pass's writes of its own LDS stay in order in the LDS queue
     }
 }
