@@ -194,43 +194,59 @@ def test_conv1d(dtype, batch, time, c, n, taps, dilation):
 
 
 def gathered(x, taps, dilation):
-    """(B, T, C) -> (B * T, taps * C) float64, zeros outside."""
+    """(B, T, C) -> (B * T, taps * C), zeros outside."""
     b, t, c = x.shape
     left = dilation * (taps - 1) // 2
-    padded = np.zeros((b, t + dilation * (taps - 1), c))
+    padded = x.new_zeros((b, t + dilation * (taps - 1), c))
     padded[:, left:left + t] = x
-    return np.concatenate([padded[:, j * dilation:j * dilation + t] for j in range(taps)], -1).reshape(b * t, -1)
+    return torch.cat([padded[:, j * dilation:j * dilation + t] for j in range(taps)], -1).reshape(b * t, -1)
+
+
+def check_product_on_device(got, rows, weight, bias, relu):
+    """check_product with the float64 product formed on the device: rows (M, K), weight (N, K) float64."""
+    dtype, k = got.dtype, rows.shape[1]
+    wt = weight.t().contiguous()
+    want, size = torch.mm(rows, wt), torch.mm(rows.abs(), wt.abs())
+    if bias is not None:
+        want, size = want + bias.double(), size + bias.double().abs()
+    if relu:
+        want = want.clamp_min(0)
+    slack = (k + 1) * 2.0 ** -23 * size
+    bound = slack + half_step(dtype) * (want.abs() + slack) + (2.0 ** -25 if dtype == torch.float16 else 1e-38)
+    err = (got.double().reshape(want.shape) - want).abs()
+    assert (err <= bound).all(), f"worst {(err / bound).max().item():.3g} of the bound"
+
+
+# odd edges of every tiling: a few hundred rows and columns, more than 3 M outputs with few and with many sums
+LARGE = [(512, 512, 1), (1000, 300, 129), (255, 2049, 385), (4100, 70, 640), (30000, 9, 200), (2000, 257, 2300),
+         (513, 6200, 100), (3100, 1100, 385), (12300, 257, 1001), (16500, 1030, 2100), (700, 8200, 1500)]
 
 
 @gpu
-@pytest.mark.parametrize("m,n,k", [(512, 512, 1), (513, 520, 128), (1000, 300, 129), (260, 1100, 256), (255, 2049, 385),
-                                   (4100, 70, 640), (30000, 9, 200), (2000, 257, 2300)])
+@pytest.mark.parametrize("m,n,k", LARGE)
 @pytest.mark.parametrize("dtype", TYPES)
 def test_linear_of_many_rows_and_columns(dtype, m, n, k):
     rng = np.random.default_rng(m + n + k)
-    x, w = draw(rng, m, k, dtype=dtype), draw(rng, n, k, scale=k ** -0.5)
+    x, w, bias = draw(rng, m, k, dtype=dtype), draw(rng, n, k, scale=k ** -0.5), draw(rng, n)
     x[m // 2] = 0
-    bias = draw(rng, n)
     q, xq = mxfp4_quantize(w), mxfp4_quantize(x)
-    xv, wv, b = f64(xq.dequantize()), f64(q.dequantize()), f64(bias)
-    want, size = xv @ wv.T, np.abs(xv) @ np.abs(wv).T
-    check_product(mxfp4_linear(x, q), want, size, k, dtype)
-    check_product(mxfp4_linear(xq, q, bias, activation="relu"), np.maximum(want + b, 0), size + np.abs(b), k, torch.float32)
+    xv, wv = xq.dequantize().double(), q.dequantize().double()
+    check_product_on_device(mxfp4_linear(x, q), xv, wv, None, False)
+    check_product_on_device(mxfp4_linear(xq, q, bias, activation="relu", out_dtype=dtype), xv, wv, bias, True)
 
 
 @gpu
-@pytest.mark.parametrize("batch,time,c,n,taps,dilation", [(4, 300, 256, 260, 3, 1), (1, 1100, 80, 256, 5, 2), (7, 129, 130, 300, 4, 3),
-                                                          (600, 1, 64, 512, 3, 1), (40, 31, 40, 256, 7, 40), (2, 600, 300, 250, 2, 1)])
+@pytest.mark.parametrize("batch,time,c,n,taps,dilation", [
+    (4, 300, 256, 260, 3, 1), (1, 1100, 80, 256, 5, 2), (7, 129, 130, 300, 4, 3), (600, 1, 64, 512, 3, 1), (40, 31, 40, 256, 7, 40),
+    (2, 600, 300, 250, 2, 1), (64, 200, 256, 256, 3, 1), (3, 4100, 80, 300, 5, 2), (5000, 3, 130, 257, 4, 1), (130, 130, 60, 1030, 17, 20)])
 def test_conv1d_of_many_rows(batch, time, c, n, taps, dilation):
     rng = np.random.default_rng(batch + time + c)
     x, w, bias = draw(rng, batch, time, c), draw(rng, n, taps, c, scale=(taps * c) ** -0.5), draw(rng, n)
     q, xq = mxfp4_quantize(w), mxfp4_quantize(x)
-    rows, wv, b = gathered(f64(xq.dequantize()), taps, dilation), f64(q.dequantize()).reshape(n, -1), f64(bias)
-    want, size = rows @ wv.T + b, np.abs(rows) @ np.abs(wv).T + np.abs(b)
+    rows, wv = gathered(xq.dequantize().double(), taps, dilation), q.dequantize().double().reshape(n, -1)
     for dtype in TYPES:
-        y = mxfp4_conv1d(xq, q, bias, dilation=dilation, out_dtype=dtype)
-        check_product(y.reshape(batch * time, n), want, size, taps * c, dtype)
-    check_product(mxfp4_conv1d(x, q, bias, dilation=dilation).reshape(batch * time, n), want, size, taps * c, torch.float32)
+        check_product_on_device(mxfp4_conv1d(xq, q, bias, dilation=dilation, out_dtype=dtype), rows, wv, bias, False)
+    check_product_on_device(mxfp4_conv1d(x, q, bias, dilation=dilation, activation="relu"), rows, wv, bias, True)
 
 
 @gpu
@@ -252,7 +268,7 @@ def test_conv1d_agrees_with_torch_same_padding():
 
 
 @gpu
-@pytest.mark.parametrize("m", [1, 5, 40, 300, 4000])
+@pytest.mark.parametrize("m", [1, 5, 40, 300, 50000])
 def test_a_spoilt_row_of_either_side_stays_in_its_place(m):
     x, w = torch.ones(m, 200, device="cuda"), torch.ones(70, 200, device="cuda")
     x[m - 1, 150] = float("nan")

@@ -243,11 +243,21 @@ __global__ __launch_bounds__(WAVES * 64) void product_direct_kernel(Product p) {
 // ---------------------------------------------------------------------------
 // the product, large: 256 x 256 tiles staged through LDS
 // ---------------------------------------------------------------------------
-constexpr int kTile = 256;         // rows of w and rows of x of a workgroup's tile
-constexpr int kTileThreads = 512;
-constexpr int kOperand = kTile * kGroupBytes;          // codes of one operand in a stage: one group of every row
-constexpr int kStage = 2 * kOperand + 2 * kTile * 4;   // both operands' codes and scales
-constexpr int kStages = 4;
+constexpr int kTileN = 256;  // rows of w of a workgroup's tile
+
+// A tile has 64 * MW rows of x and 2 * MW waves.
+template <int MW>
+struct Tiling {
+    static constexpr int kWaves = 2 * MW, kThreads = 64 * kWaves, kTileM = 64 * MW;
+    static constexpr int kStages = MW == 4 ? 4 : 3;
+    // one stage: the codes of one group of every row of w and of x, then their scales
+    static constexpr int kW = 0, kX = kTileN * kGroupBytes, kWs = kX + kTileM * kGroupBytes, kXs = kWs + kTileN * 4;
+    static constexpr int kStage = kXs + kTileM * 4;
+    // a wave's loads for a stage: pieces of 16 rows of w and x, scales of 64 rows of w and of x
+    static constexpr int kLoadsW = kTileN / 16 / kWaves, kLoadsX = kTileM / 16 / kWaves;
+    static constexpr int kLoadsS = MW == 4 ? 1 : 2;
+    static constexpr int kLoads = kLoadsW + kLoadsX + kLoadsS;
+};
 
 // what a lane reads where a tap leaves its entry
 __device__ __align__(64) const uint32_t g_zeros[16] = {};
@@ -290,8 +300,10 @@ struct Fragments {
 // The wave's 32 rows (x) by 128 columns (w) of accumulators through its own 16 KB of LDS, so that
 // a row of y leaves in pieces of 16 bytes.  Lane l holds y[m = l % 32][8 * (e / 4) + 4 * (l / 32)
 // + e % 4] of every accumulator; piece q of row m lies at place q ^ m: reads and writes both
-// spread over the banks.
-template <typename T>
+// spread over the banks.  STREAM: past the L2, for products whose y is most of their traffic (8192 x
+// 8192 x 512: 40 us against 43; 55360 x 256 x 768: 13.5 against 15.4; where sums are long and L2 holds
+// the operands it costs: 8192 x 8192 x 1024 with the wide tile 62 us without, 66 with).
+template <typename T, bool STREAM>
 __device__ inline void store_rows(const Product& p, const f32x16 (&acc)[4], const float* bias, uint8_t* lds, int m0, int n0, int lane) {
     constexpr int kPieces = 128 * sizeof(T) / 16, kEach = 16 / sizeof(T);
     const int r = lane & 31, half = lane >> 5;
@@ -320,7 +332,13 @@ __device__ inline void store_rows(const Product& p, const f32x16 (&acc)[4], cons
 #pragma unroll
         for (int k = 0; k < 32 / kRows; ++k) v[k] = own(k * kRows + sub);
 #pragma unroll
-        for (int k = 0; k < 32 / kRows; ++k) store_16(y + (int64_t)k * kRows * p.n, v[k]);
+        for (int k = 0; k < 32 / kRows; ++k) {
+            auto* at = reinterpret_cast<Unaligned<T>*>(y + (int64_t)k * kRows * p.n);
+            if (STREAM)
+                __builtin_nontemporal_store(v[k], at);
+            else
+                *at = v[k];
+        }
         return;
     }
 #pragma unroll 1
@@ -340,86 +358,101 @@ __device__ inline void store_rows(const Product& p, const f32x16 (&acc)[4], cons
     }
 }
 
-// Eight waves, each 128 rows of w by 64 of x (4 x 2 accumulators of 32 x 32).  A stage holds one
-// group of both operands: [row][4 pieces of 16 bytes], piece q of row r at place q ^ (r / 4 % 4):
-// sixteen lanes that read one piece of sixteen rows then touch each of the 64 banks once.  Of the
-// four stages one is multiplied while three are on their way.  A stage is two steps; the barrier
-// stands between them, so that the products of the second hide the first reads of the next stage.
-template <bool CONV>
-__global__ __launch_bounds__(kTileThreads) void product_tiled_kernel(Product p) {
-    __shared__ __align__(1024) uint8_t lds[kStages * kStage];
-    __shared__ __align__(16) float bias[kTile];
+template <int N>
+__device__ inline void arrive_and_wait() {  // all but the N youngest loads are here, and every wave is
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+// Each wave multiplies 128 rows of w by 64 of x (4 x 2 accumulators of 32 x 32); two waves share the
+// rows of x.  A stage holds one group of both operands: [row][4 pieces of 16 bytes], piece q of row r
+// at place q ^ (r / 4 % 4): sixteen lanes that read one piece of sixteen rows then touch each of the
+// 64 banks once.  One stage is multiplied while the others are on their way.  A stage is two steps;
+// the barrier stands early in the second, whose products hide the first reads of the next stage.
+template <bool CONV, int MW>
+__global__ __launch_bounds__(Tiling<MW>::kThreads, 2) void product_tiled_kernel(Product p) {
+    using L = Tiling<MW>;
+    __shared__ __align__(1024) uint8_t lds[L::kStages * L::kStage];
+    __shared__ __align__(16) float bias[kTileN];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 31, half = lane >> 5;
-    const int m_tiles = (p.rows + kTile - 1) / kTile, n_tiles = (p.n + kTile - 1) / kTile;
+    const int m_tiles = (p.rows + L::kTileM - 1) / L::kTileM, n_tiles = (p.n + kTileN - 1) / kTileN;
     const Tile tile = tile_of(blockIdx.x, gridDim.x, m_tiles, n_tiles);
-    const int n0 = tile.n * kTile, m0 = tile.m * kTile;
+    const int n0 = tile.n * kTileN, m0 = tile.m * L::kTileM;
     const int all = p.taps * p.groups;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
 
-    // Five loads a wave and stage: two of w and two of x (load i fills rows i * 128 + wave * 16 .. + 15, lane l
-    // the place l % 4 of row l / 4), one of scales (64 rows of w or x).  Rows behind the last repeat it.
-    const int srow = wave * 16 + (lane >> 2);
+    // Load i of a wave fills 16 rows from (i * waves + wave) * 16 on, lane l the place l % 4 of row l / 4.
+    // Rows behind the last repeat it.
     const int place = ((lane & 3) ^ (lane >> 4)) * 16;
-    uint32_t woff[2], xoff[2], soff;
-    int xt[2], st = 0;
+    uint32_t woff[L::kLoadsW], xoff[L::kLoadsX], soff[L::kLoadsS];
+    int xt[L::kLoadsX], st = 0;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        woff[i] = min(n0 + i * 128 + srow, p.n - 1) * p.taps * kGroupBytes + place;
-        const int m = min(m0 + i * 128 + srow, p.rows - 1);
+    for (int i = 0; i < L::kLoadsW; ++i)
+        woff[i] = min(n0 + (i * L::kWaves + wave) * 16 + (lane >> 2), p.n - 1) * p.taps * kGroupBytes + place;
+#pragma unroll
+    for (int i = 0; i < L::kLoadsX; ++i) {
+        const int m = min(m0 + (i * L::kWaves + wave) * 16 + (lane >> 2), p.rows - 1);
         xoff[i] = m * kGroupBytes + place;
         xt[i] = CONV ? m % p.T : 0;
     }
-    const bool wscales = wave < 4;
-    if (wscales) {
-        soff = min(n0 + (int)threadIdx.x, p.n - 1) * p.taps * 4;
-    } else {
-        const int m = min(m0 + (int)threadIdx.x - kTile, p.rows - 1);
-        soff = m * 4;
-        st = CONV ? m % p.T : 0;
+    // Scales: with eight waves the first four bring w's and the others x's; with four each brings 64 rows of w
+    // and, two of them twice, of x.
+    const bool first_w = MW == 2 || wave < 4;
+    {
+        const int m = min(m0 + (MW == 4 ? wave - 4 : wave & 1) * 64 + lane, p.rows - 1);
+        if (first_w) soff[0] = min(n0 + wave * 64 + lane, p.n - 1) * p.taps * 4;
+        if (!first_w || MW == 2) {
+            soff[L::kLoadsS - 1] = m * 4;
+            st = CONV ? m % p.T : 0;
+        }
     }
     // the next stage to be loaded: tap, group, and where their rows begin (counted in rows)
     int tap = 0, gx = 0;
     int64_t wrow = 0, xrow = 0;
-    const int64_t wstep = (int64_t)p.n * p.taps, sstep = wscales ? wstep : p.rows;
-    const uint8_t* sbase = wscales ? p.ws : p.xs;
-    int64_t srow4 = 0;
-    // loads 0 and 1: w, 2 and 3: x, 4: scales, and on to the next group; no branches
+    const int64_t wstep = (int64_t)p.n * p.taps;
+    // scale loads of this wave, first and last: base, bytes to the current group, bytes of a group
+    const uint8_t* sbase = first_w ? p.ws : p.xs;
+    const int64_t sstep = (first_w ? wstep : p.rows) * 4;
+    int64_t sat = 0;
+    // the loads in order: w, x, scales; after the last one on to the next group; no branches
     auto stage_part = [&](int slot, auto part) {
-        constexpr int i = part;
-        const uint32_t dst = lds0 + slot * kStage;
-        const int shift = CONV ? tap * p.dilation - p.left : 0;
-        const uint8_t* zeros = reinterpret_cast<const uint8_t*>(g_zeros);
-        if constexpr (i < 2) {
-            to_lds(p.wc + wrow * kGroupBytes, woff[i], dst + i * 8192 + wave * 1024);
-        } else if constexpr (i < 4) {
-            const uint8_t* xbase = p.xc + xrow * kGroupBytes;
-            const uint32_t to = dst + kOperand + (i - 2) * 8192 + wave * 1024;
-            if (CONV) {
-                const bool inside = (unsigned)(xt[i - 2] + shift) < (unsigned)p.T;
-                to_lds(inside ? xbase + (int64_t)xoff[i - 2] + (int64_t)shift * kGroupBytes : zeros, to);
+        constexpr int i = part, xi = i - L::kLoadsW, si = xi - L::kLoadsX;
+        if constexpr (i < L::kLoads) {
+            const uint32_t dst = lds0 + slot * L::kStage;
+            const int shift = CONV ? tap * p.dilation - p.left : 0;
+            const uint8_t* zeros = reinterpret_cast<const uint8_t*>(g_zeros);
+            if constexpr (i < L::kLoadsW) {
+                to_lds(p.wc + wrow * kGroupBytes, woff[i], dst + L::kW + (i * L::kWaves + wave) * 1024);
+            } else if constexpr (xi < L::kLoadsX) {
+                const uint8_t* xbase = p.xc + xrow * kGroupBytes;
+                const uint32_t to = dst + L::kX + (xi * L::kWaves + wave) * 1024;
+                if (CONV) {
+                    const bool inside = (unsigned)(xt[xi] + shift) < (unsigned)p.T;
+                    to_lds(inside ? xbase + (int64_t)xoff[xi] + (int64_t)shift * kGroupBytes : zeros, to);
+                } else {
+                    to_lds(xbase, xoff[xi], to);
+                }
             } else {
-                to_lds(xbase, xoff[i - 2], to);
+                const bool of_w = MW == 4 ? first_w : si == 0;
+                const uint32_t to = dst + (MW == 4 ? L::kWs + wave * 256 : si == 0 ? L::kWs + wave * 256 : L::kXs + (wave & 1) * 256);
+                const uint8_t* from = si == 0 ? sbase + sat : p.xs + xrow * 4;
+                if (CONV) {
+                    // of w the tap's own scales; of x those of the shifted row
+                    const int own = of_w ? tap : shift;
+                    const bool inside = of_w | ((unsigned)(st + shift) < (unsigned)p.T);
+                    dword_to_lds(inside ? from + (int64_t)soff[si] + (int64_t)own * 4 : zeros, to);
+                } else {
+                    dword_to_lds(from, soff[si], to);
+                }
             }
-        } else {
-            const uint32_t to = dst + 2 * kOperand + wave * 256;
-            if (CONV) {
-                // of w the tap's own scales; of x those of the shifted row
-                const int own = wscales ? tap : shift;
-                const bool inside = wscales | ((unsigned)(st + shift) < (unsigned)p.T);
-                dword_to_lds(inside ? sbase + srow4 + (int64_t)soff + (int64_t)own * 4 : zeros, to);
-                const bool last = ++gx == p.groups;
-                tap += last;
-                gx = last ? 0 : gx;
-                wrow = last ? tap : wrow + wstep;
-                xrow = last ? 0 : xrow + p.rows;
-                srow4 = last ? 0 : srow4 + sstep * 4;
-            } else {
-                dword_to_lds(sbase + srow4, soff, to);
-                wrow += wstep;
-                xrow += p.rows;
-                srow4 += sstep * 4;
-            }
+        }
+        if constexpr (i == L::kLoads - 1) {
+            const bool last = CONV && gx == p.groups - 1;
+            if (CONV) tap += last;
+            gx = last ? 0 : gx + 1;
+            wrow = last ? tap : wrow + wstep;
+            xrow = last ? 0 : xrow + p.rows;
+            sat = last ? 0 : sat + sstep;
         }
     };
     auto stage = [&](int slot) {
@@ -428,34 +461,37 @@ __global__ __launch_bounds__(kTileThreads) void product_tiled_kernel(Product p) 
         stage_part(slot, std::integral_constant<int, 2>{});
         stage_part(slot, std::integral_constant<int, 3>{});
         stage_part(slot, std::integral_constant<int, 4>{});
+        stage_part(slot, std::integral_constant<int, 5>{});
+        stage_part(slot, std::integral_constant<int, 6>{});
+        stage_part(slot, std::integral_constant<int, 7>{});
     };
 
 #pragma unroll
-    for (int c = 0; c < kStages; ++c)
+    for (int c = 0; c < L::kStages; ++c)
         if (c < all) stage(c);
     // asked for here, used behind the loop: no wait of its own
     float own_bias = 0.f;
-    if (p.bias && n0 + (int)threadIdx.x < p.n && threadIdx.x < kTile) own_bias = load_float(p.bias, p.bias_type, n0 + threadIdx.x);
+    if (p.bias && n0 + (int)threadIdx.x < p.n && threadIdx.x < kTileN) own_bias = load_float(p.bias, p.bias_type, n0 + threadIdx.x);
 
     const int nw = (wave & 1) * 128, mw = (wave >> 1) * 64;
     // lane l takes, of row l % 32, the blocks 2 * (l / 32) and + 1 in the two steps
     uint32_t at[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) at[k] = ((half * 2 + k) ^ ((r >> 2) & 3)) * 16;
-    const uint32_t wr = (nw + r) * kGroupBytes, xr = kOperand + (mw + r) * kGroupBytes;
+    const uint32_t wr = L::kW + (nw + r) * kGroupBytes, xr = L::kX + (mw + r) * kGroupBytes;
     auto fetch_w = [&](uint32_t base, int k, int i, Fragments& f) {
         f.w[i] = *reinterpret_cast<const i32x4*>(lds + base + wr + at[k] + i * 32 * kGroupBytes);
     };
     auto fetch_x = [&](uint32_t base, int k, int j, Fragments& f) {
         f.x[j] = *reinterpret_cast<const i32x4*>(lds + base + xr + at[k] + j * 32 * kGroupBytes);
     };
-    int ws[4], xs[2];
-    const uint32_t wsr = 2 * kOperand + (nw + r) * 4, xsr = 2 * kOperand + kTile * 4 + (mw + r) * 4;
-    auto fetch_scales = [&](uint32_t base, int (&w)[4], int (&x)[2]) {
+    int ws[4], xs[2], wnext[4], xnext[2];
+    const uint32_t wsr = L::kWs + (nw + r) * 4, xsr = L::kXs + (mw + r) * 4;
+    auto fetch_scales = [&](uint32_t base) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const int*>(lds + base + wsr + i * 128);
+        for (int i = 0; i < 4; ++i) wnext[i] = *reinterpret_cast<const int*>(lds + base + wsr + i * 128);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) x[j] = *reinterpret_cast<const int*>(lds + base + xsr + j * 128);
+        for (int j = 0; j < 2; ++j) xnext[j] = *reinterpret_cast<const int*>(lds + base + xsr + j * 128);
     };
     f32x16 acc[4][2] = {};
     auto multiply = [&](auto S, int i, int j, const Fragments& f) {
@@ -463,22 +499,22 @@ __global__ __launch_bounds__(kTileThreads) void product_tiled_kernel(Product p) 
     };
 
     Fragments fa, fb;
-    if (all >= kStages)
-        asm volatile("s_waitcnt vmcnt(15)\n\ts_barrier" ::: "memory");
+    if (all >= L::kStages)
+        arrive_and_wait<(L::kStages - 1) * L::kLoads>();
     else
-        asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-    int wnext[4], xnext[2];
+        arrive_and_wait<0>();
     for (int i = 0; i < 4; ++i) fetch_w(0, 0, i, fa);
     for (int j = 0; j < 2; ++j) fetch_x(0, 0, j, fa);
-    fetch_scales(0, wnext, xnext);
+    fetch_scales(0);
+    int slot = 0;
     uint32_t base = 0;
-    auto chunk = [&](int c, auto more) {
+    auto chunk = [&](auto more) {
         // the dword holds the group's four blocks: this lane's two go to the front
 #pragma unroll
         for (int i = 0; i < 4; ++i) ws[i] = (uint32_t)wnext[i] >> (half * 16);
 #pragma unroll
         for (int j = 0; j < 2; ++j) xs[j] = (uint32_t)xnext[j] >> (half * 16);
-        // What is not a product is issued in the shadow of one (32 cycles each): both waves of a SIMD come
+        // What is not a product is issued in the shadow of one (32 cycles each): the waves of a SIMD may come
         // through here together, so nothing else would keep the matrix core busy meanwhile.
         constexpr std::integral_constant<int, 0> first{};
         constexpr std::integral_constant<int, 1> second{};
@@ -490,53 +526,71 @@ __global__ __launch_bounds__(kTileThreads) void product_tiled_kernel(Product p) 
         multiply(first, 3, 0, fa), multiply(first, 0, 1, fa), multiply(first, 1, 1, fa), THEN;
         multiply(first, 2, 1, fa), multiply(first, 3, 1, fa), THEN;
         multiply(second, 0, 0, fb), multiply(second, 1, 0, fb), THEN;
-        // the next stage has arrived (two more may be under way), and this one has been read, everywhere
+        // the next stage has arrived (younger ones may be under way), and this one has been read, everywhere
         if constexpr (more)
-            asm volatile("s_waitcnt vmcnt(10) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            arrive_and_wait<(L::kStages - 2) * L::kLoads>();
         else
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        const int slot = c & (kStages - 1);
-        base = ((c + 1) & (kStages - 1)) * kStage;
+            arrive_and_wait<0>();
+        const int freed = slot;
+        slot = slot == L::kStages - 1 ? 0 : slot + 1;
+        base = slot * L::kStage;
         // after the last stage these reads bring whatever lies there, and nothing uses it
         fetch_w(base, 0, 0, fa), fetch_x(base, 0, 0, fa), THEN;
         multiply(second, 2, 0, fb), THEN, fetch_w(base, 0, 1, fa), fetch_w(base, 0, 2, fa), THEN;
         multiply(second, 3, 0, fb), THEN, fetch_w(base, 0, 3, fa), fetch_x(base, 0, 1, fa), THEN;
-        multiply(second, 0, 1, fb), THEN, fetch_scales(base, wnext, xnext), THEN;
+        multiply(second, 0, 1, fb), THEN, fetch_scales(base), THEN;
         multiply(second, 1, 1, fb), THEN;
         if constexpr (more) {
-            stage_part(slot, std::integral_constant<int, 0>{});
-            stage_part(slot, std::integral_constant<int, 1>{});
+            stage_part(freed, std::integral_constant<int, 0>{});
+            stage_part(freed, std::integral_constant<int, 1>{});
+            stage_part(freed, std::integral_constant<int, 2>{});
         }
         THEN, multiply(second, 2, 1, fb), THEN;
         if constexpr (more) {
-            stage_part(slot, std::integral_constant<int, 2>{});
-            stage_part(slot, std::integral_constant<int, 3>{});
+            stage_part(freed, std::integral_constant<int, 3>{});
+            stage_part(freed, std::integral_constant<int, 4>{});
+            stage_part(freed, std::integral_constant<int, 5>{});
         }
         THEN, multiply(second, 3, 1, fb), THEN;
-        if constexpr (more) stage_part(slot, std::integral_constant<int, 4>{});
+        if constexpr (more) {
+            stage_part(freed, std::integral_constant<int, 6>{});
+            stage_part(freed, std::integral_constant<int, 7>{});
+        }
         THEN;
 #undef THEN
     };
     // two loops, each without a branch inside: products stay on their side of the barrier
     int c = 0;
-    for (; c < all - kStages; ++c) chunk(c, std::true_type{});
-    for (; c < all; ++c) chunk(c, std::false_type{});
+    for (; c < all - L::kStages; ++c) chunk(std::true_type{});
+    for (; c < all; ++c) chunk(std::false_type{});
 
-    if (threadIdx.x < kTile) bias[threadIdx.x] = own_bias;
+    if (threadIdx.x < kTileN) bias[threadIdx.x] = own_bias;
     __syncthreads();
     // every read of the stages lies behind: each wave takes 16 KB of them
+    static_assert(L::kWaves * 16384 <= L::kStages * L::kStage, "the stages hold the waves' parts of y");
     uint8_t* own = lds + wave * 16384;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         const f32x16(&part)[4] = {acc[0][j], acc[1][j], acc[2][j], acc[3][j]};
         if (p.y_type == GLV_F32)
-            store_rows<float>(p, part, bias + nw, own, m0 + mw + j * 32, n0 + nw, lane);
+            store_rows<float, MW == 2>(p, part, bias + nw, own, m0 + mw + j * 32, n0 + nw, lane);
         else if (p.y_type == GLV_BF16)
-            store_rows<bf16>(p, part, bias + nw, own, m0 + mw + j * 32, n0 + nw, lane);
+            store_rows<bf16, MW == 2>(p, part, bias + nw, own, m0 + mw + j * 32, n0 + nw, lane);
         else
-            store_rows<f16>(p, part, bias + nw, own, m0 + mw + j * 32, n0 + nw, lane);
+            store_rows<f16, MW == 2>(p, part, bias + nw, own, m0 + mw + j * 32, n0 + nw, lane);
         // one wave's reads and the next pass's writes of its own LDS stay in order in the LDS queue
     }
+}
+
+template <int MW>
+int launch_tiled(const Product& p, hipStream_t st) {
+    using L = Tiling<MW>;
+    const unsigned tiles = (unsigned)((p.rows + L::kTileM - 1) / L::kTileM) * ((p.n + kTileN - 1) / kTileN);
+    if (p.taps > 1)
+        hipLaunchKernelGGL((product_tiled_kernel<true, MW>), dim3(tiles), dim3(L::kThreads), 0, st, p);
+    else
+        hipLaunchKernelGGL((product_tiled_kernel<false, MW>), dim3(tiles), dim3(L::kThreads), 0, st, p);
+    return launch_status("product_tiled_kernel");
 }
 
 // rows sixteen at a time by groups four at a time
@@ -678,13 +732,14 @@ extern "C" int glv_mxfp4_product(const void* x_dev, const uint8_t* x_scales_dev,
         if (rc != GLV_OK) return rc;
         p.xc = codes, p.xs = scales;
     }
-    if (all * n_out >= 512 * 512) {
-        const unsigned tiles = (unsigned)(((all + kTile - 1) / kTile) * ((n_out + kTile - 1) / kTile));
-        if (taps > 1)
-            hipLaunchKernelGGL(product_tiled_kernel<true>, dim3(tiles), dim3(kTileThreads), 0, st, p);
-        else
-            hipLaunchKernelGGL(product_tiled_kernel<false>, dim3(tiles), dim3(kTileThreads), 0, st, p);
-        return launch_status("product_tiled_kernel");
+    // Below 3 M outputs the small tiles win (1000 x 1000 x 1024: 5.7 us against 11.6; 1024 x 2048 x 4096: 19.1
+    // against 19.4), above it the large ones (865 x 4096 x 1024: 10.2 against 11.4; 2048 x 2048 x 4096: 21 against
+    // 35).  256 rows of x a tile pay for long sums that fill the chip (8192 x 8192 x 8192: 250 us against 276; x
+    // 2048: 93 against 100); with 128 there is room for a second workgroup on the CU, whose loop hides the ends
+    // of the first (8192 x 8192 x 512: 40 against 47; 16384 x 256 x 1024: 10.2 against 11.8).
+    if (all * n_out >= (int64_t)3 << 20) {
+        const int64_t wide = ((all + 255) / 256) * ((n_out + 255) / 256);
+        return wide >= 256 && p.taps * p.groups >= 16 ? launch_tiled<4>(p, st) : launch_tiled<2>(p, st);
     }
     const int64_t tiles = ((all + 31) / 32) * ((n_out + 31) / 32);
     if (tiles > INT32_MAX) return report(GLV_ERR_INVALID, "%s: rows x n_out too large for one call", what);
