@@ -24,24 +24,16 @@ _NORMS = {"layer": 1, "rms": 2}
 _GROUP = 128  # columns that share one dword of scales
 
 
-class _on:
-    """Makes `device` current for the launches inside the block and gives their stream."""
-
-    __slots__ = ("index", "previous")
-
-    def __init__(self, device):
-        self.index = device.index
-
-    def __enter__(self):
-        self.previous = torch.cuda.current_device()
-        if self.previous != self.index:
-            torch.cuda.set_device(self.index)
-        return torch.cuda.current_stream(self.index).cuda_stream
-
-    def __exit__(self, *exc):
-        if self.previous != self.index:
-            torch.cuda.set_device(self.previous)
-        return False
+def _launch(device, entry, *args):
+    """entry(*args, stream) with `device` current, on torch's current stream of it."""
+    index = device.index
+    if torch.cuda.current_device() == index:
+        rc = entry(*args, torch.cuda.current_stream(index).cuda_stream)
+    else:
+        with torch.cuda.device(index):
+            rc = entry(*args, torch.cuda.current_stream(index).cuda_stream)
+    if rc:
+        _lib.check(rc)
 
 
 def _check(t, name, device=None):
@@ -115,10 +107,8 @@ class MXFP4Tensor:
         if not self.codes.is_cuda:
             raise ValueError(f"the tensor must be on a ROCm GPU (there is no CPU fallback), got {self.device}")
         out = torch.empty(self.shape, dtype=dtype, device=self.device)
-        with _on(self.device) as stream:
-            _lib.check(_lib.load().glv_mxfp4_dequantize(self.codes.data_ptr(), self.scales.data_ptr(),
-                                                        self.codes.shape[1], self.shape[-1], _TYPES[dtype],
-                                                        out.data_ptr(), stream))
+        _launch(self.device, _lib.load().glv_mxfp4_dequantize, self.codes.data_ptr(), self.scales.data_ptr(),
+                self.codes.shape[1], self.shape[-1], _TYPES[dtype], out.data_ptr())
         return out
 
     def __repr__(self):
@@ -137,9 +127,8 @@ def mxfp4_quantize(x):
     rows, groups = v.shape[0] * v.shape[1], -(-v.shape[2] // _GROUP)
     codes = torch.empty((groups, rows, 64), dtype=torch.uint8, device=x.device)
     scales = torch.empty((groups, rows, 4), dtype=torch.uint8, device=x.device)
-    with _on(x.device) as stream:
-        _lib.check(_lib.load().glv_mxfp4_quantize(v.data_ptr(), _TYPES[x.dtype], v.shape[0], v.shape[1], v.shape[2],
-                                                  v.stride(0), v.stride(1), codes.data_ptr(), scales.data_ptr(), stream))
+    _launch(x.device, _lib.load().glv_mxfp4_quantize, v.data_ptr(), _TYPES[x.dtype], *v.shape, v.stride(0), v.stride(1),
+            codes.data_ptr(), scales.data_ptr())
     return MXFP4Tensor(x.shape, codes, scales)
 
 
@@ -180,12 +169,11 @@ def _product(x, weight, bias, taps, dilation, activation, out_dtype):
     y = torch.empty((*x.shape[:-1], n), dtype=out_dtype, device=device)
     need = lib.glv_mxfp4_product_workspace(kind, batch, rows, cols, n, taps)
     work = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
-    with _on(device) as stream:
-        _lib.check(lib.glv_mxfp4_product(
-            data, scales, kind, batch, rows, cols, strides[0], strides[1], weight.codes.data_ptr(),
-            weight.scales.data_ptr(), n, taps, dilation, None if bias is None else bias.data_ptr(),
-            0 if bias is None else _TYPES[bias.dtype], _ACTIVATIONS[activation], y.data_ptr(), _TYPES[out_dtype],
-            None if work is None else work.data_ptr(), max(need, 0), stream))
+    _launch(device, lib.glv_mxfp4_product, data, scales, kind, batch, rows, cols, strides[0], strides[1],
+            weight.codes.data_ptr(), weight.scales.data_ptr(), n, taps, dilation,
+            None if bias is None else bias.data_ptr(), 0 if bias is None else _TYPES[bias.dtype],
+            _ACTIVATIONS[activation], y.data_ptr(), _TYPES[out_dtype], None if work is None else work.data_ptr(),
+            max(need, 0))
     return y
 
 
@@ -304,13 +292,11 @@ def block_norm(u, *, post=None, gate=None, scale=None, residual=None, pre=None):
         r_strides = (r.stride(0), r.stride(1))
     y = torch.empty(u.shape, dtype=dtype, device=device)
     z = torch.empty(u.shape, dtype=dtype, device=device) if pre is not None else None
-    with _on(device) as stream:
-        _lib.check(_lib.load().glv_block_norm(
-            v.data_ptr(), _TYPES[dtype], batch, rows, cols, v.stride(0), v.stride(1),
+    _launch(device, _lib.load().glv_block_norm, v.data_ptr(), _TYPES[dtype], batch, rows, cols, v.stride(0), v.stride(1),
             _TYPES[torch.float32 if vector_type is None else vector_type],
             0 if post is None else _NORMS[post.kind], post_w, post_b, 0.0 if post is None else post.eps,
             None if g is None else g.data_ptr(), *g_strides, scale_vec, factor,
             None if r is None else r.data_ptr(), *r_strides,
             0 if pre is None else _NORMS[pre.kind], pre_w, pre_b, 0.0 if pre is None else pre.eps,
-            y.data_ptr(), None if z is None else z.data_ptr(), stream))
+            y.data_ptr(), None if z is None else z.data_ptr())
     return y if z is None else (y, z)

@@ -53,7 +53,7 @@ __device__ inline float row_sum(float v, float* slot) {
 }
 
 // x <- Norm(x) for the row held as V pieces of eight per thread; `valid` counts columns
-template <typename W, int TPR, int V>
+template <typename W, int TPR, int V, bool NARROW>
 __device__ inline void normalise(float (&x)[V][8], int kind, const void* weight, const void* bias, float eps, int cols,
                                  int lane, float* slot) {
     const float inv = 1.f / (float)cols;
@@ -81,8 +81,8 @@ __device__ inline void normalise(float (&x)[V][8], int kind, const void* weight,
         const int col = (v * TPR + lane) * 8;
         if (col < cols) {
             Eight<W> w, b;
-            if (weight) w = load_eight(static_cast<const W*>(weight) + col, cols - col);
-            if (bias) b = load_eight(static_cast<const W*>(bias) + col, cols - col);
+            if (weight) w = load_eight<NARROW>(static_cast<const W*>(weight), col, cols);
+            if (bias) b = load_eight<NARROW>(static_cast<const W*>(bias), col, cols);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 float t = x[v][i] * r;
@@ -95,7 +95,7 @@ __device__ inline void normalise(float (&x)[V][8], int kind, const void* weight,
 }
 
 // TPR threads a row, V pieces of eight columns a thread
-template <typename T, typename W, int TPR, int V>
+template <typename T, typename W, int TPR, int V, bool NARROW = false>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void block_norm_kernel(BlockNorm p) {
     __shared__ float slots[TPR > 64 ? 4 * (TPR / 64) : 1];
     constexpr int kRows = TPR < 256 ? 256 / TPR : 1;
@@ -112,22 +112,22 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void block_norm_kernel(Block
 #pragma unroll
     for (int v = 0; v < V; ++v) {
         const int col = (v * TPR + lane) * 8;
-        ur[v] = load_eight(u + col, p.cols - col);
-        if (gate && p.gate_col) gr[v] = load_eight(gate + col, p.cols - col);
-        if (res) rr[v] = load_eight(res + col, p.cols - col);
+        ur[v] = load_eight<NARROW>(u, col, p.cols);
+        if (gate && p.gate_col) gr[v] = load_eight<NARROW>(gate, col, p.cols);
+        if (res) rr[v] = load_eight<NARROW>(res, col, p.cols);
     }
     float x[V][8];
 #pragma unroll
     for (int v = 0; v < V; ++v)
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[v][i] = (float)ur[v].v[i];
-    if (p.post) normalise<W, TPR, V>(x, p.post, p.post_w, p.post_b, p.post_eps, p.cols, lane, slots);
+    if (p.post) normalise<W, TPR, V, NARROW>(x, p.post, p.post_w, p.post_b, p.post_eps, p.cols, lane, slots);
     const float row_factor = p.scale * (gate && !p.gate_col ? (float)gate[0] : 1.f);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
         const int col = (v * TPR + lane) * 8;
         Eight<W> sv;
-        if (p.scale_vec) sv = load_eight(static_cast<const W*>(p.scale_vec) + col, p.cols - col);
+        if (p.scale_vec) sv = load_eight<NARROW>(static_cast<const W*>(p.scale_vec), col, p.cols);
         Eight<T> o;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -141,7 +141,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void block_norm_kernel(Block
         store_eight(static_cast<T*>(p.y) + out + col, o, p.cols - col);
     }
     if (!p.pre) return;
-    normalise<W, TPR, V>(x, p.pre, p.pre_w, p.pre_b, p.pre_eps, p.cols, lane, slots + 2 * (TPR / 64));
+    normalise<W, TPR, V, NARROW>(x, p.pre, p.pre_w, p.pre_b, p.pre_eps, p.cols, lane, slots + 2 * (TPR / 64));
 #pragma unroll
     for (int v = 0; v < V; ++v) {
         const int col = (v * TPR + lane) * 8;
@@ -155,7 +155,9 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void block_norm_kernel(Block
 template <typename T, typename W>
 void launch(const BlockNorm& p, hipStream_t st) {
     const dim3 by4((p.rows + 3) / 4), by1(p.rows);
-    if (p.cols <= 512)
+    if (p.cols < 8)
+        hipLaunchKernelGGL((block_norm_kernel<T, W, 64, 1, true>), by4, dim3(256), 0, st, p);
+    else if (p.cols <= 512)
         hipLaunchKernelGGL((block_norm_kernel<T, W, 64, 1>), by4, dim3(256), 0, st, p);
     else if (p.cols <= 1024)
         hipLaunchKernelGGL((block_norm_kernel<T, W, 64, 2>), by4, dim3(256), 0, st, p);

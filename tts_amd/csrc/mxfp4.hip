@@ -27,35 +27,43 @@ constexpr int kGroupBytes = 64;   // its codes
 
 struct Rows {  // a (batch, rows, cols) array whose last dimension is contiguous
     int64_t batch_stride, row_stride;
-    int rows;  // rows of one batch entry
+    int rows;   // rows of one batch entry
+    bool flat;  // there is one entry
 };
 
 __device__ inline int64_t row_offset(const Rows& r, int row) {
+    if (r.flat) return row * r.row_stride;
     const int b = row / r.rows;
     return b * r.batch_stride + (int64_t)(row - b * r.rows) * r.row_stride;
 }
 
 // biased exponent of max|x| as float sees it (255: an infinity or a NaN is among them)
 __device__ inline int top_exponent(const Eight<float>& x) {
-    uint32_t m = 0;
+    float m = 0.f;  // the maximum that keeps a NaN: three operands an instruction, signs dropped on the way in
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, __builtin_bit_cast(uint32_t, x.v[i]) & 0x7fffffffu);
-    return (int)(m >> 23);
+    for (int i = 0; i < 8; i += 2)
+        m = __builtin_elementwise_maximum(__builtin_elementwise_maximum(m, __builtin_fabsf(x.v[i])), __builtin_fabsf(x.v[i + 1]));
+    return (int)(__builtin_bit_cast(uint32_t, m) >> 23 & 255);
 }
-__device__ inline int top_exponent(const Eight<bf16>& x) {
-    uint32_t m = 0;
+// the larger of the magnitudes' bits, two at a time: the order of the bits is that of the values
+template <typename T>
+__device__ inline uint32_t top_half_bits(const Eight<T>& x) {
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    struct Pairs {
+        uint32_t w[4];
+    };
+    const Pairs p = __builtin_bit_cast(Pairs, x);
+    u16x2 m = __builtin_bit_cast(u16x2, p.w[0] & 0x7fff7fffu);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, (uint32_t)(__builtin_bit_cast(uint16_t, x.v[i]) & 0x7fff));
-    return (int)(m >> 7);
+    for (int i = 1; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, p.w[i] & 0x7fff7fffu));
+    return max((uint32_t)m.x, (uint32_t)m.y);
 }
+__device__ inline int top_exponent(const Eight<bf16>& x) { return (int)(top_half_bits(x) >> 7); }
 __device__ inline int top_exponent(const Eight<f16>& x) {
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, (uint32_t)(__builtin_bit_cast(uint16_t, x.v[i]) & 0x7fff));
-    if (m >= 0x7c00) return 255;
+    const uint32_t m = top_half_bits(x);
     // every finite half is a normal float, so its exponent there is the true one
     const float f = (float)__builtin_bit_cast(f16, (uint16_t)m);
-    return (int)(__builtin_bit_cast(uint32_t, f) >> 23);
+    return m >= 0x7c00 ? 255 : (int)(__builtin_bit_cast(uint32_t, f) >> 23);
 }
 
 __device__ inline int scale_byte(int top) { return top == 255 ? 255 : max(top - 2, 0); }
@@ -91,11 +99,12 @@ __device__ inline uint32_t quantise_eight(const Eight<T>& x, int* byte) {
     top = max(top, __builtin_amdgcn_mov_dpp(top, 0x4E, 0xf, 0xf, true));  // quad_perm 2,3,0,1
     const int s = scale_byte(top);
     *byte = s;
-    return s == 255 ? 0u : encode(x, __builtin_bit_cast(float, (uint32_t)s << 23));
+    const uint32_t codes = encode(x, __builtin_bit_cast(float, (uint32_t)s << 23));
+    return s == 255 ? 0u : codes;
 }
 
 // Sixteen lanes a group; a workgroup takes sixteen rows of up to four groups.
-template <typename T>
+template <typename T, bool NARROW>
 __global__ __launch_bounds__(256) void quantise_kernel(const T* __restrict__ x, Rows xr, int rows, int cols, int groups,
                                                        uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
     const int spans = (groups + 3) / 4;
@@ -107,7 +116,7 @@ __global__ __launch_bounds__(256) void quantise_kernel(const T* __restrict__ x, 
     for (int g = first; g < min(groups, first + 4); ++g) {
         const int col = g * kGroup + piece * 8;
         int byte;
-        const uint32_t c = quantise_eight(load_eight(src + col, cols - col), &byte);
+        const uint32_t c = quantise_eight(load_eight<NARROW>(src, col, cols), &byte);
         reinterpret_cast<uint32_t*>(codes)[((int64_t)g * rows + row) * 16 + piece] = c;
         if ((piece & 3) == 0) scales[((int64_t)g * rows + row) * 4 + (piece >> 2)] = (uint8_t)byte;
     }
@@ -145,7 +154,10 @@ __global__ __launch_bounds__(256) void dequantise_kernel(const uint8_t* __restri
 // the product
 // ---------------------------------------------------------------------------
 struct Product {
-    const uint8_t *xc, *xs;  // quantised activations: rows = batch * T
+    const uint8_t *xc, *xs;  // quantised activations: rows = batch * T, or
+    const void* x;           // float ones, of `cols` columns
+    Rows xr;
+    int cols;
     const uint8_t *wc, *ws;  // weights: n * taps rows of `groups` groups
     const void* bias;
     void* y;
@@ -175,70 +187,108 @@ __device__ inline float at_least(float v, float least) { return __builtin_elemen
 
 __device__ inline i32x8 widen(i32x4 v) { return __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1); }
 
-// acc += W (32 rows) * X (32 rows)^T over the 64 columns of step S: lane l holds row l % 32 and, of
-// the two groups of a step, group l / 32: its 32 columns of block S.  Which columns meet in one
-// instruction is free as long as both operands agree, so a lane takes the four blocks of its own
-// group in the four steps, and one scale dword serves them all.
+// acc += W (32 rows) * X (32 rows)^T over 64 columns: lane l holds 32 of them, one block, of row l % 32;
+// byte S of its scale dwords is that block's.  Which columns meet in one instruction is free as long
+// as both operands agree: of a group's four blocks the lanes below 32 take the first two in the two
+// steps, the others the last two, and a shift by 16 puts a lane's two scales in front.
 template <int S>
 __device__ inline f32x16 step(i32x4 w, i32x4 x, int wscale, int xscale, f32x16 acc) {
     return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(widen(w), widen(x), acc, 4, 4, S, wscale, S, xscale);
 }
 
-// One 32 x 32 tile of y a workgroup; the waves deal the groups out among themselves two at a time
-// (one for each half of the lanes) and their sums meet in LDS in a fixed order.
-template <int WAVES>
+// One 32 x 32 tile of y a workgroup; the waves deal the groups out among themselves and their sums meet
+// in LDS in a fixed order.  X is `void` for activations that are quantised already; otherwise a wave
+// quantises the 32 rows of its group itself, sixteen lanes a row, and passes the codes to the lanes
+// that multiply them through LDS of its own, so that a small product is one launch.
+template <typename X, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void product_direct_kernel(Product p) {
+    constexpr bool kOwn = !std::is_void_v<X>;
     __shared__ float sums[WAVES][32][33];
+    __shared__ __align__(16) uint32_t codes[kOwn ? WAVES : 1][32][16];
+    __shared__ __align__(4) uint8_t scales[kOwn ? WAVES : 1][32][4];
+    __shared__ int64_t row_at[32];  // where the tile's rows begin, and their places in their entries
+    __shared__ int row_t[32];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int r = lane & 31, half = lane >> 5;
     const int n_tiles = (p.n + 31) / 32;
     const int m_tile = blockIdx.x / n_tiles;
     const int n0 = (blockIdx.x - m_tile * n_tiles) * 32, m0 = m_tile * 32;
     const int n = min(n0 + r, p.n - 1), m = min(m0 + r, p.rows - 1);  // rows beyond the ends: computed, not stored
-    const int t = m % p.T;
+    const int rows = min(32, p.rows - m0);
+    const int t = p.taps == 1 ? 0 : m % p.T;
     const int all = p.taps * p.groups;
+    if constexpr (kOwn) {
+        if (threadIdx.x < 32) {
+            row_at[threadIdx.x] = row_offset(p.xr, m);
+            row_t[threadIdx.x] = t;
+        }
+        __syncthreads();
+    }
     f32x16 acc = {};
-    for (int g0 = wave * 2; g0 < all; g0 += WAVES * 2) {
-        const int g = g0 + half;
-        const int tap = g / p.groups, gx = g - tap * p.groups;
+    for (int g = wave; g < all; g += WAVES) {
+        const int tap = p.taps == 1 ? 0 : g / p.groups, gx = g - tap * p.groups;
         const int shift = tap * p.dilation - p.left;
-        const bool have = g < all && t + shift >= 0 && t + shift < p.T;
-        i32x4 w[4] = {}, x[4] = {};
-        int wscale = 0, xscale = 0;
-        if (g < all) {
-            const int64_t row = ((int64_t)gx * p.n + n) * p.taps + tap;
-            const i32x4* wp = reinterpret_cast<const i32x4*>(p.wc + row * kGroupBytes);
+        const int64_t wrow = ((int64_t)gx * p.n + n) * p.taps + tap;
+        const i32x4* wp = reinterpret_cast<const i32x4*>(p.wc + wrow * kGroupBytes) + half * 2;
+        const i32x4 w0 = wp[0], w1 = wp[1];
+        const uint32_t wscale = reinterpret_cast<const uint32_t*>(p.ws)[wrow];
+        i32x4 x0 = {}, x1 = {};
+        uint32_t xscale = 0;
+        if constexpr (kOwn) {
+            const int piece = lane & 15, col = gx * kGroup + piece * 8;
+            Eight<X> v[8];  // rows lane / 16 + 0, 4, .. 28: all loads before the first use
+            int at[8];
+            const int i0 = lane >> 4;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = wp[i];
-            wscale = reinterpret_cast<const int*>(p.ws)[row];
-        }
-        if (have) {  // a tap outside the entry meets zeros
+            for (int k = 0; k < 8; ++k) {
+                if (4 * k >= rows) break;
+                const int64_t from = row_at[4 * k + i0];
+                const bool inside = (unsigned)(row_t[4 * k + i0] + shift) < (unsigned)p.T;
+                at[k] = inside ? col : max(col, p.cols);  // behind the row's end: zeros
+                v[k] = fetch_eight<false>(static_cast<const X*>(p.x) + from + (inside ? shift * p.xr.row_stride : 0), at[k], p.cols);
+            }
+            const bool ragged = p.taps > 1 || (gx + 1) * kGroup > p.cols;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                if (4 * k >= rows) break;
+                if (ragged) v[k] = place_eight<false>(v[k], at[k], p.cols);
+                int byte;
+                const uint32_t c = quantise_eight(v[k], &byte);
+                // piece q of 16 bytes of row i at place q ^ (i / 4 % 4)
+                codes[wave][4 * k + i0][(((piece >> 2) ^ k) & 3) * 4 + (piece & 3)] = c;
+                if ((piece & 3) == 0) scales[wave][4 * k + i0][piece >> 2] = (uint8_t)byte;
+            }
+            // the wave's own LDS: its queue keeps the order, the compiler the wait
+            __builtin_amdgcn_wave_barrier();
+            const int place = r >> 2 & 3;
+            x0 = *reinterpret_cast<const i32x4*>(&codes[wave][r][((half * 2) ^ place) * 4]);
+            x1 = *reinterpret_cast<const i32x4*>(&codes[wave][r][((half * 2 + 1) ^ place) * 4]);
+            xscale = *reinterpret_cast<const uint32_t*>(&scales[wave][r][0]);
+            __builtin_amdgcn_wave_barrier();
+        } else if ((unsigned)(t + shift) < (unsigned)p.T) {
             const int64_t row = (int64_t)gx * p.rows + m + shift;
-            const i32x4* xp = reinterpret_cast<const i32x4*>(p.xc + row * kGroupBytes);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = xp[i];
-            xscale = reinterpret_cast<const int*>(p.xs)[row];
+            const i32x4* xp = reinterpret_cast<const i32x4*>(p.xc + row * kGroupBytes) + half * 2;
+            x0 = xp[0], x1 = xp[1];
+            xscale = reinterpret_cast<const uint32_t*>(p.xs)[row];
         }
-        acc = step<0>(w[0], x[0], wscale, xscale, acc);
-        acc = step<1>(w[1], x[1], wscale, xscale, acc);
-        acc = step<2>(w[2], x[2], wscale, xscale, acc);
-        acc = step<3>(w[3], x[3], wscale, xscale, acc);
+        // lane l takes, of row l % 32, the blocks 2 * (l / 32) and + 1 in the two steps
+        const int ws = wscale >> (half * 16), xs = xscale >> (half * 16);
+        acc = step<0>(w0, x0, ws, xs, acc);
+        acc = step<1>(w1, x1, ws, xs, acc);
     }
 #pragma unroll
     for (int i = 0; i < 16; ++i) sums[wave][r][8 * (i >> 2) + 4 * half + (i & 3)] = acc[i];
     __syncthreads();
-    for (int e = threadIdx.x; e < 1024; e += WAVES * 64) {
+    for (int e = threadIdx.x; e < 32 * rows; e += WAVES * 64) {
         const int mm = e >> 5, nn = e & 31;
-        if (m0 + mm >= p.rows || n0 + nn >= p.n) continue;
+        if (n0 + nn >= p.n) continue;
         float v = sums[0][mm][nn];
 #pragma unroll
         for (int k = 1; k < WAVES; ++k) v += sums[k][mm][nn];
         if (p.bias) v += load_float(p.bias, p.bias_type, n0 + nn);
-        v = at_least(v, p.least);
-        store_float(p.y, p.y_type, (int64_t)(m0 + mm) * p.n + n0 + nn, v);
+        store_float(p.y, p.y_type, (int64_t)(m0 + mm) * p.n + n0 + nn, at_least(v, p.least));
     }
 }
-
 
 // ---------------------------------------------------------------------------
 // the product, large: 256 x 256 tiles staged through LDS
@@ -599,13 +649,39 @@ unsigned span_blocks(int rows, int groups) { return (unsigned)((rows + 15) / 16)
 int quantise(const void* x, int type, Rows xr, int rows, int cols, uint8_t* codes, uint8_t* scales, hipStream_t st) {
     const int groups = (cols + kGroup - 1) / kGroup;
     const dim3 grid(span_blocks(rows, groups)), block(256);
+    auto launch = [&](auto* typed) {
+        using T = std::remove_const_t<std::remove_pointer_t<decltype(typed)>>;
+        if (cols < 8)
+            hipLaunchKernelGGL((quantise_kernel<T, true>), grid, block, 0, st, typed, xr, rows, cols, groups, codes, scales);
+        else
+            hipLaunchKernelGGL((quantise_kernel<T, false>), grid, block, 0, st, typed, xr, rows, cols, groups, codes, scales);
+    };
     if (type == GLV_F32)
-        hipLaunchKernelGGL(quantise_kernel<float>, grid, block, 0, st, (const float*)x, xr, rows, cols, groups, codes, scales);
+        launch(static_cast<const float*>(x));
     else if (type == GLV_BF16)
-        hipLaunchKernelGGL(quantise_kernel<bf16>, grid, block, 0, st, (const bf16*)x, xr, rows, cols, groups, codes, scales);
+        launch(static_cast<const bf16*>(x));
     else
-        hipLaunchKernelGGL(quantise_kernel<f16>, grid, block, 0, st, (const f16*)x, xr, rows, cols, groups, codes, scales);
+        launch(static_cast<const f16*>(x));
     return launch_status("quantise_kernel");
+}
+
+template <typename X>
+void launch_direct(const Product& p, unsigned tiles, hipStream_t st) {
+    if (p.taps * p.groups <= 4)
+        hipLaunchKernelGGL((product_direct_kernel<X, 4>), dim3(tiles), dim3(256), 0, st, p);
+    else
+        hipLaunchKernelGGL((product_direct_kernel<X, 8>), dim3(tiles), dim3(512), 0, st, p);
+}
+
+// Whether a product quantises its activations itself: every tile of 32 columns of y does so anew, for
+// every tap, against a launch and a workspace less.  It does while a wave's walk stays within 16 pieces
+// of four rows of a group (32 x 1024 x 4096, 32 pieces: 9.9 us against 7.1 in two launches; 32 x 4096 x 1024,
+// 8 pieces: 4.8 against 5.7) and all tiles together within 8 M columns of x (865 x 256 x 1024, 7 M: 5.0
+// against 6.5; 2000 x 500 x 500, 16 M: 8.1 against 7.8, float32 12.2 against 8.1).
+bool quantised_in_product(int64_t rows, int cols, int n_out, int taps) {
+    const int64_t groups = (int64_t)taps * ((cols + kGroup - 1) / kGroup);
+    const int64_t pieces = ((groups + 7) / 8) * (rows < 32 ? (rows + 3) / 4 : 8);
+    return cols >= 8 && pieces <= 16 && rows * cols * taps * ((n_out + 31) / 32) <= (int64_t)8 << 20;
 }
 
 // Row counts and widths are ints in the kernels, row * groups is formed in 64 bits, and every
@@ -646,7 +722,7 @@ extern "C" int glv_mxfp4_quantize(const void* x_dev, int x_type, int batch, int 
     if (misaligned(x_dev, x_type == GLV_F32 ? 4 : 2)) return report(GLV_ERR_INVALID, "%s: x is not aligned to its elements", what);
     rc = check_quantised(what, codes_dev, scales_dev);
     if (rc != GLV_OK) return rc;
-    return quantise(x_dev, x_type, Rows{batch_stride, row_stride, rows}, (int)all, cols, codes_dev, scales_dev,
+    return quantise(x_dev, x_type, Rows{batch_stride, row_stride, rows, batch == 1}, (int)all, cols, codes_dev, scales_dev,
                     (hipStream_t)stream);
 }
 
@@ -676,7 +752,7 @@ extern "C" int glv_mxfp4_dequantize(const uint8_t* codes_dev, const uint8_t* sca
 extern "C" int64_t glv_mxfp4_product_workspace(int x_type, int batch, int rows, int cols, int n_out, int taps) {
     if (batch < 0 || rows < 0 || n_out < 0 || taps < 1 || cols < 1 || cols > kMaxCols) return -1;
     if ((int64_t)batch * rows > kMaxRows || !(float_type(x_type) || x_type == GLV_MXFP4)) return -1;
-    if (x_type == GLV_MXFP4) return 0;
+    if (x_type == GLV_MXFP4 || quantised_in_product((int64_t)batch * rows, cols, n_out, taps)) return 0;
     return quantised_bytes((int64_t)batch * rows, (cols + kGroup - 1) / kGroup);
 }
 
@@ -716,10 +792,22 @@ extern "C" int glv_mxfp4_product(const void* x_dev, const uint8_t* x_scales_dev,
     p.wc = w_codes_dev, p.ws = w_scales_dev;
     p.bias = bias_dev, p.bias_type = bias_type, p.least = activation == GLV_ACT_RELU ? 0.f : -__builtin_huge_valf();
     p.y = y_dev, p.y_type = y_type;
+    // unused waves cost nothing but their launch; more of them shorten the walk over the groups
+    const int64_t tiles = ((all + 31) / 32) * (int64_t)((n_out + 31) / 32);
+    if (tiles > INT32_MAX) return report(GLV_ERR_INVALID, "%s: rows x n_out too large for one call", what);
     if (x_type == GLV_MXFP4) {
         rc = check_quantised(what, x_dev, x_scales_dev);
         if (rc != GLV_OK) return rc;
         p.xc = static_cast<const uint8_t*>(x_dev), p.xs = x_scales_dev;
+    } else if (quantised_in_product(all, cols, n_out, taps)) {
+        p.x = x_dev, p.xr = Rows{x_batch_stride, x_row_stride, rows, batch == 1}, p.cols = cols;
+        if (x_type == GLV_F32)
+            launch_direct<float>(p, (unsigned)tiles, st);
+        else if (x_type == GLV_BF16)
+            launch_direct<bf16>(p, (unsigned)tiles, st);
+        else
+            launch_direct<f16>(p, (unsigned)tiles, st);
+        return launch_status("product_direct_kernel");
     } else {
         const int64_t need = quantised_bytes(all, p.groups);
         if (!workspace_dev || workspace_bytes < need)
@@ -728,7 +816,7 @@ extern "C" int glv_mxfp4_product(const void* x_dev, const uint8_t* x_scales_dev,
         if (misaligned(workspace_dev, 16)) return report(GLV_ERR_INVALID, "%s: the workspace is not 16-byte aligned", what);
         uint8_t* codes = static_cast<uint8_t*>(workspace_dev);
         uint8_t* scales = codes + all * p.groups * kGroupBytes;
-        rc = quantise(x_dev, x_type, Rows{x_batch_stride, x_row_stride, rows}, p.rows, cols, codes, scales, st);
+        rc = quantise(x_dev, x_type, Rows{x_batch_stride, x_row_stride, rows, batch == 1}, p.rows, cols, codes, scales, st);
         if (rc != GLV_OK) return rc;
         p.xc = codes, p.xs = scales;
     }
@@ -741,8 +829,6 @@ extern "C" int glv_mxfp4_product(const void* x_dev, const uint8_t* x_scales_dev,
         const int64_t wide = ((all + 255) / 256) * ((n_out + 255) / 256);
         return wide >= 256 && p.taps * p.groups >= 16 ? launch_tiled<4>(p, st) : launch_tiled<2>(p, st);
     }
-    const int64_t tiles = ((all + 31) / 32) * ((n_out + 31) / 32);
-    if (tiles > INT32_MAX) return report(GLV_ERR_INVALID, "%s: rows x n_out too large for one call", what);
-    hipLaunchKernelGGL(product_direct_kernel<4>, dim3((unsigned)tiles), dim3(256), 0, st, p);
+    launch_direct<void>(p, (unsigned)tiles, st);
     return launch_status("product_direct_kernel");
 }
