@@ -554,16 +554,18 @@ def test_c_entries_validate_before_any_device_call():
         return lib.glv_mxfp4_product(x, xs, kind, batch, rows, cols, rows * cols, cols, wc, ws, n, taps, dilation, bias,
                                      bias_kind, act, y, y_kind, work, size, None)
 
-    for kw in (dict(x=None), dict(wc=None), dict(ws=None), dict(y=None), dict(work=None), dict(size=8), dict(kind=4),
+    for kw in (dict(x=None), dict(wc=None), dict(ws=None), dict(y=None), dict(rows=64, cols=4096, work=None), dict(rows=64, cols=4096, size=8),
+               dict(kind=4),
                dict(kind=3), dict(y_kind=3), dict(act=2), dict(taps=0), dict(dilation=0), dict(n=-1), dict(cols=0), dict(rows=-1),
                dict(taps=1 << 14), dict(taps=2, dilation=(1 << 24) + 1), dict(n=(1 << 18) + 1), dict(y=odd), dict(bias=odd), dict(x=odd),
-               dict(bias=a, bias_kind=3), dict(wc=ctypes.c_void_p(4104)), dict(work=ctypes.c_void_p(4104)),
+               dict(bias=a, bias_kind=3), dict(wc=ctypes.c_void_p(4104)),
+               dict(rows=64, cols=4096, work=ctypes.c_void_p(4104)),
                dict(kind=3, xs=a, x=ctypes.c_void_p(4104)), dict(taps=128, n=1 << 18)):
         assert product(**kw) == -1, kw
         assert b"glv_mxfp4_product" in lib.glv_last_error()
     assert product(rows=0, x=None, y=None, work=None) == 0 and product(n=0, wc=None) == 0
     size = lib.glv_mxfp4_product_workspace
-    assert size(0, 1, 4, 32, 8, 1) > 0 and size(3, 1, 4, 32, 8, 1) == 0
+    assert size(0, 1, 64, 4096, 8, 1) > 0 and size(3, 1, 64, 4096, 8, 1) == 0
     assert size(9, 1, 4, 32, 8, 1) == -1 and size(0, 1, 4, 0, 8, 1) == -1 and size(0, 1 << 13, 1 << 13, 32, 8, 1) == -1
 
     def norm(u=a, kind=0, batch=1, rows=4, cols=32, vkind=0, post=1, pw=None, eps=1e-5, gate=None, gate_col=1, scale=None, res=None,

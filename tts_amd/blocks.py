@@ -24,22 +24,30 @@ _NORMS = {"layer": 1, "rms": 2}
 _GROUP = 128  # columns that share one dword of scales
 
 
+# The calls below take a few microseconds on the host, as much as a small launch on the device, so
+# the checks are written to cost little when nothing is wrong.
+_current_device = torch.cuda.current_device
+_current_stream = torch._C._cuda_getCurrentRawStream  # the handle alone, without a Stream object around it
+
+
 def _launch(device, entry, *args):
     """entry(*args, stream) with `device` current, on torch's current stream of it."""
     index = device.index
-    if torch.cuda.current_device() == index:
-        rc = entry(*args, torch.cuda.current_stream(index).cuda_stream)
+    if _current_device() == index:
+        rc = entry(*args, _current_stream(index))
     else:
         with torch.cuda.device(index):
-            rc = entry(*args, torch.cuda.current_stream(index).cuda_stream)
+            rc = entry(*args, _current_stream(index))
     if rc:
         _lib.check(rc)
 
 
 def _check(t, name, device=None):
+    """The element type's number, after the checks that every float input passes."""
     if not isinstance(t, torch.Tensor):
         raise ValueError(f"{name} must be a tensor, got {type(t).__name__}")
-    if t.dtype not in _TYPES:
+    kind = _TYPES.get(t.dtype)
+    if kind is None:
         raise ValueError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
     if not t.is_cuda:
         raise ValueError(f"{name} must be on a ROCm GPU (there is no CPU fallback), got {t.device}")
@@ -47,26 +55,33 @@ def _check(t, name, device=None):
         raise ValueError(f"{name} is on {t.device}, not on {device}")
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} requires a gradient: this operator is for inference (use torch.no_grad() or detach)")
+    return kind
 
 
 def _vector(t, name, n, device):
-    _check(t, name, device)
+    """(n,) vector as (tensor, number of its type); the tensor is contiguous."""
+    kind = _check(t, name, device)
     if t.dim() != 1 or t.shape[0] != n:
         raise ValueError(f"{name} must have shape ({n},), got {tuple(t.shape)}")
-    return t if t.stride(0) == 1 or n == 1 else t.contiguous()
+    return (t if t.stride(0) == 1 or n == 1 else t.contiguous()), kind
 
 
-def _rows(x):
-    """x as (batch, rows, cols) with a contiguous last dimension; a copy only where no view will do."""
-    if x.dim() == 1:
-        x = x[None, None]
-    elif x.dim() == 2:
-        x = x[None]
-    elif x.dim() > 3:
-        x = x.reshape(-1, x.shape[-2], x.shape[-1]) if x.numel() else x.new_empty((0, *x.shape[-2:]))
-    if x.stride(2) != 1 and x.shape[2] > 1:
+def _rows(x, shape):
+    """(tensor, batch, rows, batch stride, row stride) of x as (batch, rows, cols) with a contiguous last
+    dimension; a copy only where no view will do."""
+    dims = len(shape)
+    if dims > 3:
+        x = x.reshape(-1, shape[-2], shape[-1]) if x.numel() else x.new_empty((0, shape[-2], shape[-1]))
+        shape, dims = x.shape, 3
+    strides = x.stride()
+    if strides[-1] != 1 and shape[-1] > 1:
         x = x.contiguous()
-    return x
+        strides = x.stride()
+    if dims == 2:
+        return x, 1, shape[0], 0, strides[0]
+    if dims == 3:
+        return x, shape[0], shape[1], strides[0], strides[1]
+    return x, 1, 1, 0, 0
 
 
 class MXFP4Tensor:
@@ -93,22 +108,31 @@ class MXFP4Tensor:
             raise ValueError(f"codes on {codes.device} but scales on {scales.device}")
         self.shape, self.codes, self.scales = shape, codes, scales
 
+    @classmethod
+    def _of(cls, shape, codes, scales):
+        """From parts that are known to fit."""
+        self = object.__new__(cls)
+        self.shape, self.codes, self.scales = shape, codes, scales
+        return self
+
     @property
     def device(self):
         return self.codes.device
 
     def to(self, device):
-        return MXFP4Tensor(self.shape, self.codes.to(device), self.scales.to(device))
+        return MXFP4Tensor._of(self.shape, self.codes.to(device), self.scales.to(device))
 
     def dequantize(self, dtype=torch.float32):
         """The values the codes stand for, exact in float32 and bfloat16 (float16: within its range)."""
-        if dtype not in _TYPES:
+        kind = _TYPES.get(dtype)
+        if kind is None:
             raise ValueError(f"dtype must be float32, bfloat16 or float16, got {dtype}")
-        if not self.codes.is_cuda:
+        codes, shape = self.codes, self.shape
+        if not codes.is_cuda:
             raise ValueError(f"the tensor must be on a ROCm GPU (there is no CPU fallback), got {self.device}")
-        out = torch.empty(self.shape, dtype=dtype, device=self.device)
-        _launch(self.device, _lib.load().glv_mxfp4_dequantize, self.codes.data_ptr(), self.scales.data_ptr(),
-                self.codes.shape[1], self.shape[-1], _TYPES[dtype], out.data_ptr())
+        out = codes.new_empty(shape, dtype=dtype)
+        _launch(codes.device, _lib.load().glv_mxfp4_dequantize, codes.data_ptr(), self.scales.data_ptr(), codes.shape[1],
+                shape[-1], kind, out.data_ptr())
         return out
 
     def __repr__(self):
@@ -120,60 +144,65 @@ def mxfp4_quantize(x):
     at least 2 ** -127; an element goes to the nearest code, ties to the even one, beyond 6 to 6.  A block
     that holds an infinity or a NaN reads back as NaN.  Any strides; a last dimension that is not
     contiguous is copied first."""
-    _check(x, "x")
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError(f"x must have a last dimension of at least 1, got {tuple(x.shape)}")
-    v = _rows(x)
-    rows, groups = v.shape[0] * v.shape[1], -(-v.shape[2] // _GROUP)
-    codes = torch.empty((groups, rows, 64), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((groups, rows, 4), dtype=torch.uint8, device=x.device)
-    _launch(x.device, _lib.load().glv_mxfp4_quantize, v.data_ptr(), _TYPES[x.dtype], *v.shape, v.stride(0), v.stride(1),
+    kind, shape = _check(x, "x"), x.shape
+    if len(shape) < 1 or shape[-1] < 1:
+        raise ValueError(f"x must have a last dimension of at least 1, got {tuple(shape)}")
+    v, batch, rows, batch_stride, row_stride = _rows(x, shape)
+    cols = shape[-1]
+    groups = -(-cols // _GROUP)
+    codes = x.new_empty((groups, batch * rows, 64), dtype=torch.uint8)
+    scales = x.new_empty((groups, batch * rows, 4), dtype=torch.uint8)
+    _launch(x.device, _lib.load().glv_mxfp4_quantize, v.data_ptr(), kind, batch, rows, cols, batch_stride, row_stride,
             codes.data_ptr(), scales.data_ptr())
-    return MXFP4Tensor(x.shape, codes, scales)
+    return MXFP4Tensor._of(shape, codes, scales)
 
 
 def _product(x, weight, bias, taps, dilation, activation, out_dtype):
-    if activation not in _ACTIVATIONS:
+    act = _ACTIVATIONS.get(activation)
+    if act is None:
         raise ValueError(f"activation must be None or 'relu', got {activation!r}")
-    n, cols = weight.shape[0], weight.shape[-1]
-    device = weight.device
+    wshape, codes = weight.shape, weight.codes
+    n, cols, device, shape = wshape[0], wshape[-1], codes.device, x.shape
+    scales, batch_stride, row_stride = None, 0, 0
     if isinstance(x, MXFP4Tensor):
-        if not x.codes.is_cuda:
-            raise ValueError(f"x must be on a ROCm GPU (there is no CPU fallback), got {x.device}")
-        if x.device != device:
-            raise ValueError(f"x is on {x.device}, not on {device}")
-        kind, data, scales = _MXFP4, x.codes.data_ptr(), x.scales.data_ptr()
-        rows = x.shape[-2] if len(x.shape) > 1 else 1
-        batch = x.codes.shape[1] // rows if rows else 0
-        strides = (0, 0)
+        like = x.codes
+        if not like.is_cuda:
+            raise ValueError(f"x must be on a ROCm GPU (there is no CPU fallback), got {like.device}")
+        if like.device != device:
+            raise ValueError(f"x is on {like.device}, not on {device}")
+        kind, scales = _MXFP4, x.scales.data_ptr()
+        rows = shape[-2] if len(shape) > 1 else 1
+        batch = like.shape[1] // rows if rows else 0
     else:
-        _check(x, "x", device)
-        if x.dim() < 1:
+        like, kind = x, _check(x, "x", device)
+        if len(shape) < 1:
             raise ValueError("x must have at least one dimension")
-    if x.shape[-1] != cols:
-        raise ValueError(f"x has {x.shape[-1]} columns but the weight {cols}")
-    if not isinstance(x, MXFP4Tensor):
-        v = _rows(x)
-        kind, data, scales = _TYPES[x.dtype], v.data_ptr(), None
-        batch, rows, strides = v.shape[0], v.shape[1], (v.stride(0), v.stride(1))
-    if taps == 1:  # rows of a linear layer need no batch entries, and fewer entries are fewer edges
-        if strides[0] == rows * strides[1] or batch == 1:
-            batch, rows = 1, batch * rows
+    if shape[-1] != cols:
+        raise ValueError(f"x has {shape[-1]} columns but the weight {cols}")
+    if scales is None:
+        like, batch, rows, batch_stride, row_stride = _rows(x, shape)
+    if taps == 1 and batch != 1 and batch_stride == rows * row_stride:
+        batch, rows = 1, batch * rows  # rows of a linear layer need no entries
     if out_dtype is None:
-        out_dtype = torch.float32 if kind == _MXFP4 else x.dtype
-    if out_dtype not in _TYPES:
-        raise ValueError(f"out_dtype must be float32, bfloat16 or float16, got {out_dtype}")
+        out_dtype, out_kind = (torch.float32, 0) if kind == _MXFP4 else (x.dtype, kind)
+    else:
+        out_kind = _TYPES.get(out_dtype)
+        if out_kind is None:
+            raise ValueError(f"out_dtype must be float32, bfloat16 or float16, got {out_dtype}")
+    bias_ptr, bias_kind = None, 0
     if bias is not None:
-        bias = _vector(bias, "bias", n, device)
+        bias, bias_kind = _vector(bias, "bias", n, device)
+        bias_ptr = bias.data_ptr()
     lib = _lib.load()
-    y = torch.empty((*x.shape[:-1], n), dtype=out_dtype, device=device)
+    y = like.new_empty((*shape[:-1], n), dtype=out_dtype)
     need = lib.glv_mxfp4_product_workspace(kind, batch, rows, cols, n, taps)
-    work = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
-    _launch(device, lib.glv_mxfp4_product, data, scales, kind, batch, rows, cols, strides[0], strides[1],
-            weight.codes.data_ptr(), weight.scales.data_ptr(), n, taps, dilation,
-            None if bias is None else bias.data_ptr(), 0 if bias is None else _TYPES[bias.dtype],
-            _ACTIVATIONS[activation], y.data_ptr(), _TYPES[out_dtype], None if work is None else work.data_ptr(),
-            max(need, 0))
+    work_ptr = None
+    if need > 0:
+        work = like.new_empty(need, dtype=torch.uint8)
+        work_ptr = work.data_ptr()
+    _launch(device, lib.glv_mxfp4_product, like.data_ptr(), scales, kind, batch, rows, cols, batch_stride, row_stride,
+            codes.data_ptr(), weight.scales.data_ptr(), n, taps, dilation, bias_ptr, bias_kind, act, y.data_ptr(),
+            out_kind, work_ptr, need if need > 0 else 0)
     return y
 
 
@@ -240,63 +269,74 @@ def block_norm(u, *, post=None, gate=None, scale=None, residual=None, pre=None):
     pre       `Norm` the next block starts with, or None
 
     Statistics are 32 bits; y enters `pre` before it is rounded to u's type.  C is at most 32768."""
-    _check(u, "u")
-    if u.dim() < 1 or u.shape[-1] < 1:
-        raise ValueError(f"u must have a last dimension of at least 1, got {tuple(u.shape)}")
-    device, dtype, cols = u.device, u.dtype, u.shape[-1]
-    v = _rows(u)
-    batch, rows, _ = v.shape
-    vector_type = None
-    vectors = []
+    kind, shape, device, dtype = _check(u, "u"), u.shape, u.device, u.dtype
+    if len(shape) < 1 or shape[-1] < 1:
+        raise ValueError(f"u must have a last dimension of at least 1, got {tuple(shape)}")
+    cols = shape[-1]
+    v, batch, rows, u_batch, u_row = _rows(u, shape)
+    vector_kind = None
+
+    def vector(t, name):
+        nonlocal vector_kind
+        if t is None:
+            return None
+        t, k = _vector(t, name, cols, device)
+        if k not in (0, kind) or vector_kind not in (None, k):
+            raise ValueError(f"weights, biases and scale must all be float32 or all {dtype}, got {t.dtype}")
+        vector_kind = k
+        held.append(t)
+        return t.data_ptr()
+
+    held = []  # contiguous copies live until the launch
+    sides = []
     for side, norm in (("post", post), ("pre", pre)):
-        if norm is not None and not isinstance(norm, Norm):
+        if norm is None:
+            sides.append((0, None, None, 0.0))
+        elif isinstance(norm, Norm):
+            sides.append((_NORMS[norm.kind], vector(norm.weight, f"{side}.weight"), vector(norm.bias, f"{side}.bias"),
+                          norm.eps))
+        else:
             raise ValueError(f"{side} must be a Norm or None, got {type(norm).__name__}")
-        for name in ("weight", "bias"):
-            t = getattr(norm, name, None)
-            vectors.append(None if t is None else _vector(t, f"{side}.{name}", cols, device))
-    factor = 1.0
+    scale_ptr, factor = None, 1.0
     if isinstance(scale, torch.Tensor):
-        vectors.append(_vector(scale, "scale", cols, device))
-    else:
-        vectors.append(None)
-        if scale is not None:
-            factor = float(scale)
-    for t in vectors:
-        if t is not None:
-            if t.dtype not in (torch.float32, dtype) or vector_type not in (None, t.dtype):
-                raise ValueError(f"weights, biases and scale must all be float32 or all {dtype}, got {t.dtype}")
-            vector_type = t.dtype
-    post_w, post_b, pre_w, pre_b, scale_vec = (None if t is None else t.data_ptr() for t in vectors)
-    g = r = None
-    g_strides, r_strides = (0, 0, 1), (0, 0)
+        scale_ptr = vector(scale, "scale")
+    elif scale is not None:
+        factor = float(scale)
+    gate_ptr, gate_strides = None, (0, 0, 1)
     if gate is not None:
         _check(gate, "gate", device)
         if gate.dtype != dtype:
             raise ValueError(f"gate must be {dtype} like u, got {gate.dtype}")
-        try:
-            g = gate.expand(u.shape)
-        except RuntimeError:
-            raise ValueError(f"gate of shape {tuple(gate.shape)} does not broadcast to {tuple(u.shape)}") from None
-        g = g[None, None] if g.dim() == 1 else g[None] if g.dim() == 2 else g
-        if g.dim() > 3:
+        g = gate
+        if len(shape) > 3:  # leading dimensions that a broadcast gate need not collapse like u's
+            try:
+                g = g.expand(shape)
+            except RuntimeError:
+                raise ValueError(f"gate of shape {tuple(gate.shape)} does not broadcast to {tuple(shape)}") from None
             g = g.reshape(batch, rows, cols) if g.numel() else g.new_empty((batch, rows, cols))
-        if g.stride(2) not in (0, 1) and cols > 1:
+        full = (batch, rows, cols)[-len(shape):]
+        if g.dim() > len(full) or any(a != 1 and a != b for a, b in zip(reversed(g.shape), reversed(full))):
+            raise ValueError(f"gate of shape {tuple(gate.shape)} does not broadcast to {tuple(shape)}")
+        if g.dim() and g.shape[-1] != 1 and g.stride(-1) != 1:
             g = g.contiguous()
-        g_strides = (g.stride(0), g.stride(1), g.stride(2) if cols > 1 else 0)
+        gate_strides = [0, 0, 0]
+        for i, (size, stride) in enumerate(zip(reversed(g.shape), reversed(g.stride()))):
+            if size != 1:
+                gate_strides[2 - i] = stride
+        gate_ptr = g.data_ptr()
+        held.append(g)
+    res_ptr, res_strides = None, (0, 0)
     if residual is not None:
         _check(residual, "residual", device)
-        if residual.dtype != dtype or residual.shape != u.shape:
-            raise ValueError(f"residual must be {dtype} {tuple(u.shape)} like u, got {residual.dtype} "
+        if residual.dtype != dtype or residual.shape != shape:
+            raise ValueError(f"residual must be {dtype} {tuple(shape)} like u, got {residual.dtype} "
                              f"{tuple(residual.shape)}")
-        r = _rows(residual)
-        r_strides = (r.stride(0), r.stride(1))
-    y = torch.empty(u.shape, dtype=dtype, device=device)
-    z = torch.empty(u.shape, dtype=dtype, device=device) if pre is not None else None
-    _launch(device, _lib.load().glv_block_norm, v.data_ptr(), _TYPES[dtype], batch, rows, cols, v.stride(0), v.stride(1),
-            _TYPES[torch.float32 if vector_type is None else vector_type],
-            0 if post is None else _NORMS[post.kind], post_w, post_b, 0.0 if post is None else post.eps,
-            None if g is None else g.data_ptr(), *g_strides, scale_vec, factor,
-            None if r is None else r.data_ptr(), *r_strides,
-            0 if pre is None else _NORMS[pre.kind], pre_w, pre_b, 0.0 if pre is None else pre.eps,
-            y.data_ptr(), None if z is None else z.data_ptr())
+        r, _, _, *res_strides = _rows(residual, shape)
+        res_ptr = r.data_ptr()
+        held.append(r)
+    y = v.new_empty(shape)
+    z = v.new_empty(shape) if pre is not None else None
+    _launch(device, _lib.load().glv_block_norm, v.data_ptr(), kind, batch, rows, cols, u_batch, u_row, vector_kind or 0,
+            *sides[0], gate_ptr, *gate_strides, scale_ptr, factor, res_ptr, *res_strides, *sides[1], y.data_ptr(),
+            None if z is None else z.data_ptr())
     return y if z is None else (y, z)
