@@ -24,110 +24,134 @@ struct BlockNorm {
     int rows, T, cols;
 };
 
-__device__ inline float wave_sum(float v) {
-    v += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0xB1, 0xf, 0xf, true));
-    v += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x4E, 0xf, 0xf, true));
-    v += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x141, 0xf, 0xf, true));
-    v += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x140, 0xf, 0xf, true));
-    const unsigned b = __builtin_bit_cast(unsigned, v);
-    const auto s16 = __builtin_amdgcn_permlane16_swap(b, b, false, false);
-    v = __builtin_bit_cast(float, (unsigned)s16[0]) + __builtin_bit_cast(float, (unsigned)s16[1]);
-    const unsigned c = __builtin_bit_cast(unsigned, v);
-    const auto s32 = __builtin_amdgcn_permlane32_swap(c, c, false, false);
-    return __builtin_bit_cast(float, (unsigned)s32[0]) + __builtin_bit_cast(float, (unsigned)s32[1]);
+template <int CTRL>
+__device__ inline float plus_dpp(float v) {
+    return v + __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
 }
 
-// sum over the TPR threads of a row; `slot` is a different array for every use within a kernel
-template <int TPR>
-__device__ inline float row_sum(float v, float* slot) {
-    v = wave_sum(v);
-    if constexpr (TPR > 64) {
-        const int wave = threadIdx.x >> 6;
-        if ((threadIdx.x & 63) == 0) slot[wave] = v;
-        __syncthreads();
-        v = 0.f;
-#pragma unroll
-        for (int i = 0; i < TPR / 64; ++i) v += slot[i];
+// sum over LANES neighbouring lanes (16, 32 or 64), in all of them
+template <int LANES>
+__device__ inline float lanes_sum(float v) {
+    v = plus_dpp<0xB1>(v);   // quad_perm 1,0,3,2
+    v = plus_dpp<0x4E>(v);   // quad_perm 2,3,0,1
+    v = plus_dpp<0x141>(v);  // row_half_mirror
+    v = plus_dpp<0x140>(v);  // row_mirror
+    if constexpr (LANES >= 32) {
+        const unsigned b = __builtin_bit_cast(unsigned, v);
+        const auto s = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+        v = __builtin_bit_cast(float, (unsigned)s[0]) + __builtin_bit_cast(float, (unsigned)s[1]);
+    }
+    if constexpr (LANES == 64) {
+        const unsigned b = __builtin_bit_cast(unsigned, v);
+        const auto s = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+        v = __builtin_bit_cast(float, (unsigned)s[0]) + __builtin_bit_cast(float, (unsigned)s[1]);
     }
     return v;
 }
 
-// x <- Norm(x) for the row held as V pieces of eight per thread; `valid` counts columns
-template <typename W, int TPR, int V, bool NARROW>
+// Lanes of a row: 16, 32 or 64 of a wave, or (0) all waves of the workgroup, at most 16.
+template <int LANES>
+struct Row {
+    int lane, lanes;
+    float* slots;  // LANES 0: 16 for every sum of the kernel, used once each
+
+    __device__ float sum(float v, int use) const {
+        if constexpr (LANES > 0) return lanes_sum<LANES>(v);
+        v = lanes_sum<64>(v);
+        float* s = slots + 16 * use;
+        const int at = threadIdx.x & 15;
+        if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
+        __syncthreads();
+        return lanes_sum<16>(at < lanes >> 6 ? s[at] : 0.f);
+    }
+};
+
+// x <- Norm(x) for the row held as V pieces of eight a lane, zeros behind `cols`
+template <typename W, int LANES, int V, bool NARROW>
 __device__ inline void normalise(float (&x)[V][8], int kind, const void* weight, const void* bias, float eps, int cols,
-                                 int lane, float* slot) {
+                                 const Row<LANES>& row, int use) {
     const float inv = 1.f / (float)cols;
+    Eight<W> w[V], b[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {  // under way while the sums are formed
+        const int col = (v * row.lanes + row.lane) * 8;
+        if (weight) w[v] = fetch_eight<NARROW>(static_cast<const W*>(weight), col, cols);
+        if (bias) b[v] = fetch_eight<NARROW>(static_cast<const W*>(bias), col, cols);
+    }
     if (kind == GLV_NORM_LAYER) {
         float s = 0.f;
 #pragma unroll
         for (int v = 0; v < V; ++v)
 #pragma unroll
             for (int i = 0; i < 8; ++i) s += x[v][i];
-        const float mean = row_sum<TPR>(s, slot) * inv;
+        const float mean = row.sum(s, use) * inv;
 #pragma unroll
         for (int v = 0; v < V; ++v)
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                x[v][i] = (v * TPR + lane) * 8 + i < cols ? x[v][i] - mean : 0.f;
+                x[v][i] = (v * row.lanes + row.lane) * 8 + i < cols ? x[v][i] - mean : 0.f;
     }
     float q = 0.f;
 #pragma unroll
     for (int v = 0; v < V; ++v)
 #pragma unroll
         for (int i = 0; i < 8; ++i) q += x[v][i] * x[v][i];
-    const float r = rsqrtf(row_sum<TPR>(q, slot + TPR / 64) * inv + eps);
+    const float r = rsqrtf(row.sum(q, use + 1) * inv + eps);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        const int col = (v * TPR + lane) * 8;
-        if (col < cols) {
-            Eight<W> w, b;
-            if (weight) w = load_eight<NARROW>(static_cast<const W*>(weight), col, cols);
-            if (bias) b = load_eight<NARROW>(static_cast<const W*>(bias), col, cols);
+        const int col = (v * row.lanes + row.lane) * 8;
+        if (weight) w[v] = place_eight<NARROW>(w[v], col, cols);
+        if (bias) b[v] = place_eight<NARROW>(b[v], col, cols);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                float t = x[v][i] * r;
-                if (weight) t *= (float)w.v[i];
-                if (bias) t += (float)b.v[i];
-                x[v][i] = t;
-            }
+        for (int i = 0; i < 8; ++i) {
+            float t = x[v][i] * r;
+            if (weight) t *= (float)w[v].v[i];
+            if (bias) t += (float)b[v].v[i];
+            x[v][i] = t;
         }
     }
 }
 
-// TPR threads a row, V pieces of eight columns a thread
-template <typename T, typename W, int TPR, int V, bool NARROW = false>
-__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void block_norm_kernel(BlockNorm p) {
-    __shared__ float slots[TPR > 64 ? 4 * (TPR / 64) : 1];
-    constexpr int kRows = TPR < 256 ? 256 / TPR : 1;
-    const int row = blockIdx.x * kRows + (TPR < 256 ? threadIdx.x / TPR : 0);
-    const int lane = threadIdx.x % TPR;
-    if (row >= p.rows) return;  // whole waves: a row is one wave here, or the workgroup
-    const int b = row / p.T, t = row - b * p.T;
+// V pieces of eight columns a lane
+template <typename T, typename W, int LANES, int V, bool NARROW = false>
+__global__ __launch_bounds__(LANES > 0 ? 256 : 1024) void block_norm_kernel(BlockNorm p) {
+    __shared__ float slots[LANES > 0 ? 1 : 64];
+    constexpr int kRows = LANES > 0 ? 256 / LANES : 1;
+    const int index = blockIdx.x * kRows + (LANES > 0 ? threadIdx.x / LANES : 0);
+    // the rows behind the last are computed from the last, for their lanes take part in the sums' exchanges
+    const int at = min(index, p.rows - 1);
+    const Row<LANES> row{LANES > 0 ? (int)threadIdx.x % LANES : (int)threadIdx.x, LANES > 0 ? LANES : (int)blockDim.x, slots};
+    const int b = at / p.T, t = at - b * p.T;
     const T* u = static_cast<const T*>(p.u) + b * p.u_batch + t * p.u_row;
     const T* gate = p.gate ? static_cast<const T*>(p.gate) + b * p.gate_batch + t * p.gate_row : nullptr;
     const T* res = p.residual ? static_cast<const T*>(p.residual) + b * p.res_batch + t * p.res_row : nullptr;
-    const int64_t out = (int64_t)row * p.cols;
+    const int64_t out = (int64_t)at * p.cols;
+    const int cols = p.cols, store_cols = index < p.rows ? p.cols : 0;
 
     Eight<T> ur[V], gr[V], rr[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        const int col = (v * TPR + lane) * 8;
-        ur[v] = load_eight<NARROW>(u, col, p.cols);
-        if (gate && p.gate_col) gr[v] = load_eight<NARROW>(gate, col, p.cols);
-        if (res) rr[v] = load_eight<NARROW>(res, col, p.cols);
+        const int col = (v * row.lanes + row.lane) * 8;
+        ur[v] = fetch_eight<NARROW>(u, col, cols);
+        if (gate && p.gate_col) gr[v] = fetch_eight<NARROW>(gate, col, cols);
+        if (res) rr[v] = fetch_eight<NARROW>(res, col, cols);
     }
+    const float row_factor = p.scale * (gate && !p.gate_col ? (float)gate[0] : 1.f);
     float x[V][8];
 #pragma unroll
-    for (int v = 0; v < V; ++v)
+    for (int v = 0; v < V; ++v) {
+        const Eight<T> placed = place_eight<NARROW>(ur[v], (v * row.lanes + row.lane) * 8, cols);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[v][i] = (float)ur[v].v[i];
-    if (p.post) normalise<W, TPR, V, NARROW>(x, p.post, p.post_w, p.post_b, p.post_eps, p.cols, lane, slots);
-    const float row_factor = p.scale * (gate && !p.gate_col ? (float)gate[0] : 1.f);
+        for (int i = 0; i < 8; ++i) x[v][i] = (float)placed.v[i];
+    }
+    if (p.post) normalise<W, LANES, V, NARROW>(x, p.post, p.post_w, p.post_b, p.post_eps, cols, row, 0);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        const int col = (v * TPR + lane) * 8;
+        const int col = (v * row.lanes + row.lane) * 8;
         Eight<W> sv;
-        if (p.scale_vec) sv = load_eight<NARROW>(static_cast<const W*>(p.scale_vec), col, p.cols);
+        if (p.scale_vec) sv = load_eight<NARROW>(static_cast<const W*>(p.scale_vec), col, cols);
+        if (gate && p.gate_col) gr[v] = place_eight<NARROW>(gr[v], col, cols);
+        if (res) rr[v] = place_eight<NARROW>(rr[v], col, cols);
         Eight<T> o;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -135,38 +159,41 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void block_norm_kernel(Block
             if (gate && p.gate_col) k *= (float)gr[v].v[i];
             if (p.scale_vec) k *= (float)sv.v[i];
             if (res) k += (float)rr[v].v[i];
-            x[v][i] = col + i < p.cols ? k : 0.f;
+            x[v][i] = col + i < cols ? k : 0.f;
             o.v[i] = (T)k;
         }
-        store_eight(static_cast<T*>(p.y) + out + col, o, p.cols - col);
+        store_eight(static_cast<T*>(p.y) + out + col, o, store_cols - col);
     }
     if (!p.pre) return;
-    normalise<W, TPR, V, NARROW>(x, p.pre, p.pre_w, p.pre_b, p.pre_eps, p.cols, lane, slots + 2 * (TPR / 64));
+    normalise<W, LANES, V, NARROW>(x, p.pre, p.pre_w, p.pre_b, p.pre_eps, cols, row, 2);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        const int col = (v * TPR + lane) * 8;
+        const int col = (v * row.lanes + row.lane) * 8;
         Eight<T> o;
 #pragma unroll
         for (int i = 0; i < 8; ++i) o.v[i] = (T)x[v][i];
-        store_eight(static_cast<T*>(p.z) + out + col, o, p.cols - col);
+        store_eight(static_cast<T*>(p.z) + out + col, o, store_cols - col);
     }
 }
 
 template <typename T, typename W>
 void launch(const BlockNorm& p, hipStream_t st) {
-    const dim3 by4((p.rows + 3) / 4), by1(p.rows);
+    const int pieces = (p.cols + 7) / 8;
+    auto rows_a_wave = [&](int lanes) { return dim3((unsigned)(((int64_t)p.rows * lanes + 255) / 256)); };
     if (p.cols < 8)
-        hipLaunchKernelGGL((block_norm_kernel<T, W, 64, 1, true>), by4, dim3(256), 0, st, p);
-    else if (p.cols <= 512)
-        hipLaunchKernelGGL((block_norm_kernel<T, W, 64, 1>), by4, dim3(256), 0, st, p);
-    else if (p.cols <= 1024)
-        hipLaunchKernelGGL((block_norm_kernel<T, W, 64, 2>), by4, dim3(256), 0, st, p);
-    else if (p.cols <= 4096)
-        hipLaunchKernelGGL((block_norm_kernel<T, W, 256, 2>), by1, dim3(256), 0, st, p);
-    else if (p.cols <= 8192)
-        hipLaunchKernelGGL((block_norm_kernel<T, W, 256, 4>), by1, dim3(256), 0, st, p);
+        hipLaunchKernelGGL((block_norm_kernel<T, W, 16, 1, true>), rows_a_wave(16), dim3(256), 0, st, p);
+    else if (pieces <= 16)
+        hipLaunchKernelGGL((block_norm_kernel<T, W, 16, 1>), rows_a_wave(16), dim3(256), 0, st, p);
+    else if (pieces <= 32)
+        hipLaunchKernelGGL((block_norm_kernel<T, W, 32, 1>), rows_a_wave(32), dim3(256), 0, st, p);
+    else if (pieces <= 64)
+        hipLaunchKernelGGL((block_norm_kernel<T, W, 64, 1>), rows_a_wave(64), dim3(256), 0, st, p);
+    else if (pieces <= 128)
+        hipLaunchKernelGGL((block_norm_kernel<T, W, 64, 2>), rows_a_wave(64), dim3(256), 0, st, p);
+    else if (pieces <= 2048)
+        hipLaunchKernelGGL((block_norm_kernel<T, W, 0, 2>), dim3(p.rows), dim3((pieces + 127) / 128 * 64), 0, st, p);
     else
-        hipLaunchKernelGGL((block_norm_kernel<T, W, 1024, 4>), by1, dim3(1024), 0, st, p);
+        hipLaunchKernelGGL((block_norm_kernel<T, W, 0, 4>), dim3(p.rows), dim3((pieces + 255) / 256 * 64), 0, st, p);
 }
 
 constexpr int kMaxCols = 32768;         // 1024 threads of 32 columns
