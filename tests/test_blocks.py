@@ -494,8 +494,7 @@ def test_other_streams_at_once_give_the_same_bits():
 # -- refusals -----------------------------------------------------------------------------
 def packed(shape, device="cpu"):
     rows, groups = int(np.prod(shape[:-1])), -(-shape[-1] // 128)
-    return MXFP4Tensor(shape, torch.zeros(groups, rows, 64, dtype=torch.uint8, device=device),
-                       torch.zeros(groups, rows, 4, dtype=torch.uint8, device=device))
+    return MXFP4Tensor(shape, torch.zeros(groups * rows * 68, dtype=torch.uint8, device=device))
 
 
 def test_refusals_without_gpu():
@@ -520,12 +519,15 @@ def test_refusals_without_gpu():
     for bad in (dict(kind="batch"), dict(eps=-1.0), dict(eps=float("nan"))):
         with pytest.raises(ValueError):
             Norm(**bad)
-    with pytest.raises(ValueError, match="codes"):
-        MXFP4Tensor((5, 40), torch.zeros(5, 64, dtype=torch.uint8), torch.zeros(1, 5, 4, dtype=torch.uint8))
-    with pytest.raises(ValueError, match="scales"):
-        MXFP4Tensor((5, 40), torch.zeros(1, 5, 64, dtype=torch.uint8), torch.zeros(5, 1, 4, dtype=torch.uint8))
+    for data in (torch.zeros(5 * 68 - 1, dtype=torch.uint8), torch.zeros(5 * 68), torch.zeros(1, 5 * 68, dtype=torch.uint8),
+                 torch.zeros(10 * 68, dtype=torch.uint8)[::2]):
+        with pytest.raises(ValueError, match="data must be"):
+            MXFP4Tensor((5, 40), data)
+    with pytest.raises(ValueError, match="16 bytes"):
+        MXFP4Tensor((5, 40), torch.zeros(5 * 68 + 1, dtype=torch.uint8)[1:])
     with pytest.raises(ValueError, match="last dimension"):
-        MXFP4Tensor((5, 0), torch.zeros(0, 5, 64, dtype=torch.uint8), torch.zeros(0, 5, 4, dtype=torch.uint8))
+        MXFP4Tensor((5, 0), torch.zeros(0, dtype=torch.uint8))
+    assert w.codes.shape == (1, 5, 64) and w.scales.shape == (1, 5, 4) and w.to("cpu").shape == (5, 40)
     for name in ("MXFP4Tensor", "Norm", "block_norm", "mxfp4_conv1d", "mxfp4_linear", "mxfp4_quantize"):
         assert name in tts_amd.__all__
 
@@ -594,6 +596,11 @@ def test_refusals_on_the_device():
     with torch.no_grad():
         assert mxfp4_linear(grad, w).shape == (3, 5)
     bad = [
+        (lambda: mxfp4_linear([1.0], w), "x must be a tensor"),
+        (lambda: mxfp4_conv1d([1.0], wc), "x must be a tensor"),
+        (lambda: block_norm(x, gate=[1.0]), "gate must be a tensor"),
+        (lambda: block_norm(x, residual=1.0), "residual must be a tensor"),
+        (lambda: mxfp4_linear(x, w, 1.0), "bias must be a tensor"),
         (lambda: mxfp4_linear(x[:, :39], w), "39 columns"),
         (lambda: mxfp4_linear(mxfp4_quantize(x[:, :39]), w), "39 columns"),
         (lambda: mxfp4_linear(x, w, torch.ones(6, device="cuda")), "bias must have shape"),

@@ -66,24 +66,22 @@ class _MaskedBiLSTM(nn.Module):
 
 class _SequenceConv(nn.Conv1d):
     """Conv1D(padding='same') whose weight can be held in MXFP4 beside the float one.  The quantised
-    copy lies in buffers outside the state dict: it moves with the module, and checkpoints stay what
+    copy lies in a buffer outside the state dict: it moves with the module, and checkpoints stay what
     they were."""
 
     def __init__(self, in_dim, out_dim, kernel, dilation=1):
         super().__init__(in_dim, out_dim, kernel, padding="same", dilation=dilation)
-        self.register_buffer("mxfp4_codes", None, persistent=False)
-        self.register_buffer("mxfp4_scales", None, persistent=False)
+        self.register_buffer("mxfp4_data", None, persistent=False)
 
     def quantize(self, on):
-        q = mxfp4_quantize(self.weight.detach().permute(0, 2, 1)) if on else None
-        self.mxfp4_codes, self.mxfp4_scales = (q.codes, q.scales) if on else (None, None)
+        self.mxfp4_data = mxfp4_quantize(self.weight.detach().permute(0, 2, 1)).data if on else None
 
     def sequence(self, x, relu=False):  # (B, T, C)
-        if self.mxfp4_codes is None:
+        if self.mxfp4_data is None:
             y = self(x.transpose(1, 2))
             return (F.relu(y) if relu else y).transpose(1, 2)
         n, c, taps = self.weight.shape
-        weight = MXFP4Tensor((n, taps, c) if taps > 1 else (n, c), self.mxfp4_codes, self.mxfp4_scales)
+        weight = MXFP4Tensor((n, taps, c) if taps > 1 else (n, c), self.mxfp4_data)
         activation = "relu" if relu else None
         if taps == 1:
             return mxfp4_linear(x, weight, self.bias, activation=activation)
@@ -100,7 +98,7 @@ class _ConvNorm(nn.Module):
 
     def forward(self, x):  # (B, T, C)
         y = self.conv.sequence(x, relu=True)
-        if self.conv.mxfp4_codes is None:
+        if self.conv.mxfp4_data is None:
             return self.norm(y)
         return block_norm(y, post=Norm(self.norm.weight, self.norm.bias, eps=_KERAS_EPS))
 
@@ -214,7 +212,7 @@ class FastSpeechAcousticModel(nn.Module):
 
     def _refresh_mxfp4(self, *unused):
         for layer in self._mxfp4_layers():
-            if layer.mxfp4_codes is not None:
+            if layer.mxfp4_data is not None:
                 layer.quantize(True)
 
     # -- Keras checkpoint layout ------------------------------------------------------

@@ -30,9 +30,8 @@ _current_device = torch.cuda.current_device
 _current_stream = torch._C._cuda_getCurrentRawStream  # the handle alone, without a Stream object around it
 
 
-def _launch(device, entry, *args):
-    """entry(*args, stream) with `device` current, on torch's current stream of it."""
-    index = device.index
+def _launch(index, entry, *args):
+    """entry(*args, stream) with device `index` current, on torch's current stream of it."""
     if _current_device() == index:
         rc = entry(*args, _current_stream(index))
     else:
@@ -42,26 +41,28 @@ def _launch(device, entry, *args):
         _lib.check(rc)
 
 
-def _check(t, name, device=None):
-    """The element type's number, after the checks that every float input passes."""
+def _check(t, name, index=None):
+    """The element type's number, after the checks that every float input passes; `index` is the device
+    that the call runs on."""
     if not isinstance(t, torch.Tensor):
         raise ValueError(f"{name} must be a tensor, got {type(t).__name__}")
     kind = _TYPES.get(t.dtype)
     if kind is None:
         raise ValueError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
-    if not t.is_cuda:
+    at = t.get_device()
+    if at < 0:
         raise ValueError(f"{name} must be on a ROCm GPU (there is no CPU fallback), got {t.device}")
-    if device is not None and t.device != device:
-        raise ValueError(f"{name} is on {t.device}, not on {device}")
+    if index is not None and at != index:
+        raise ValueError(f"{name} is on {t.device}, not on cuda:{index}")
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} requires a gradient: this operator is for inference (use torch.no_grad() or detach)")
     return kind
 
 
-def _vector(t, name, n, device):
-    """(n,) vector as (tensor, number of its type); the tensor is contiguous."""
-    kind = _check(t, name, device)
-    if t.dim() != 1 or t.shape[0] != n:
+def _vector(t, name, n, index):
+    """(n,) vector as (contiguous tensor, number of its type)."""
+    kind = _check(t, name, index)
+    if t.shape != (n,):
         raise ValueError(f"{name} must have shape ({n},), got {tuple(t.shape)}")
     return (t if t.stride(0) == 1 or n == 1 else t.contiguous()), kind
 
@@ -88,51 +89,58 @@ class MXFP4Tensor:
     """A tensor in MXFP4: along the last dimension every 32 elements share one power of two (E8M0)
     and an element is a 4-bit code for 0, 0.5, 1, 1.5, 2, 3, 4 or 6 with a sign (E2M1).
 
-    shape   of the tensor it stands for
-    codes   (groups, rows, 64) uint8, a group being 128 columns, two to a byte, the even one low
-    scales  (groups, rows, 4) uint8, biased exponents of the group's four blocks; 255 is a NaN block
+    shape   of the tensor it stands for; with rows = the product of all dimensions but the last and
+            groups of 128 columns, the last one padded with zeros,
+    data    the storage, (groups * rows * 68,) uint8 on one device: all codes, then all scales
+    codes   (groups, rows, 64) view of it, two codes to a byte, the even column low
+    scales  (groups, rows, 4) view of it, biased exponents of a group's four blocks; 255 is a NaN block
     """
 
-    __slots__ = ("shape", "codes", "scales")
+    __slots__ = ("shape", "data", "rows", "groups")
 
-    def __init__(self, shape, codes, scales):
+    def __init__(self, shape, data):
         shape = torch.Size(shape)
         if len(shape) < 1 or shape[-1] < 1:
             raise ValueError(f"an MXFP4 tensor needs a last dimension of at least 1, got {tuple(shape)}")
         rows, groups = shape[:-1].numel(), -(-shape[-1] // _GROUP)
-        for t, name, want in ((codes, "codes", (groups, rows, 64)), (scales, "scales", (groups, rows, 4))):
-            if t.dtype != torch.uint8 or tuple(t.shape) != want or not t.is_contiguous():
-                raise ValueError(f"{name} must be a contiguous uint8 tensor of shape {want}, got {t.dtype} "
-                                 f"{tuple(t.shape)}")
-        if codes.device != scales.device:
-            raise ValueError(f"codes on {codes.device} but scales on {scales.device}")
-        self.shape, self.codes, self.scales = shape, codes, scales
-
-    @classmethod
-    def _of(cls, shape, codes, scales):
-        """From parts that are known to fit."""
-        self = object.__new__(cls)
-        self.shape, self.codes, self.scales = shape, codes, scales
-        return self
+        size = groups * rows * 68
+        if data.dtype != torch.uint8 or data.shape != (size,) or not data.is_contiguous():
+            raise ValueError(f"data must be a contiguous uint8 tensor of shape ({size},), got {data.dtype} "
+                             f"{tuple(data.shape)}")
+        if data.data_ptr() % 16:
+            raise ValueError("data must start at a multiple of 16 bytes")
+        self.shape, self.data, self.rows, self.groups = shape, data, rows, groups
 
     @property
     def device(self):
-        return self.codes.device
+        return self.data.device
+
+    @property
+    def codes(self):
+        return self.data[: self.groups * self.rows * 64].view(self.groups, self.rows, 64)
+
+    @property
+    def scales(self):
+        return self.data[self.groups * self.rows * 64:].view(self.groups, self.rows, 4)
+
+    def _pointers(self):
+        at = self.data.data_ptr()
+        return at, at + self.groups * self.rows * 64
 
     def to(self, device):
-        return MXFP4Tensor._of(self.shape, self.codes.to(device), self.scales.to(device))
+        return MXFP4Tensor(self.shape, self.data.to(device))
 
     def dequantize(self, dtype=torch.float32):
         """The values the codes stand for, exact in float32 and bfloat16 (float16: within its range)."""
         kind = _TYPES.get(dtype)
         if kind is None:
             raise ValueError(f"dtype must be float32, bfloat16 or float16, got {dtype}")
-        codes, shape = self.codes, self.shape
-        if not codes.is_cuda:
+        data, shape = self.data, self.shape
+        index = data.get_device()
+        if index < 0:
             raise ValueError(f"the tensor must be on a ROCm GPU (there is no CPU fallback), got {self.device}")
-        out = codes.new_empty(shape, dtype=dtype)
-        _launch(codes.device, _lib.load().glv_mxfp4_dequantize, codes.data_ptr(), self.scales.data_ptr(), codes.shape[1],
-                shape[-1], kind, out.data_ptr())
+        out = data.new_empty(shape, dtype=dtype)
+        _launch(index, _lib.load().glv_mxfp4_dequantize, *self._pointers(), self.rows, shape[-1], kind, out.data_ptr())
         return out
 
     def __repr__(self):
@@ -149,38 +157,39 @@ def mxfp4_quantize(x):
         raise ValueError(f"x must have a last dimension of at least 1, got {tuple(shape)}")
     v, batch, rows, batch_stride, row_stride = _rows(x, shape)
     cols = shape[-1]
-    groups = -(-cols // _GROUP)
-    codes = x.new_empty((groups, batch * rows, 64), dtype=torch.uint8)
-    scales = x.new_empty((groups, batch * rows, 4), dtype=torch.uint8)
-    _launch(x.device, _lib.load().glv_mxfp4_quantize, v.data_ptr(), kind, batch, rows, cols, batch_stride, row_stride,
-            codes.data_ptr(), scales.data_ptr())
-    return MXFP4Tensor._of(shape, codes, scales)
+    q = object.__new__(MXFP4Tensor)
+    q.shape, q.rows, q.groups = shape, batch * rows, -(-cols // _GROUP)
+    q.data = x.new_empty(q.rows * q.groups * 68, dtype=torch.uint8)
+    _launch(x.get_device(), _lib.load().glv_mxfp4_quantize, v.data_ptr(), kind, batch, rows, cols, batch_stride,
+            row_stride, *q._pointers())
+    return q
 
 
 def _product(x, weight, bias, taps, dilation, activation, out_dtype):
     act = _ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"activation must be None or 'relu', got {activation!r}")
-    wshape, codes = weight.shape, weight.codes
-    n, cols, device, shape = wshape[0], wshape[-1], codes.device, x.shape
+    wshape = weight.shape
+    n, cols, index = wshape[0], wshape[-1], weight.data.get_device()
     scales, batch_stride, row_stride = None, 0, 0
     if isinstance(x, MXFP4Tensor):
-        like = x.codes
-        if not like.is_cuda:
+        like, shape = x.data, x.shape
+        if like.get_device() < 0:
             raise ValueError(f"x must be on a ROCm GPU (there is no CPU fallback), got {like.device}")
-        if like.device != device:
-            raise ValueError(f"x is on {like.device}, not on {device}")
-        kind, scales = _MXFP4, x.scales.data_ptr()
+        if like.get_device() != index:
+            raise ValueError(f"x is on {like.device}, not on cuda:{index}")
+        kind, (data, scales) = _MXFP4, x._pointers()
         rows = shape[-2] if len(shape) > 1 else 1
-        batch = like.shape[1] // rows if rows else 0
+        batch = x.rows // rows if rows else 0
     else:
-        like, kind = x, _check(x, "x", device)
+        kind, shape = _check(x, "x", index), x.shape
         if len(shape) < 1:
             raise ValueError("x must have at least one dimension")
     if shape[-1] != cols:
         raise ValueError(f"x has {shape[-1]} columns but the weight {cols}")
     if scales is None:
         like, batch, rows, batch_stride, row_stride = _rows(x, shape)
+        data = like.data_ptr()
     if taps == 1 and batch != 1 and batch_stride == rows * row_stride:
         batch, rows = 1, batch * rows  # rows of a linear layer need no entries
     if out_dtype is None:
@@ -191,7 +200,7 @@ def _product(x, weight, bias, taps, dilation, activation, out_dtype):
             raise ValueError(f"out_dtype must be float32, bfloat16 or float16, got {out_dtype}")
     bias_ptr, bias_kind = None, 0
     if bias is not None:
-        bias, bias_kind = _vector(bias, "bias", n, device)
+        bias, bias_kind = _vector(bias, "bias", n, index)
         bias_ptr = bias.data_ptr()
     lib = _lib.load()
     y = like.new_empty((*shape[:-1], n), dtype=out_dtype)
@@ -200,16 +209,16 @@ def _product(x, weight, bias, taps, dilation, activation, out_dtype):
     if need > 0:
         work = like.new_empty(need, dtype=torch.uint8)
         work_ptr = work.data_ptr()
-    _launch(device, lib.glv_mxfp4_product, like.data_ptr(), scales, kind, batch, rows, cols, batch_stride, row_stride,
-            codes.data_ptr(), weight.scales.data_ptr(), n, taps, dilation, bias_ptr, bias_kind, act, y.data_ptr(),
-            out_kind, work_ptr, need if need > 0 else 0)
+    _launch(index, lib.glv_mxfp4_product, data, scales, kind, batch, rows, cols, batch_stride, row_stride,
+            *weight._pointers(), n, taps, dilation, bias_ptr, bias_kind, act, y.data_ptr(), out_kind, work_ptr,
+            need if need > 0 else 0)
     return y
 
 
 def _check_weight(weight, dims, shape):
     if not isinstance(weight, MXFP4Tensor) or len(weight.shape) != dims:
         raise ValueError(f"weight must be an MXFP4Tensor of shape {shape} (mxfp4_quantize), got {weight!r}")
-    if not weight.codes.is_cuda:
+    if weight.data.get_device() < 0:
         raise ValueError(f"weight must be on a ROCm GPU (there is no CPU fallback), got {weight.device}")
 
 
@@ -234,6 +243,8 @@ def mxfp4_conv1d(x, weight, bias=None, *, dilation=1, activation=None, out_dtype
     weight is an `MXFP4Tensor` of shape (N, taps, C): a torch.nn.Conv1d weight is
     ``mxfp4_quantize(conv.weight.permute(0, 2, 1))``.  The other arguments are `mxfp4_linear`'s."""
     _check_weight(weight, 3, "(N, taps, C)")
+    if not isinstance(x, (torch.Tensor, MXFP4Tensor)):
+        raise ValueError(f"x must be a tensor, got {type(x).__name__}")
     if len(x.shape) not in (2, 3):
         raise ValueError(f"x must be (B, T, C) or (T, C), got {tuple(x.shape)}")
     if weight.shape[1] < 1:
@@ -269,7 +280,7 @@ def block_norm(u, *, post=None, gate=None, scale=None, residual=None, pre=None):
     pre       `Norm` the next block starts with, or None
 
     Statistics are 32 bits; y enters `pre` before it is rounded to u's type.  C is at most 32768."""
-    kind, shape, device, dtype = _check(u, "u"), u.shape, u.device, u.dtype
+    kind, shape, index, dtype = _check(u, "u"), u.shape, u.get_device(), u.dtype
     if len(shape) < 1 or shape[-1] < 1:
         raise ValueError(f"u must have a last dimension of at least 1, got {tuple(shape)}")
     cols = shape[-1]
@@ -280,7 +291,7 @@ def block_norm(u, *, post=None, gate=None, scale=None, residual=None, pre=None):
         nonlocal vector_kind
         if t is None:
             return None
-        t, k = _vector(t, name, cols, device)
+        t, k = _vector(t, name, cols, index)
         if k not in (0, kind) or vector_kind not in (None, k):
             raise ValueError(f"weights, biases and scale must all be float32 or all {dtype}, got {t.dtype}")
         vector_kind = k
@@ -304,7 +315,7 @@ def block_norm(u, *, post=None, gate=None, scale=None, residual=None, pre=None):
         factor = float(scale)
     gate_ptr, gate_strides = None, (0, 0, 1)
     if gate is not None:
-        _check(gate, "gate", device)
+        _check(gate, "gate", index)
         if gate.dtype != dtype:
             raise ValueError(f"gate must be {dtype} like u, got {gate.dtype}")
         g = gate
@@ -327,7 +338,7 @@ def block_norm(u, *, post=None, gate=None, scale=None, residual=None, pre=None):
         held.append(g)
     res_ptr, res_strides = None, (0, 0)
     if residual is not None:
-        _check(residual, "residual", device)
+        _check(residual, "residual", index)
         if residual.dtype != dtype or residual.shape != shape:
             raise ValueError(f"residual must be {dtype} {tuple(shape)} like u, got {residual.dtype} "
                              f"{tuple(residual.shape)}")
@@ -336,7 +347,7 @@ def block_norm(u, *, post=None, gate=None, scale=None, residual=None, pre=None):
         held.append(r)
     y = v.new_empty(shape)
     z = v.new_empty(shape) if pre is not None else None
-    _launch(device, _lib.load().glv_block_norm, v.data_ptr(), kind, batch, rows, cols, u_batch, u_row, vector_kind or 0,
+    _launch(index, _lib.load().glv_block_norm, v.data_ptr(), kind, batch, rows, cols, u_batch, u_row, vector_kind or 0,
             *sides[0], gate_ptr, *gate_strides, scale_ptr, factor, res_ptr, *res_strides, *sides[1], y.data_ptr(),
             None if z is None else z.data_ptr())
     return y if z is None else (y, z)

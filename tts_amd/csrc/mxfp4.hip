@@ -185,6 +185,14 @@ __device__ inline void store_float(void* p, int type, int64_t i, float v) {
 // max(v, least) that keeps a NaN: the rectifier with least = 0, nothing with -infinity
 __device__ inline float at_least(float v, float least) { return __builtin_elementwise_maximum(v, least); }
 
+// Between a wave's writes to its own LDS and other lanes' reads of them (and back): the LDS queue keeps
+// a wave's accesses in order, this keeps the compiler from changing it.
+__device__ inline void wave_lds_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 __device__ inline i32x8 widen(i32x4 v) { return __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1); }
 
 // acc += W (32 rows) * X (32 rows)^T over 64 columns: lane l holds 32 of them, one block, of row l % 32;
@@ -258,13 +266,12 @@ __global__ __launch_bounds__(WAVES * 64) void product_direct_kernel(Product p) {
                 codes[wave][4 * k + i0][(((piece >> 2) ^ k) & 3) * 4 + (piece & 3)] = c;
                 if ((piece & 3) == 0) scales[wave][4 * k + i0][piece >> 2] = (uint8_t)byte;
             }
-            // the wave's own LDS: its queue keeps the order, the compiler the wait
-            __builtin_amdgcn_wave_barrier();
+            wave_lds_fence();
             const int place = r >> 2 & 3;
             x0 = *reinterpret_cast<const i32x4*>(&codes[wave][r][((half * 2) ^ place) * 4]);
             x1 = *reinterpret_cast<const i32x4*>(&codes[wave][r][((half * 2 + 1) ^ place) * 4]);
             xscale = *reinterpret_cast<const uint32_t*>(&scales[wave][r][0]);
-            __builtin_amdgcn_wave_barrier();
+            wave_lds_fence();
         } else if ((unsigned)(t + shift) < (unsigned)p.T) {
             const int64_t row = (int64_t)gx * p.rows + m + shift;
             const i32x4* xp = reinterpret_cast<const i32x4*>(p.xc + row * kGroupBytes) + half * 2;
@@ -370,6 +377,7 @@ __device__ inline void store_rows(const Product& p, const f32x16 (&acc)[4], cons
             const int at = (i * 32 + 8 * q + 4 * half) * sizeof(T);
             *reinterpret_cast<Four*>(lds + r * (kPieces * 16) + (((at >> 4) ^ (r & (kPieces - 1))) << 4) + (at & 15)) = four;
         }
+    wave_lds_fence();
     constexpr int kRows = 64 / kPieces;  // rows that one instruction covers
     const int piece = lane % kPieces, sub = lane / kPieces;
     const int n = n0 + piece * kEach;
@@ -628,7 +636,7 @@ __global__ __launch_bounds__(Tiling<MW>::kThreads, 2) void product_tiled_kernel(
             store_rows<bf16, MW == 2>(p, part, bias + nw, own, m0 + mw + j * 32, n0 + nw, lane);
         else
             store_rows<f16, MW == 2>(p, part, bias + nw, own, m0 + mw + j * 32, n0 + nw, lane);
-        // one wave's reads and the next pass's writes of its own LDS stay in order in the LDS queue
+        wave_lds_fence();
     }
 }
 
@@ -665,6 +673,8 @@ int quantise(const void* x, int type, Rows xr, int rows, int cols, uint8_t* code
     return launch_status("quantise_kernel");
 }
 
+// Four waves where there are no more groups than that, else eight (sixteen gain 0.5 us at 10 groups in
+// half precision and lose as much in float32, whose registers no longer fit).
 template <typename X>
 void launch_direct(const Product& p, unsigned tiles, hipStream_t st) {
     if (p.taps * p.groups <= 4)
@@ -792,7 +802,6 @@ extern "C" int glv_mxfp4_product(const void* x_dev, const uint8_t* x_scales_dev,
     p.wc = w_codes_dev, p.ws = w_scales_dev;
     p.bias = bias_dev, p.bias_type = bias_type, p.least = activation == GLV_ACT_RELU ? 0.f : -__builtin_huge_valf();
     p.y = y_dev, p.y_type = y_type;
-    // unused waves cost nothing but their launch; more of them shorten the walk over the groups
     const int64_t tiles = ((all + 31) / 32) * (int64_t)((n_out + 31) / 32);
     if (tiles > INT32_MAX) return report(GLV_ERR_INVALID, "%s: rows x n_out too large for one call", what);
     if (x_type == GLV_MXFP4) {
