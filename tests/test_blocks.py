@@ -491,6 +491,68 @@ def test_other_streams_at_once_give_the_same_bits():
         assert all(torch.equal(p, q) for p, q in zip(a, b))
 
 
+@gpu
+def test_calls_from_several_threads_at_once():
+    import threading
+    rng = np.random.default_rng(24)
+    w, post = mxfp4_quantize(draw(rng, 96, 96, scale=0.1)), norm_vectors(rng, "layer", 96, torch.float32)
+    xs = [draw(rng, m, 96) for m in (1, 33, 400, 2500)]
+    want = [block_norm(mxfp4_linear(x, w), post=post) for x in xs]
+    torch.cuda.synchronize()
+    got, errors = [None] * len(xs), []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    got[i] = block_norm(mxfp4_linear(xs[i], w), post=post)
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # noqa: BLE001 - reported below
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(xs))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    assert all(torch.equal(g, v) for g, v in zip(got, want))
+
+
+@gpu
+def test_arrays_beyond_32_bit_offsets():
+    """Inputs and outputs of more than 2^31 elements: their last rows against the same rows alone."""
+    rng = np.random.default_rng(25)
+    rows, cols, tail = 530000, 4100, 70
+    x = torch.zeros(rows, cols, dtype=torch.bfloat16, device="cuda")
+    assert x.numel() > 2 ** 31
+    x[-tail:] = draw(rng, tail, cols, dtype=torch.bfloat16)
+    part = x[-tail:].clone()
+    q = mxfp4_quantize(x)
+    alone = mxfp4_quantize(part)
+    assert torch.equal(q.codes[:, -tail:], alone.codes) and torch.equal(q.scales[:, -tail:], alone.scales)
+    assert not q.codes[:, :-tail].any()
+    values = q.dequantize(torch.bfloat16)
+    assert torch.equal(values[-tail:], alone.dequantize(torch.bfloat16))
+    del values
+    w = mxfp4_quantize(draw(rng, 9, cols, scale=cols ** -0.5))
+    y = mxfp4_linear(q, w)
+    check_product_on_device(y[-tail:], alone.dequantize().double(), w.dequantize().double(), None, False)
+    assert not y[:-tail].any()
+    post = norm_vectors(rng, "layer", cols, torch.float32)
+    z = block_norm(x, post=post, residual=x)
+    assert torch.equal(z[-tail:], block_norm(part, post=post, residual=part))
+    del x, q, y, z
+    # a product whose result is that long
+    m, n, k = 300000, 7300, 64
+    x, w = torch.zeros(m, k, dtype=torch.float16, device="cuda"), mxfp4_quantize(draw(rng, n, k))
+    x[-tail:] = draw(rng, tail, k, dtype=torch.float16)
+    y = mxfp4_linear(x, w)
+    assert y.numel() > 2 ** 31
+    check_product_on_device(y[-tail:], mxfp4_quantize(x[-tail:]).dequantize().double(), w.dequantize().double(), None, False)
+    assert not y[:5].any() and not y[m // 2].any()
+
+
 # -- refusals -----------------------------------------------------------------------------
 def packed(shape, device="cpu"):
     rows, groups = int(np.prod(shape[:-1])), -(-shape[-1] // 128)
