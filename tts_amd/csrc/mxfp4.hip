@@ -298,23 +298,30 @@ __global__ __launch_bounds__(WAVES * 64) void product_direct_kernel(Product p) {
 }
 
 // ---------------------------------------------------------------------------
-// the product, large: 256 x 256 tiles staged through LDS
+// the product, large: tiles staged through LDS
 // ---------------------------------------------------------------------------
-constexpr int kTileN = 256;  // rows of w of a workgroup's tile
-
-// A tile has 64 * MW rows of x and 2 * MW waves.
-template <int MW>
+// A workgroup's tile has TN rows of w and TM of x; a wave multiplies half of the w rows by 64 of x.
+template <int TM, int TN>
 struct Tiling {
-    static constexpr int kWaves = 2 * MW, kThreads = 64 * kWaves, kTileM = 64 * MW;
-    static constexpr int kStages = MW == 4 ? 4 : 3;
+    static constexpr int kWaves = TM / 32, kThreads = 64 * kWaves, kWt = TN / 64;
+    static constexpr int kStages = TM == 256 ? 4 : 3;
+    static constexpr int kWavesPerSimd = TN == 128 ? 3 : 2;
     // one stage: the codes of one group of every row of w and of x, then their scales
-    static constexpr int kW = 0, kX = kTileN * kGroupBytes, kWs = kX + kTileM * kGroupBytes, kXs = kWs + kTileN * 4;
-    static constexpr int kStage = kXs + kTileM * 4;
-    // a wave's loads for a stage: pieces of 16 rows of w and x, scales of 64 rows of w and of x
-    static constexpr int kLoadsW = kTileN / 16 / kWaves, kLoadsX = kTileM / 16 / kWaves;
-    static constexpr int kLoadsS = MW == 4 ? 1 : 2;
+    static constexpr int kW = 0, kX = TN * kGroupBytes, kWs = kX + TM * kGroupBytes, kXs = kWs + TN * 4;
+    static constexpr int kStage = kXs + TM * 4;
+    // a wave's loads for a stage: pieces of 16 rows of w and x, scales of 64 rows
+    static constexpr int kLoadsW = TN / 16 / kWaves, kLoadsX = TM / 16 / kWaves;
+    static constexpr int kLoadsS = ((TN + TM) / 64 + kWaves - 1) / kWaves;
     static constexpr int kLoads = kLoadsW + kLoadsX + kLoadsS;
 };
+
+template <int FROM, int TO, typename F>
+__device__ inline void each(F&& f) {
+    if constexpr (FROM < TO) {
+        f(std::integral_constant<int, FROM>{});
+        each<FROM + 1, TO>(f);
+    }
+}
 
 // what a lane reads where a tap leaves its entry
 __device__ __align__(64) const uint32_t g_zeros[16] = {};
@@ -350,22 +357,23 @@ __device__ inline void dword_to_lds(const uint8_t* src, uint32_t dst) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(dst), "v"(src) : "memory");
 }
 
+template <int WT>
 struct Fragments {
-    i32x4 w[4], x[2];
+    i32x4 w[WT], x[2];
 };
 
-// The wave's 32 rows (x) by 128 columns (w) of accumulators through its own 16 KB of LDS, so that
+// The wave's 32 rows (x) by 32 * WT columns (w) of accumulators through LDS of its own, so that
 // a row of y leaves in pieces of 16 bytes.  Lane l holds y[m = l % 32][8 * (e / 4) + 4 * (l / 32)
 // + e % 4] of every accumulator; piece q of row m lies at place q ^ m: reads and writes both
-// spread over the banks.  STREAM: past the L2, for products whose y is most of their traffic (8192 x
-// 8192 x 512: 40 us against 43; 55360 x 256 x 768: 13.5 against 15.4; where sums are long and L2 holds
-// the operands it costs: 8192 x 8192 x 1024 with the wide tile 62 us without, 66 with).
-template <typename T, bool STREAM>
-__device__ inline void store_rows(const Product& p, const f32x16 (&acc)[4], const float* bias, uint8_t* lds, int m0, int n0, int lane) {
-    constexpr int kPieces = 128 * sizeof(T) / 16, kEach = 16 / sizeof(T);
+// spread over the banks.  STREAM: past the L2, in the tiles for products whose y is most of their
+// traffic (128 x 256, 8192 x 8192 x 512: 40 us against 43; 55360 x 256 x 768: 13.5 against 15.4; with long
+// sums, where L2 holds the operands, it costs: 256 x 256, 8192 x 8192 x 1024: 66 against 62).
+template <typename T, bool STREAM, int WT>
+__device__ inline void store_rows(const Product& p, const f32x16 (&acc)[WT], const float* bias, uint8_t* lds, int m0, int n0, int lane) {
+    constexpr int kPieces = 32 * WT * sizeof(T) / 16, kEach = 16 / sizeof(T);
     const int r = lane & 31, half = lane >> 5;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < WT; ++i)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             struct __attribute__((aligned(4 * sizeof(T)))) Four {
@@ -385,7 +393,7 @@ __device__ inline void store_rows(const Product& p, const f32x16 (&acc)[4], cons
     auto own = [&](int row) {
         return *reinterpret_cast<const i32x4*>(lds + row * (kPieces * 16) + ((piece ^ (row & (kPieces - 1))) << 4));
     };
-    if (m0 + 32 <= p.rows && n0 + 128 <= p.n) {
+    if (m0 + 32 <= p.rows && n0 + 32 * WT <= p.n) {
         i32x4 v[32 / kRows];
 #pragma unroll
         for (int k = 0; k < 32 / kRows; ++k) v[k] = own(k * kRows + sub);
@@ -421,21 +429,22 @@ __device__ inline void arrive_and_wait() {  // all but the N youngest loads are 
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
-// Each wave multiplies 128 rows of w by 64 of x (4 x 2 accumulators of 32 x 32); two waves share the
-// rows of x.  A stage holds one group of both operands: [row][4 pieces of 16 bytes], piece q of row r
-// at place q ^ (r / 4 % 4): sixteen lanes that read one piece of sixteen rows then touch each of the
-// 64 banks once.  One stage is multiplied while the others are on their way.  A stage is two steps;
-// the barrier stands early in the second, whose products hide the first reads of the next stage.
-template <bool CONV, int MW>
-__global__ __launch_bounds__(Tiling<MW>::kThreads, 2) void product_tiled_kernel(Product p) {
-    using L = Tiling<MW>;
+// Each wave multiplies 32 * WT rows of w by 64 of x (WT x 2 accumulators of 32 x 32); two waves share
+// the rows of x.  A stage holds one group of both operands: [row][4 pieces of 16 bytes], piece q of row
+// r at place q ^ (r / 4 % 4): sixteen lanes that read one piece of sixteen rows then touch each of the
+// 64 banks once.  One stage is multiplied while the others are on their way.  A stage is two steps; the
+// barrier stands early in the second, whose products hide the first reads of the next stage.
+template <bool CONV, int TM, int TN>
+__global__ __launch_bounds__((Tiling<TM, TN>::kThreads), (Tiling<TM, TN>::kWavesPerSimd)) void product_tiled_kernel(Product p) {
+    using L = Tiling<TM, TN>;
+    constexpr int WT = L::kWt;
     __shared__ __align__(1024) uint8_t lds[L::kStages * L::kStage];
-    __shared__ __align__(16) float bias[kTileN];
+    __shared__ __align__(16) float bias[TN];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 31, half = lane >> 5;
-    const int m_tiles = (p.rows + L::kTileM - 1) / L::kTileM, n_tiles = (p.n + kTileN - 1) / kTileN;
+    const int m_tiles = (p.rows + TM - 1) / TM, n_tiles = (p.n + TN - 1) / TN;
     const Tile tile = tile_of(blockIdx.x, gridDim.x, m_tiles, n_tiles);
-    const int n0 = tile.n * kTileN, m0 = tile.m * L::kTileM;
+    const int n0 = tile.n * TN, m0 = tile.m * TM;
     const int all = p.taps * p.groups;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
 
@@ -453,13 +462,13 @@ __global__ __launch_bounds__(Tiling<MW>::kThreads, 2) void product_tiled_kernel(
         xoff[i] = m * kGroupBytes + place;
         xt[i] = CONV ? m % p.T : 0;
     }
-    // Scales: with eight waves the first four bring w's and the others x's; with four each brings 64 rows of w
-    // and, two of them twice, of x.
-    const bool first_w = MW == 2 || wave < 4;
+    // Scales, 64 rows a load: with one load a wave the first TN / 64 waves bring w's, the others x's; with two
+    // every wave brings w's and then x's (four waves for two loads of x: two of them the same).
+    const bool first_w = L::kLoadsS == 2 || wave < TN / 64;
     {
-        const int m = min(m0 + (MW == 4 ? wave - 4 : wave & 1) * 64 + lane, p.rows - 1);
+        const int m = min(m0 + (L::kLoadsS == 1 ? wave - TN / 64 : wave & (TM / 64 - 1)) * 64 + lane, p.rows - 1);
         if (first_w) soff[0] = min(n0 + wave * 64 + lane, p.n - 1) * p.taps * 4;
-        if (!first_w || MW == 2) {
+        if (!first_w || L::kLoadsS == 2) {
             soff[L::kLoadsS - 1] = m * 4;
             st = CONV ? m % p.T : 0;
         }
@@ -468,40 +477,39 @@ __global__ __launch_bounds__(Tiling<MW>::kThreads, 2) void product_tiled_kernel(
     int tap = 0, gx = 0;
     int64_t wrow = 0, xrow = 0;
     const int64_t wstep = (int64_t)p.n * p.taps;
-    // scale loads of this wave, first and last: base, bytes to the current group, bytes of a group
+    // first scale load of this wave: base, bytes to the current group, bytes of a group
     const uint8_t* sbase = first_w ? p.ws : p.xs;
     const int64_t sstep = (first_w ? wstep : p.rows) * 4;
     int64_t sat = 0;
     // the loads in order: w, x, scales; after the last one on to the next group; no branches
     auto stage_part = [&](int slot, auto part) {
         constexpr int i = part, xi = i - L::kLoadsW, si = xi - L::kLoadsX;
-        if constexpr (i < L::kLoads) {
-            const uint32_t dst = lds0 + slot * L::kStage;
-            const int shift = CONV ? tap * p.dilation - p.left : 0;
-            const uint8_t* zeros = reinterpret_cast<const uint8_t*>(g_zeros);
-            if constexpr (i < L::kLoadsW) {
-                to_lds(p.wc + wrow * kGroupBytes, woff[i], dst + L::kW + (i * L::kWaves + wave) * 1024);
-            } else if constexpr (xi < L::kLoadsX) {
-                const uint8_t* xbase = p.xc + xrow * kGroupBytes;
-                const uint32_t to = dst + L::kX + (xi * L::kWaves + wave) * 1024;
-                if (CONV) {
-                    const bool inside = (unsigned)(xt[xi] + shift) < (unsigned)p.T;
-                    to_lds(inside ? xbase + (int64_t)xoff[xi] + (int64_t)shift * kGroupBytes : zeros, to);
-                } else {
-                    to_lds(xbase, xoff[xi], to);
-                }
+        const uint32_t dst = lds0 + slot * L::kStage;
+        const int shift = CONV ? tap * p.dilation - p.left : 0;
+        const uint8_t* zeros = reinterpret_cast<const uint8_t*>(g_zeros);
+        if constexpr (i < L::kLoadsW) {
+            to_lds(p.wc + wrow * kGroupBytes, woff[i], dst + L::kW + (i * L::kWaves + wave) * 1024);
+        } else if constexpr (xi < L::kLoadsX) {
+            const uint8_t* xbase = p.xc + xrow * kGroupBytes;
+            const uint32_t to = dst + L::kX + (xi * L::kWaves + wave) * 1024;
+            if (CONV) {
+                const bool inside = (unsigned)(xt[xi] + shift) < (unsigned)p.T;
+                to_lds(inside ? xbase + (int64_t)xoff[xi] + (int64_t)shift * kGroupBytes : zeros, to);
             } else {
-                const bool of_w = MW == 4 ? first_w : si == 0;
-                const uint32_t to = dst + (MW == 4 ? L::kWs + wave * 256 : si == 0 ? L::kWs + wave * 256 : L::kXs + (wave & 1) * 256);
-                const uint8_t* from = si == 0 ? sbase + sat : p.xs + xrow * 4;
-                if (CONV) {
-                    // of w the tap's own scales; of x those of the shifted row
-                    const int own = of_w ? tap : shift;
-                    const bool inside = of_w | ((unsigned)(st + shift) < (unsigned)p.T);
-                    dword_to_lds(inside ? from + (int64_t)soff[si] + (int64_t)own * 4 : zeros, to);
-                } else {
-                    dword_to_lds(from, soff[si], to);
-                }
+                to_lds(xbase, xoff[xi], to);
+            }
+        } else {
+            // with one load a wave, x's scales follow w's as the waves follow each other
+            const bool of_w = L::kLoadsS == 1 ? first_w : si == 0;
+            const uint32_t to = dst + (si == 0 ? L::kWs + wave * 256 : L::kXs + (wave & (TM / 64 - 1)) * 256);
+            const uint8_t* from = si == 0 ? sbase + sat : p.xs + xrow * 4;
+            if (CONV) {
+                // of w the tap's own scales; of x those of the shifted row
+                const int own = of_w ? tap : shift;
+                const bool inside = of_w | ((unsigned)(st + shift) < (unsigned)p.T);
+                dword_to_lds(inside ? from + (int64_t)soff[si] + (int64_t)own * 4 : zeros, to);
+            } else {
+                dword_to_lds(from, soff[si], to);
             }
         }
         if constexpr (i == L::kLoads - 1) {
@@ -513,141 +521,131 @@ __global__ __launch_bounds__(Tiling<MW>::kThreads, 2) void product_tiled_kernel(
             sat = last ? 0 : sat + sstep;
         }
     };
-    auto stage = [&](int slot) {
-        stage_part(slot, std::integral_constant<int, 0>{});
-        stage_part(slot, std::integral_constant<int, 1>{});
-        stage_part(slot, std::integral_constant<int, 2>{});
-        stage_part(slot, std::integral_constant<int, 3>{});
-        stage_part(slot, std::integral_constant<int, 4>{});
-        stage_part(slot, std::integral_constant<int, 5>{});
-        stage_part(slot, std::integral_constant<int, 6>{});
-        stage_part(slot, std::integral_constant<int, 7>{});
-    };
 
 #pragma unroll
     for (int c = 0; c < L::kStages; ++c)
-        if (c < all) stage(c);
+        if (c < all) each<0, L::kLoads>([&](auto part) { stage_part(c, part); });
     // asked for here, used behind the loop: no wait of its own
+    static_assert(L::kThreads >= TN, "a thread for every bias");
     float own_bias = 0.f;
-    if (p.bias && n0 + (int)threadIdx.x < p.n && threadIdx.x < kTileN) own_bias = load_float(p.bias, p.bias_type, n0 + threadIdx.x);
+    if (p.bias && n0 + (int)threadIdx.x < p.n && threadIdx.x < TN) own_bias = load_float(p.bias, p.bias_type, n0 + threadIdx.x);
 
-    const int nw = (wave & 1) * 128, mw = (wave >> 1) * 64;
+    const int nw = (wave & 1) * 32 * WT, mw = (wave >> 1) * 64;
     // lane l takes, of row l % 32, the blocks 2 * (l / 32) and + 1 in the two steps
     uint32_t at[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) at[k] = ((half * 2 + k) ^ ((r >> 2) & 3)) * 16;
     const uint32_t wr = L::kW + (nw + r) * kGroupBytes, xr = L::kX + (mw + r) * kGroupBytes;
-    auto fetch_w = [&](uint32_t base, int k, int i, Fragments& f) {
-        f.w[i] = *reinterpret_cast<const i32x4*>(lds + base + wr + at[k] + i * 32 * kGroupBytes);
+    // the reads of a step in the order of their use: w0 x0 w1 .. x1
+    constexpr int kReads = WT + 2, kProducts = WT * 2;
+    auto fetch = [&](uint32_t base, int k, auto q, Fragments<WT>& f) {
+        constexpr bool x = q == 1 || q == WT + 1;
+        constexpr int i = q == 0 ? 0 : x ? q / (WT + 1) : q - 1;
+        const i32x4 v = *reinterpret_cast<const i32x4*>(lds + base + (x ? xr : wr) + at[k] + i * 32 * kGroupBytes);
+        if constexpr (x)
+            f.x[i] = v;
+        else
+            f.w[i] = v;
     };
-    auto fetch_x = [&](uint32_t base, int k, int j, Fragments& f) {
-        f.x[j] = *reinterpret_cast<const i32x4*>(lds + base + xr + at[k] + j * 32 * kGroupBytes);
-    };
-    int ws[4], xs[2], wnext[4], xnext[2];
+    int ws[WT], xs[2], wnext[WT], xnext[2];
     const uint32_t wsr = L::kWs + (nw + r) * 4, xsr = L::kXs + (mw + r) * 4;
     auto fetch_scales = [&](uint32_t base) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) wnext[i] = *reinterpret_cast<const int*>(lds + base + wsr + i * 128);
+        for (int i = 0; i < WT; ++i) wnext[i] = *reinterpret_cast<const int*>(lds + base + wsr + i * 128);
 #pragma unroll
         for (int j = 0; j < 2; ++j) xnext[j] = *reinterpret_cast<const int*>(lds + base + xsr + j * 128);
     };
-    f32x16 acc[4][2] = {};
-    auto multiply = [&](auto S, int i, int j, const Fragments& f) {
+    f32x16 acc[WT][2] = {};
+    auto multiply = [&](auto S, auto q, const Fragments<WT>& f) {
+        constexpr int i = q % WT, j = q / WT;
         acc[i][j] = step<S>(f.w[i], f.x[j], ws[i], xs[j], acc[i][j]);
     };
 
-    Fragments fa, fb;
+    Fragments<WT> fa, fb;
     if (all >= L::kStages)
         arrive_and_wait<(L::kStages - 1) * L::kLoads>();
     else
         arrive_and_wait<0>();
-    for (int i = 0; i < 4; ++i) fetch_w(0, 0, i, fa);
-    for (int j = 0; j < 2; ++j) fetch_x(0, 0, j, fa);
+    each<0, kReads>([&](auto q) { fetch(0, 0, q, fa); });
     fetch_scales(0);
     int slot = 0;
     uint32_t base = 0;
     auto chunk = [&](auto more) {
         // the dword holds the group's four blocks: this lane's two go to the front
 #pragma unroll
-        for (int i = 0; i < 4; ++i) ws[i] = (uint32_t)wnext[i] >> (half * 16);
+        for (int i = 0; i < WT; ++i) ws[i] = (uint32_t)wnext[i] >> (half * 16);
 #pragma unroll
         for (int j = 0; j < 2; ++j) xs[j] = (uint32_t)xnext[j] >> (half * 16);
         // What is not a product is issued in the shadow of one (32 cycles each): the waves of a SIMD may come
         // through here together, so nothing else would keep the matrix core busy meanwhile.
         constexpr std::integral_constant<int, 0> first{};
         constexpr std::integral_constant<int, 1> second{};
-#define THEN __builtin_amdgcn_sched_barrier(0)
-        THEN;
-        multiply(first, 0, 0, fa), THEN, fetch_w(base, 1, 0, fb), fetch_x(base, 1, 0, fb), THEN;
-        multiply(first, 1, 0, fa), THEN, fetch_w(base, 1, 1, fb), fetch_w(base, 1, 2, fb), THEN;
-        multiply(first, 2, 0, fa), THEN, fetch_w(base, 1, 3, fb), fetch_x(base, 1, 1, fb), THEN;
-        multiply(first, 3, 0, fa), multiply(first, 0, 1, fa), multiply(first, 1, 1, fa), THEN;
-        multiply(first, 2, 1, fa), multiply(first, 3, 1, fa), THEN;
-        multiply(second, 0, 0, fb), multiply(second, 1, 0, fb), THEN;
-        // the next stage has arrived (younger ones may be under way), and this one has been read, everywhere
-        if constexpr (more)
-            arrive_and_wait<(L::kStages - 2) * L::kLoads>();
-        else
-            arrive_and_wait<0>();
+        __builtin_amdgcn_sched_barrier(0);
+        each<0, kProducts>([&](auto q) {
+            multiply(first, q, fa);
+            __builtin_amdgcn_sched_barrier(0);
+            each<2 * q, (2 * q + 2 < kReads ? 2 * q + 2 : kReads)>([&](auto i) { fetch(base, 1, i, fb); });
+            __builtin_amdgcn_sched_barrier(0);
+        });
         const int freed = slot;
-        slot = slot == L::kStages - 1 ? 0 : slot + 1;
-        base = slot * L::kStage;
-        // after the last stage these reads bring whatever lies there, and nothing uses it
-        fetch_w(base, 0, 0, fa), fetch_x(base, 0, 0, fa), THEN;
-        multiply(second, 2, 0, fb), THEN, fetch_w(base, 0, 1, fa), fetch_w(base, 0, 2, fa), THEN;
-        multiply(second, 3, 0, fb), THEN, fetch_w(base, 0, 3, fa), fetch_x(base, 0, 1, fa), THEN;
-        multiply(second, 0, 1, fb), THEN, fetch_scales(base), THEN;
-        multiply(second, 1, 1, fb), THEN;
-        if constexpr (more) {
-            stage_part(freed, std::integral_constant<int, 0>{});
-            stage_part(freed, std::integral_constant<int, 1>{});
-            stage_part(freed, std::integral_constant<int, 2>{});
-        }
-        THEN, multiply(second, 2, 1, fb), THEN;
-        if constexpr (more) {
-            stage_part(freed, std::integral_constant<int, 3>{});
-            stage_part(freed, std::integral_constant<int, 4>{});
-            stage_part(freed, std::integral_constant<int, 5>{});
-        }
-        THEN, multiply(second, 3, 1, fb), THEN;
-        if constexpr (more) {
-            stage_part(freed, std::integral_constant<int, 6>{});
-            stage_part(freed, std::integral_constant<int, 7>{});
-        }
-        THEN;
-#undef THEN
+        each<0, kProducts>([&](auto q) {
+            multiply(second, q, fb);
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (q == 1) {
+                // the next stage has arrived (younger ones may be under way), and this one has been read, everywhere
+                if constexpr (more)
+                    arrive_and_wait<(L::kStages - 2) * L::kLoads>();
+                else
+                    arrive_and_wait<0>();
+                slot = slot == L::kStages - 1 ? 0 : slot + 1;
+                base = slot * L::kStage;
+            }
+            // then the next stage's first reads (behind the last stage: of whatever lies there, and nothing
+            // uses them), its scales, and the loads into the stage that is free now, over the products left
+            constexpr int kScales = 1 + kReads / 2 < kProducts - 2 ? 1 + kReads / 2 : kProducts - 2, kLeft = kProducts - 1 - kScales;
+            if constexpr (q >= 1) each<2 * (q - 1), (2 * q < kReads ? 2 * q : kReads)>([&](auto i) { fetch(base, 0, i, fa); });
+            if constexpr (q == kScales) fetch_scales(base);
+            if constexpr (more && q > kScales) {
+                constexpr int n = q - kScales - 1;
+                each<n * L::kLoads / kLeft, (n + 1) * L::kLoads / kLeft>([&](auto part) { stage_part(freed, part); });
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        });
     };
     // two loops, each without a branch inside: products stay on their side of the barrier
     int c = 0;
     for (; c < all - L::kStages; ++c) chunk(std::true_type{});
     for (; c < all; ++c) chunk(std::false_type{});
 
-    if (threadIdx.x < kTileN) bias[threadIdx.x] = own_bias;
+    if (threadIdx.x < TN) bias[threadIdx.x] = own_bias;
     __syncthreads();
-    // every read of the stages lies behind: each wave takes 16 KB of them
-    static_assert(L::kWaves * 16384 <= L::kStages * L::kStage, "the stages hold the waves' parts of y");
-    uint8_t* own = lds + wave * 16384;
+    // every read of the stages lies behind: each wave takes a part of them
+    constexpr int kOwn = 32 * 32 * WT * 4;
+    static_assert(L::kWaves * kOwn <= L::kStages * L::kStage, "the stages hold the waves' parts of y");
+    uint8_t* own = lds + wave * kOwn;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-        const f32x16(&part)[4] = {acc[0][j], acc[1][j], acc[2][j], acc[3][j]};
+        f32x16 part[WT];
+#pragma unroll
+        for (int i = 0; i < WT; ++i) part[i] = acc[i][j];
         if (p.y_type == GLV_F32)
-            store_rows<float, MW == 2>(p, part, bias + nw, own, m0 + mw + j * 32, n0 + nw, lane);
+            store_rows<float, TM == 128>(p, part, bias + nw, own, m0 + mw + j * 32, n0 + nw, lane);
         else if (p.y_type == GLV_BF16)
-            store_rows<bf16, MW == 2>(p, part, bias + nw, own, m0 + mw + j * 32, n0 + nw, lane);
+            store_rows<bf16, TM == 128>(p, part, bias + nw, own, m0 + mw + j * 32, n0 + nw, lane);
         else
-            store_rows<f16, MW == 2>(p, part, bias + nw, own, m0 + mw + j * 32, n0 + nw, lane);
+            store_rows<f16, TM == 128>(p, part, bias + nw, own, m0 + mw + j * 32, n0 + nw, lane);
         wave_lds_fence();
     }
 }
 
-template <int MW>
+template <int TM, int TN>
 int launch_tiled(const Product& p, hipStream_t st) {
-    using L = Tiling<MW>;
-    const unsigned tiles = (unsigned)((p.rows + L::kTileM - 1) / L::kTileM) * ((p.n + kTileN - 1) / kTileN);
+    using L = Tiling<TM, TN>;
+    const unsigned tiles = (unsigned)((p.rows + TM - 1) / TM) * ((p.n + TN - 1) / TN);
     if (p.taps > 1)
-        hipLaunchKernelGGL((product_tiled_kernel<true, MW>), dim3(tiles), dim3(L::kThreads), 0, st, p);
+        hipLaunchKernelGGL((product_tiled_kernel<true, TM, TN>), dim3(tiles), dim3(L::kThreads), 0, st, p);
     else
-        hipLaunchKernelGGL((product_tiled_kernel<false, MW>), dim3(tiles), dim3(L::kThreads), 0, st, p);
+        hipLaunchKernelGGL((product_tiled_kernel<false, TM, TN>), dim3(tiles), dim3(L::kThreads), 0, st, p);
     return launch_status("product_tiled_kernel");
 }
 
@@ -829,14 +827,24 @@ extern "C" int glv_mxfp4_product(const void* x_dev, const uint8_t* x_scales_dev,
         if (rc != GLV_OK) return rc;
         p.xc = codes, p.xs = scales;
     }
-    // Below 3 M outputs the small tiles win (1000 x 1000 x 1024: 5.7 us against 11.6; 1024 x 2048 x 4096: 19.1
-    // against 19.4), above it the large ones (865 x 4096 x 1024: 10.2 against 11.4; 2048 x 2048 x 4096: 21 against
-    // 35).  256 rows of x a tile pay for long sums that fill the chip (8192 x 8192 x 8192: 250 us against 276; x
-    // 2048: 93 against 100); with 128 there is room for a second workgroup on the CU, whose loop hides the ends
-    // of the first (8192 x 8192 x 512: 40 against 47; 16384 x 256 x 1024: 10.2 against 11.8).
-    if (all * n_out >= (int64_t)3 << 20) {
+    // Which tile, measured in us for codes that are there already, y in bfloat16:
+    //                        32 x 32   128 x 128   128 x 256   256 x 256   (rows of x times rows of w)
+    //    1000 x 1000 x 1024      5.6         7.7        12.0        13.7
+    //    1024 x 2048 x  256      5.2         5.5         7.5         8.6
+    //    1024 x 2048 x 1024      7.9         7.0        10.0        11.7
+    //    2048 x 2048 x 4096     36.8        15.4        21.4        26.6
+    //   16384 x  256 x 1024     15.3         7.5        10.4        12.6
+    //   55360 x  256 x  512     24.2        13.0        11.9        13.9
+    //   10560 x 4096 x 1024     94.9        34.2        37.0        43.3
+    //    8192 x 8192 x 2048    256          82.4        78.5        84.2
+    //    8192 x 8192 x 4096    481         147         138         135
+    // 32 x 32 spreads small outputs over the chip; 128 x 128 has three workgroups on a CU to hide each
+    // other's ends; with one tile across w, x is read once; long sums on a full chip pay for the largest.
+    if (all * n_out >= (int64_t)2 << 20) {
         const int64_t wide = ((all + 255) / 256) * ((n_out + 255) / 256);
-        return wide >= 256 && p.taps * p.groups >= 16 ? launch_tiled<4>(p, st) : launch_tiled<2>(p, st);
+        if (wide >= 192 && p.taps * p.groups >= 32) return launch_tiled<256, 256>(p, st);
+        if (n_out > 128 && n_out <= 256 && all >= 32768) return launch_tiled<128, 256>(p, st);
+        return launch_tiled<128, 128>(p, st);
     }
     launch_direct<void>(p, (unsigned)tiles, st);
     return launch_status("product_direct_kernel");
