@@ -456,7 +456,7 @@ int glv_mxfp4_dequantize(const uint8_t* codes_dev, const uint8_t* scales_dev, in
  * taps * cols and n_out are at most 2^18, n_out * taps and (taps - 1) * dilation at most 2^24.
  */
 enum { GLV_ACT_NONE = 0, GLV_ACT_RELU = 1 };
-int64_t glv_mxfp4_product_workspace(int x_type, int batch, int rows, int cols, int n_out, int taps);
+int64_t glv_mxfp4_product_workspace(int x_type, int batch, int rows, int cols, int n_out, int taps, int dilation);
 int glv_mxfp4_product(const void* x_dev, const uint8_t* x_scales_dev, int x_type, int batch, int rows, int cols,
                       int64_t x_batch_stride, int64_t x_row_stride, const uint8_t* w_codes_dev,
                       const uint8_t* w_scales_dev, int n_out, int taps, int dilation, const void* bias_dev,

@@ -631,8 +631,9 @@ def test_c_entries_validate_before_any_device_call():
         assert b"glv_mxfp4_product" in lib.glv_last_error()
     assert product(rows=0, x=None, y=None, work=None) == 0 and product(n=0, wc=None) == 0
     size = lib.glv_mxfp4_product_workspace
-    assert size(0, 1, 64, 4096, 8, 1) > 0 and size(3, 1, 64, 4096, 8, 1) == 0
-    assert size(9, 1, 4, 32, 8, 1) == -1 and size(0, 1, 4, 0, 8, 1) == -1 and size(0, 1 << 13, 1 << 13, 32, 8, 1) == -1
+    assert size(0, 1, 64, 4096, 8, 1, 1) > 0 and size(3, 1, 64, 4096, 8, 1, 1) == 0
+    assert size(9, 1, 4, 32, 8, 1, 1) == -1 and size(0, 1, 4, 0, 8, 1, 1) == -1 and size(0, 1 << 13, 1 << 13, 32, 8, 1, 1) == -1
+    assert size(0, 1, 4, 32, 8, 1, 0) == -1 and size(0, 1, 4, 32, 8, 0, 1) == -1
 
     def norm(u=a, kind=0, batch=1, rows=4, cols=32, vkind=0, post=1, pw=None, eps=1e-5, gate=None, gate_col=1, scale=None, res=None,
              pre=0, y=a, z=None):

@@ -93,7 +93,7 @@ SIGNATURES = {
                                           ctypes.c_void_p]),
     "glv_mxfp4_dequantize": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_int,
                                             ctypes.c_void_p, ctypes.c_void_p]),
-    "glv_mxfp4_product_workspace": (ctypes.c_int64, [ctypes.c_int] * 6),
+    "glv_mxfp4_product_workspace": (ctypes.c_int64, [ctypes.c_int] * 7),
     "glv_mxfp4_product": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_int,
                                          ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p,
                                          ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_void_p,

@@ -204,7 +204,7 @@ def _product(x, weight, bias, taps, dilation, activation, out_dtype):
         bias_ptr = bias.data_ptr()
     lib = _lib.load()
     y = like.new_empty((*shape[:-1], n), dtype=out_dtype)
-    need = lib.glv_mxfp4_product_workspace(kind, batch, rows, cols, n, taps)
+    need = lib.glv_mxfp4_product_workspace(kind, batch, rows, cols, n, taps, dilation)
     work_ptr = None
     if need > 0:
         work = like.new_empty(need, dtype=torch.uint8)

@@ -205,17 +205,15 @@ __device__ inline f32x16 step(i32x4 w, i32x4 x, int wscale, int xscale, f32x16 a
 }
 
 // One 32 x 32 tile of y a workgroup; the waves deal the groups out among themselves and their sums meet
-// in LDS in a fixed order.  X is `void` for activations that are quantised already; otherwise a wave
-// quantises the 32 rows of its group itself, sixteen lanes a row, and passes the codes to the lanes
-// that multiply them through LDS of its own, so that a small product is one launch.
+// in LDS in a fixed order.  X is `void` for activations that are quantised already; otherwise the
+// workgroup first quantises the rows of x that its tile reaches, all groups of them, into LDS, so that
+// a small product is one launch, and every tap of a convolution finds them there.
+//   codes in LDS  [group][row][64], piece q of 16 bytes of row i at place q ^ (i / 4 % 4);  scales [group][row][4]
 template <typename X, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void product_direct_kernel(Product p) {
     constexpr bool kOwn = !std::is_void_v<X>;
     __shared__ float sums[WAVES][32][33];
-    __shared__ __align__(16) uint32_t codes[kOwn ? WAVES : 1][32][16];
-    __shared__ __align__(4) uint8_t scales[kOwn ? WAVES : 1][32][4];
-    __shared__ int64_t row_at[32];  // where the tile's rows begin, and their places in their entries
-    __shared__ int row_t[32];
+    extern __shared__ __align__(16) uint8_t held[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int r = lane & 31, half = lane >> 5;
     const int n_tiles = (p.n + 31) / 32;
@@ -225,63 +223,82 @@ __global__ __launch_bounds__(WAVES * 64) void product_direct_kernel(Product p) {
     const int rows = min(32, p.rows - m0);
     const int t = p.taps == 1 ? 0 : m % p.T;
     const int all = p.taps * p.groups;
+
+    i32x4 w0 = {}, w1 = {};
+    uint32_t wscale = 0;
+    auto fetch_w = [&](int g) {
+        const int tap = p.taps == 1 ? 0 : g / p.groups, gx = g - tap * p.groups;
+        const int64_t row = ((int64_t)gx * p.n + n) * p.taps + tap;
+        const i32x4* wp = reinterpret_cast<const i32x4*>(p.wc + row * kGroupBytes) + half * 2;
+        w0 = wp[0], w1 = wp[1];
+        wscale = reinterpret_cast<const uint32_t*>(p.ws)[row];
+    };
+    if (wave < all) fetch_w(wave);  // under way while x is quantised
+
+    // rows first .. first + span - 1 of x, whatever entries they belong to
+    const int first = max(m0 - p.left, 0);
+    const int span = min(m0 + rows - 1 + (p.taps - 1) * p.dilation - p.left, p.rows - 1) - first + 1;
+    uint32_t* const codes = reinterpret_cast<uint32_t*>(held);
+    uint8_t* const scales = held + span * p.groups * kGroupBytes;
     if constexpr (kOwn) {
-        if (threadIdx.x < 32) {
-            row_at[threadIdx.x] = row_offset(p.xr, m);
-            row_t[threadIdx.x] = t;
+        constexpr int kTeams = WAVES * 4, kDeep = sizeof(X) == 4 ? 4 : 8;  // sixteen lanes a row and group
+        const int team = threadIdx.x >> 4, piece = threadIdx.x & 15, units = span * p.groups;
+        // unit u is group u % groups of row u / groups; one team's units are kTeams apart
+        struct Unit {
+            int i, gx;
+        };
+        const int step_i = kTeams / p.groups, step_gx = kTeams - step_i * p.groups;
+        auto next = [&](Unit u) {
+            u.i += step_i, u.gx += step_gx;
+            const bool over = u.gx >= p.groups;
+            return Unit{u.i + over, over ? u.gx - p.groups : u.gx};
+        };
+        Unit at{team / p.groups, team % p.groups};
+        for (int u0 = team; u0 < units; u0 += kTeams * kDeep) {
+            Eight<X> v[kDeep];  // all loads before the first use
+            Unit u = at;
+#pragma unroll
+            for (int k = 0; k < kDeep; ++k, u = next(u)) {
+                if (u0 + k * kTeams >= units) break;
+                v[k] = fetch_eight<false>(static_cast<const X*>(p.x) + row_offset(p.xr, first + u.i), u.gx * kGroup + piece * 8, p.cols);
+            }
+#pragma unroll
+            for (int k = 0; k < kDeep; ++k, at = next(at)) {
+                if (u0 + k * kTeams >= units) break;
+                int byte;
+                const uint32_t c = quantise_eight(place_eight<false>(v[k], at.gx * kGroup + piece * 8, p.cols), &byte);
+                const int row = at.gx * span + at.i;
+                codes[(row * 4 + (((piece >> 2) ^ (at.i >> 2)) & 3)) * 4 + (piece & 3)] = c;
+                if ((piece & 3) == 0) scales[row * 4 + (piece >> 2)] = (uint8_t)byte;
+            }
         }
         __syncthreads();
     }
+
     f32x16 acc = {};
     for (int g = wave; g < all; g += WAVES) {
         const int tap = p.taps == 1 ? 0 : g / p.groups, gx = g - tap * p.groups;
         const int shift = tap * p.dilation - p.left;
-        const int64_t wrow = ((int64_t)gx * p.n + n) * p.taps + tap;
-        const i32x4* wp = reinterpret_cast<const i32x4*>(p.wc + wrow * kGroupBytes) + half * 2;
-        const i32x4 w0 = wp[0], w1 = wp[1];
-        const uint32_t wscale = reinterpret_cast<const uint32_t*>(p.ws)[wrow];
         i32x4 x0 = {}, x1 = {};
         uint32_t xscale = 0;
-        if constexpr (kOwn) {
-            const int piece = lane & 15, col = gx * kGroup + piece * 8;
-            Eight<X> v[8];  // rows lane / 16 + 0, 4, .. 28: all loads before the first use
-            int at[8];
-            const int i0 = lane >> 4;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                if (4 * k >= rows) break;
-                const int64_t from = row_at[4 * k + i0];
-                const bool inside = (unsigned)(row_t[4 * k + i0] + shift) < (unsigned)p.T;
-                at[k] = inside ? col : max(col, p.cols);  // behind the row's end: zeros
-                v[k] = fetch_eight<false>(static_cast<const X*>(p.x) + from + (inside ? shift * p.xr.row_stride : 0), at[k], p.cols);
+        if ((unsigned)(t + shift) < (unsigned)p.T) {  // a tap outside the entry meets zeros
+            if constexpr (kOwn) {
+                const int i = m + shift - first, row = gx * span + i, place = i >> 2;
+                x0 = *reinterpret_cast<const i32x4*>(codes + (row * 4 + ((half * 2 ^ place) & 3)) * 4);
+                x1 = *reinterpret_cast<const i32x4*>(codes + (row * 4 + (((half * 2 + 1) ^ place) & 3)) * 4);
+                xscale = *reinterpret_cast<const uint32_t*>(scales + row * 4);
+            } else {
+                const int64_t row = (int64_t)gx * p.rows + m + shift;
+                const i32x4* xp = reinterpret_cast<const i32x4*>(p.xc + row * kGroupBytes) + half * 2;
+                x0 = xp[0], x1 = xp[1];
+                xscale = reinterpret_cast<const uint32_t*>(p.xs)[row];
             }
-            const bool ragged = p.taps > 1 || (gx + 1) * kGroup > p.cols;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                if (4 * k >= rows) break;
-                if (ragged) v[k] = place_eight<false>(v[k], at[k], p.cols);
-                int byte;
-                const uint32_t c = quantise_eight(v[k], &byte);
-                // piece q of 16 bytes of row i at place q ^ (i / 4 % 4)
-                codes[wave][4 * k + i0][(((piece >> 2) ^ k) & 3) * 4 + (piece & 3)] = c;
-                if ((piece & 3) == 0) scales[wave][4 * k + i0][piece >> 2] = (uint8_t)byte;
-            }
-            wave_lds_fence();
-            const int place = r >> 2 & 3;
-            x0 = *reinterpret_cast<const i32x4*>(&codes[wave][r][((half * 2) ^ place) * 4]);
-            x1 = *reinterpret_cast<const i32x4*>(&codes[wave][r][((half * 2 + 1) ^ place) * 4]);
-            xscale = *reinterpret_cast<const uint32_t*>(&scales[wave][r][0]);
-            wave_lds_fence();
-        } else if ((unsigned)(t + shift) < (unsigned)p.T) {
-            const int64_t row = (int64_t)gx * p.rows + m + shift;
-            const i32x4* xp = reinterpret_cast<const i32x4*>(p.xc + row * kGroupBytes) + half * 2;
-            x0 = xp[0], x1 = xp[1];
-            xscale = reinterpret_cast<const uint32_t*>(p.xs)[row];
         }
         // lane l takes, of row l % 32, the blocks 2 * (l / 32) and + 1 in the two steps
         const int ws = wscale >> (half * 16), xs = xscale >> (half * 16);
         acc = step<0>(w0, x0, ws, xs, acc);
         acc = step<1>(w1, x1, ws, xs, acc);
+        if (g + WAVES < all) fetch_w(g + WAVES);
     }
 #pragma unroll
     for (int i = 0; i < 16; ++i) sums[wave][r][8 * (i >> 2) + 4 * half + (i & 3)] = acc[i];
@@ -671,25 +688,31 @@ int quantise(const void* x, int type, Rows xr, int rows, int cols, uint8_t* code
     return launch_status("quantise_kernel");
 }
 
-// Four waves where there are no more groups than that, else eight (sixteen gain 0.5 us at 10 groups in
-// half precision and lose as much in float32, whose registers no longer fit).
-template <typename X>
-void launch_direct(const Product& p, unsigned tiles, hipStream_t st) {
-    if (p.taps * p.groups <= 4)
-        hipLaunchKernelGGL((product_direct_kernel<X, 4>), dim3(tiles), dim3(256), 0, st, p);
-    else
-        hipLaunchKernelGGL((product_direct_kernel<X, 8>), dim3(tiles), dim3(512), 0, st, p);
+// Rows of x that one tile of 32 rows of y reaches, at most.
+int64_t reached_rows(int64_t rows, int taps, int dilation) {
+    const int64_t span = 32 + (int64_t)(taps - 1) * dilation;
+    return span < rows ? span : rows;
 }
 
-// Whether a product quantises its activations itself: every tile of 32 columns of y does so anew, for
-// every tap, against a launch and a workspace less.  It does while a wave's walk stays within 16 pieces
-// of four rows of a group (32 x 1024 x 4096, 32 pieces: 9.9 us against 7.1 in two launches; 32 x 4096 x 1024,
-// 8 pieces: 4.8 against 5.7) and all tiles together within 8 M columns of x (865 x 256 x 1024, 7 M: 5.0
-// against 6.5; 2000 x 500 x 500, 16 M: 8.1 against 7.8, float32 12.2 against 8.1).
-bool quantised_in_product(int64_t rows, int cols, int n_out, int taps) {
-    const int64_t groups = (int64_t)taps * ((cols + kGroup - 1) / kGroup);
-    const int64_t pieces = ((groups + 7) / 8) * (rows < 32 ? (rows + 3) / 4 : 8);
-    return cols >= 8 && pieces <= 16 && rows * cols * taps * ((n_out + 31) / 32) <= (int64_t)8 << 20;
+// Four waves where there are no more groups than that, else eight.
+template <typename X>
+void launch_direct(const Product& p, unsigned tiles, hipStream_t st) {
+    const size_t held = std::is_void_v<X> ? 0 : reached_rows(p.rows, p.taps, p.dilation) * p.groups * (kGroupBytes + 4);
+    if (p.taps * p.groups <= 4)
+        hipLaunchKernelGGL((product_direct_kernel<X, 4>), dim3(tiles), dim3(256), held, st, p);
+    else
+        hipLaunchKernelGGL((product_direct_kernel<X, 8>), dim3(tiles), dim3(512), held, st, p);
+}
+
+// Whether a product quantises its activations itself: every tile of 32 x 32 of y does so anew with the
+// rows it reaches, against a launch and a workspace less.  It does while those are at most 256 pairs
+// of a row and a group (us, bfloat16, device: 32 x 4096 x 1024, 256 pairs, 5.7 against 5.8 in two launches; 32 x
+// 1024 x 2048, 512 pairs, 8.2 against 6.3; 165 rows, 256 -> 256, 5 taps, 80 pairs, 4.2 against 5.6) and at most 8 M
+// elements in all tiles together (865 x 256 x 1024, 7 M, 5.8 against 6.6; 2000 x 500 x 500, 16 M, 9.7 against 7.9).
+bool quantised_in_product(int64_t rows, int cols, int n_out, int taps, int dilation) {
+    const int64_t pairs = reached_rows(rows, taps, dilation) * ((cols + kGroup - 1) / kGroup);
+    const int64_t tiles = ((rows + 31) / 32) * ((n_out + 31) / 32);
+    return cols >= 8 && pairs <= 256 && tiles * pairs * kGroup <= (int64_t)8 << 20;
 }
 
 // Row counts and widths are ints in the kernels, row * groups is formed in 64 bits, and every
@@ -757,10 +780,10 @@ extern "C" int glv_mxfp4_dequantize(const uint8_t* codes_dev, const uint8_t* sca
     return launch_status("dequantise_kernel");
 }
 
-extern "C" int64_t glv_mxfp4_product_workspace(int x_type, int batch, int rows, int cols, int n_out, int taps) {
-    if (batch < 0 || rows < 0 || n_out < 0 || taps < 1 || cols < 1 || cols > kMaxCols) return -1;
+extern "C" int64_t glv_mxfp4_product_workspace(int x_type, int batch, int rows, int cols, int n_out, int taps, int dilation) {
+    if (batch < 0 || rows < 0 || n_out < 0 || taps < 1 || dilation < 1 || cols < 1 || cols > kMaxCols) return -1;
     if ((int64_t)batch * rows > kMaxRows || !(float_type(x_type) || x_type == GLV_MXFP4)) return -1;
-    if (x_type == GLV_MXFP4 || quantised_in_product((int64_t)batch * rows, cols, n_out, taps)) return 0;
+    if (x_type == GLV_MXFP4 || quantised_in_product((int64_t)batch * rows, cols, n_out, taps, dilation)) return 0;
     return quantised_bytes((int64_t)batch * rows, (cols + kGroup - 1) / kGroup);
 }
 
@@ -806,7 +829,7 @@ extern "C" int glv_mxfp4_product(const void* x_dev, const uint8_t* x_scales_dev,
         rc = check_quantised(what, x_dev, x_scales_dev);
         if (rc != GLV_OK) return rc;
         p.xc = static_cast<const uint8_t*>(x_dev), p.xs = x_scales_dev;
-    } else if (quantised_in_product(all, cols, n_out, taps)) {
+    } else if (quantised_in_product(all, cols, n_out, taps, dilation)) {
         p.x = x_dev, p.xr = Rows{x_batch_stride, x_row_stride, rows, batch == 1}, p.cols = cols;
         if (x_type == GLV_F32)
             launch_direct<float>(p, (unsigned)tiles, st);
