@@ -25,20 +25,12 @@ _GROUP = 128  # columns that share one dword of scales
 
 
 # The calls below take a few microseconds on the host, as much as a small launch on the device, so
-# the checks are written to cost little when nothing is wrong.
+# the checks are written to cost little when nothing is wrong, and the library is called in place.
+# A call for another device than the current one makes that device current and starts again.
 _current_device = torch.cuda.current_device
-_current_stream = torch._C._cuda_getCurrentRawStream  # the handle alone, without a Stream object around it
-
-
-def _launch(index, entry, *args):
-    """entry(*args, stream) with device `index` current, on torch's current stream of it."""
-    if _current_device() == index:
-        rc = entry(*args, _current_stream(index))
-    else:
-        with torch.cuda.device(index):
-            rc = entry(*args, _current_stream(index))
-    if rc:
-        _lib.check(rc)
+# the handle alone, without a Stream object around it, where torch offers that
+_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _check(t, name, index=None):
@@ -139,8 +131,15 @@ class MXFP4Tensor:
         index = data.get_device()
         if index < 0:
             raise ValueError(f"the tensor must be on a ROCm GPU (there is no CPU fallback), got {self.device}")
+        if _current_device() != index:
+            with torch.cuda.device(index):
+                return self.dequantize(dtype)
         out = data.new_empty(shape, dtype=dtype)
-        _launch(index, _lib.load().glv_mxfp4_dequantize, *self._pointers(), self.rows, shape[-1], kind, out.data_ptr())
+        codes, scales = self._pointers()
+        rc = _lib.load().glv_mxfp4_dequantize(codes, scales, self.rows, shape[-1], kind, out.data_ptr(),
+                                              _current_stream(index))
+        if rc:
+            _lib.check(rc)
         return out
 
     def __repr__(self):
@@ -155,13 +154,20 @@ def mxfp4_quantize(x):
     kind, shape = _check(x, "x"), x.shape
     if len(shape) < 1 or shape[-1] < 1:
         raise ValueError(f"x must have a last dimension of at least 1, got {tuple(shape)}")
+    index = x.get_device()
+    if _current_device() != index:
+        with torch.cuda.device(index):
+            return mxfp4_quantize(x)
     v, batch, rows, batch_stride, row_stride = _rows(x, shape)
     cols = shape[-1]
     q = object.__new__(MXFP4Tensor)
     q.shape, q.rows, q.groups = shape, batch * rows, -(-cols // _GROUP)
     q.data = x.new_empty(q.rows * q.groups * 68, dtype=torch.uint8)
-    _launch(x.get_device(), _lib.load().glv_mxfp4_quantize, v.data_ptr(), kind, batch, rows, cols, batch_stride,
-            row_stride, *q._pointers())
+    codes, scales = q._pointers()
+    rc = _lib.load().glv_mxfp4_quantize(v.data_ptr(), kind, batch, rows, cols, batch_stride, row_stride, codes, scales,
+                                        _current_stream(index))
+    if rc:
+        _lib.check(rc)
     return q
 
 
@@ -171,6 +177,9 @@ def _product(x, weight, bias, taps, dilation, activation, out_dtype):
         raise ValueError(f"activation must be None or 'relu', got {activation!r}")
     wshape = weight.shape
     n, cols, index = wshape[0], wshape[-1], weight.data.get_device()
+    if _current_device() != index:
+        with torch.cuda.device(index):
+            return _product(x, weight, bias, taps, dilation, activation, out_dtype)
     scales, batch_stride, row_stride = None, 0, 0
     if isinstance(x, MXFP4Tensor):
         like, shape = x.data, x.shape
@@ -209,9 +218,12 @@ def _product(x, weight, bias, taps, dilation, activation, out_dtype):
     if need > 0:
         work = like.new_empty(need, dtype=torch.uint8)
         work_ptr = work.data_ptr()
-    _launch(index, lib.glv_mxfp4_product, data, scales, kind, batch, rows, cols, batch_stride, row_stride,
-            *weight._pointers(), n, taps, dilation, bias_ptr, bias_kind, act, y.data_ptr(), out_kind, work_ptr,
-            need if need > 0 else 0)
+    w_codes, w_scales = weight._pointers()
+    rc = lib.glv_mxfp4_product(data, scales, kind, batch, rows, cols, batch_stride, row_stride, w_codes, w_scales, n, taps,
+                               dilation, bias_ptr, bias_kind, act, y.data_ptr(), out_kind, work_ptr,
+                               need if need > 0 else 0, _current_stream(index))
+    if rc:
+        _lib.check(rc)
     return y
 
 
@@ -268,6 +280,15 @@ class Norm:
         self.weight, self.bias, self.eps, self.kind = weight, bias, float(eps), kind
 
 
+def _norm_vector(t, name, cols, index, kind, seen, held):
+    """(pointer, number of its type) of a weight, bias or scale; all of a call share one type."""
+    t, k = _vector(t, name, cols, index)
+    if (k != 0 and k != kind) or (seen is not None and seen != k):
+        raise ValueError(f"weights, biases and scale must all be float32 or all of u's type, got {t.dtype}")
+    held.append(t)
+    return t.data_ptr(), k
+
+
 def block_norm(u, *, post=None, gate=None, scale=None, residual=None, pre=None):
     """y = residual + scale * gate * post(u), and z = pre(y) where `pre` is given: the end of a block
     and the start of the next in one pass.  Returns y, or (y, z).
@@ -283,34 +304,27 @@ def block_norm(u, *, post=None, gate=None, scale=None, residual=None, pre=None):
     kind, shape, index, dtype = _check(u, "u"), u.shape, u.get_device(), u.dtype
     if len(shape) < 1 or shape[-1] < 1:
         raise ValueError(f"u must have a last dimension of at least 1, got {tuple(shape)}")
+    if _current_device() != index:
+        with torch.cuda.device(index):
+            return block_norm(u, post=post, gate=gate, scale=scale, residual=residual, pre=pre)
     cols = shape[-1]
     v, batch, rows, u_batch, u_row = _rows(u, shape)
-    vector_kind = None
-
-    def vector(t, name):
-        nonlocal vector_kind
-        if t is None:
-            return None
-        t, k = _vector(t, name, cols, index)
-        if k not in (0, kind) or vector_kind not in (None, k):
-            raise ValueError(f"weights, biases and scale must all be float32 or all {dtype}, got {t.dtype}")
-        vector_kind = k
-        held.append(t)
-        return t.data_ptr()
-
-    held = []  # contiguous copies live until the launch
-    sides = []
+    held, sides, vector_kind = [], [], None  # contiguous copies live until the launch
     for side, norm in (("post", post), ("pre", pre)):
         if norm is None:
             sides.append((0, None, None, 0.0))
         elif isinstance(norm, Norm):
-            sides.append((_NORMS[norm.kind], vector(norm.weight, f"{side}.weight"), vector(norm.bias, f"{side}.bias"),
-                          norm.eps))
+            weight, bias = norm.weight, norm.bias
+            if weight is not None:
+                weight, vector_kind = _norm_vector(weight, f"{side}.weight", cols, index, kind, vector_kind, held)
+            if bias is not None:
+                bias, vector_kind = _norm_vector(bias, f"{side}.bias", cols, index, kind, vector_kind, held)
+            sides.append((_NORMS[norm.kind], weight, bias, norm.eps))
         else:
             raise ValueError(f"{side} must be a Norm or None, got {type(norm).__name__}")
     scale_ptr, factor = None, 1.0
     if isinstance(scale, torch.Tensor):
-        scale_ptr = vector(scale, "scale")
+        scale_ptr, vector_kind = _norm_vector(scale, "scale", cols, index, kind, vector_kind, held)
     elif scale is not None:
         factor = float(scale)
     gate_ptr, gate_strides = None, (0, 0, 1)
@@ -336,18 +350,23 @@ def block_norm(u, *, post=None, gate=None, scale=None, residual=None, pre=None):
                 gate_strides[2 - i] = stride
         gate_ptr = g.data_ptr()
         held.append(g)
-    res_ptr, res_strides = None, (0, 0)
+    res_ptr, res_batch, res_row = None, 0, 0
     if residual is not None:
         _check(residual, "residual", index)
         if residual.dtype != dtype or residual.shape != shape:
             raise ValueError(f"residual must be {dtype} {tuple(shape)} like u, got {residual.dtype} "
                              f"{tuple(residual.shape)}")
-        r, _, _, *res_strides = _rows(residual, shape)
+        r, _, _, res_batch, res_row = _rows(residual, shape)
         res_ptr = r.data_ptr()
         held.append(r)
     y = v.new_empty(shape)
     z = v.new_empty(shape) if pre is not None else None
-    _launch(index, _lib.load().glv_block_norm, v.data_ptr(), kind, batch, rows, cols, u_batch, u_row, vector_kind or 0,
-            *sides[0], gate_ptr, *gate_strides, scale_ptr, factor, res_ptr, *res_strides, *sides[1], y.data_ptr(),
-            None if z is None else z.data_ptr())
+    post_kind, post_w, post_b, post_eps = sides[0]
+    pre_kind, pre_w, pre_b, pre_eps = sides[1]
+    rc = _lib.load().glv_block_norm(v.data_ptr(), kind, batch, rows, cols, u_batch, u_row, vector_kind or 0, post_kind,
+                                    post_w, post_b, post_eps, gate_ptr, gate_strides[0], gate_strides[1], gate_strides[2],
+                                    scale_ptr, factor, res_ptr, res_batch, res_row, pre_kind, pre_w, pre_b, pre_eps,
+                                    y.data_ptr(), None if z is None else z.data_ptr(), _current_stream(index))
+    if rc:
+        _lib.check(rc)
     return y if z is None else (y, z)
