@@ -66,44 +66,47 @@ struct Row {
     }
 };
 
-// x <- Norm(x) for the row held as V pieces of eight a lane, zeros behind `cols`
-template <typename W, int LANES, int V, bool NARROW>
-__device__ inline void normalise(float (&x)[V][8], int kind, const void* weight, const void* bias, float eps, int cols,
+// A lane holds V pieces of N columns: 16 bytes of a stream each, so that what the lanes of a row touch
+// at once is one run of memory.
+//
+// x <- Norm(x), zeros behind `cols`
+template <typename W, int LANES, int V, int N, bool NARROW>
+__device__ inline void normalise(float (&x)[V][N], int kind, const void* weight, const void* bias, float eps, int cols,
                                  const Row<LANES>& row, int use) {
     const float inv = 1.f / (float)cols;
-    Eight<W> w[V], b[V];
+    Pack<W, N> w[V], b[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) {  // under way while the sums are formed
-        const int col = (v * row.lanes + row.lane) * 8;
-        if (weight) w[v] = fetch_eight<NARROW>(static_cast<const W*>(weight), col, cols);
-        if (bias) b[v] = fetch_eight<NARROW>(static_cast<const W*>(bias), col, cols);
+        const int col = (v * row.lanes + row.lane) * N;
+        if (weight) w[v] = fetch_pack<NARROW, N>(static_cast<const W*>(weight), col, cols);
+        if (bias) b[v] = fetch_pack<NARROW, N>(static_cast<const W*>(bias), col, cols);
     }
     if (kind == GLV_NORM_LAYER) {
         float s = 0.f;
 #pragma unroll
         for (int v = 0; v < V; ++v)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) s += x[v][i];
+            for (int i = 0; i < N; ++i) s += x[v][i];
         const float mean = row.sum(s, use) * inv;
 #pragma unroll
         for (int v = 0; v < V; ++v)
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                x[v][i] = (v * row.lanes + row.lane) * 8 + i < cols ? x[v][i] - mean : 0.f;
+            for (int i = 0; i < N; ++i)
+                x[v][i] = (v * row.lanes + row.lane) * N + i < cols ? x[v][i] - mean : 0.f;
     }
     float q = 0.f;
 #pragma unroll
     for (int v = 0; v < V; ++v)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) q += x[v][i] * x[v][i];
+        for (int i = 0; i < N; ++i) q += x[v][i] * x[v][i];
     const float r = rsqrtf(row.sum(q, use + 1) * inv + eps);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        const int col = (v * row.lanes + row.lane) * 8;
-        if (weight) w[v] = place_eight<NARROW>(w[v], col, cols);
-        if (bias) b[v] = place_eight<NARROW>(b[v], col, cols);
+        const int col = (v * row.lanes + row.lane) * N;
+        if (weight) w[v] = place_pack<NARROW>(w[v], col, cols);
+        if (bias) b[v] = place_pack<NARROW>(b[v], col, cols);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < N; ++i) {
             float t = x[v][i] * r;
             if (weight) t *= (float)w[v].v[i];
             if (bias) t += (float)b[v].v[i];
@@ -112,10 +115,11 @@ __device__ inline void normalise(float (&x)[V][8], int kind, const void* weight,
     }
 }
 
-// V pieces of eight columns a lane
-template <typename T, typename W, int LANES, int V, bool NARROW = false>
+// EIGHTS: columns a lane holds, in eights
+template <typename T, typename W, int LANES, int EIGHTS, bool NARROW = false>
 __global__ __launch_bounds__(LANES > 0 ? 256 : 1024) void block_norm_kernel(BlockNorm p) {
     __shared__ float slots[LANES > 0 ? 1 : 64];
+    constexpr int N = 16 / sizeof(T), V = EIGHTS * 8 / N;
     constexpr int kRows = LANES > 0 ? 256 / LANES : 1;
     const int index = blockIdx.x * kRows + (LANES > 0 ? threadIdx.x / LANES : 0);
     // the rows behind the last are computed from the last, for their lanes take part in the sums' exchanges
@@ -128,33 +132,33 @@ __global__ __launch_bounds__(LANES > 0 ? 256 : 1024) void block_norm_kernel(Bloc
     const int64_t out = (int64_t)at * p.cols;
     const int cols = p.cols, store_cols = index < p.rows ? p.cols : 0;
 
-    Eight<T> ur[V], gr[V], rr[V];
+    Pack<T, N> ur[V], gr[V], rr[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        const int col = (v * row.lanes + row.lane) * 8;
-        ur[v] = fetch_eight<NARROW>(u, col, cols);
-        if (gate && p.gate_col) gr[v] = fetch_eight<NARROW>(gate, col, cols);
-        if (res) rr[v] = fetch_eight<NARROW>(res, col, cols);
+        const int col = (v * row.lanes + row.lane) * N;
+        ur[v] = fetch_pack<NARROW, N>(u, col, cols);
+        if (gate && p.gate_col) gr[v] = fetch_pack<NARROW, N>(gate, col, cols);
+        if (res) rr[v] = fetch_pack<NARROW, N>(res, col, cols);
     }
     const float row_factor = p.scale * (gate && !p.gate_col ? (float)gate[0] : 1.f);
-    float x[V][8];
+    float x[V][N];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        const Eight<T> placed = place_eight<NARROW>(ur[v], (v * row.lanes + row.lane) * 8, cols);
+        const Pack<T, N> placed = place_pack<NARROW>(ur[v], (v * row.lanes + row.lane) * N, cols);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[v][i] = (float)placed.v[i];
+        for (int i = 0; i < N; ++i) x[v][i] = (float)placed.v[i];
     }
-    if (p.post) normalise<W, LANES, V, NARROW>(x, p.post, p.post_w, p.post_b, p.post_eps, cols, row, 0);
+    if (p.post) normalise<W, LANES, V, N, NARROW>(x, p.post, p.post_w, p.post_b, p.post_eps, cols, row, 0);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        const int col = (v * row.lanes + row.lane) * 8;
-        Eight<W> sv;
-        if (p.scale_vec) sv = load_eight<NARROW>(static_cast<const W*>(p.scale_vec), col, cols);
-        if (gate && p.gate_col) gr[v] = place_eight<NARROW>(gr[v], col, cols);
-        if (res) rr[v] = place_eight<NARROW>(rr[v], col, cols);
-        Eight<T> o;
+        const int col = (v * row.lanes + row.lane) * N;
+        Pack<W, N> sv;
+        if (p.scale_vec) sv = load_pack<NARROW, N>(static_cast<const W*>(p.scale_vec), col, cols);
+        if (gate && p.gate_col) gr[v] = place_pack<NARROW>(gr[v], col, cols);
+        if (res) rr[v] = place_pack<NARROW>(rr[v], col, cols);
+        Pack<T, N> o;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < N; ++i) {
             float k = x[v][i] * row_factor;
             if (gate && p.gate_col) k *= (float)gr[v].v[i];
             if (p.scale_vec) k *= (float)sv.v[i];
@@ -162,30 +166,30 @@ __global__ __launch_bounds__(LANES > 0 ? 256 : 1024) void block_norm_kernel(Bloc
             x[v][i] = col + i < cols ? k : 0.f;
             o.v[i] = (T)k;
         }
-        store_eight(static_cast<T*>(p.y) + out + col, o, store_cols - col);
+        store_pack(static_cast<T*>(p.y) + out + col, o, store_cols - col);
     }
     if (!p.pre) return;
-    normalise<W, LANES, V, NARROW>(x, p.pre, p.pre_w, p.pre_b, p.pre_eps, cols, row, 2);
+    normalise<W, LANES, V, N, NARROW>(x, p.pre, p.pre_w, p.pre_b, p.pre_eps, cols, row, 2);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        const int col = (v * row.lanes + row.lane) * 8;
-        Eight<T> o;
+        const int col = (v * row.lanes + row.lane) * N;
+        Pack<T, N> o;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) o.v[i] = (T)x[v][i];
-        store_eight(static_cast<T*>(p.z) + out + col, o, store_cols - col);
+        for (int i = 0; i < N; ++i) o.v[i] = (T)x[v][i];
+        store_pack(static_cast<T*>(p.z) + out + col, o, store_cols - col);
     }
 }
 
 // The fewest lanes that hold a row: 16 or 32 leave room for the other rows of a wave (32768 x 256 fp16,
-// the whole boundary: 25.5 us at 64 lanes, 19.2 at 32); beyond a wave as many waves as two pieces a lane ask
-// for (1001 x 5000: 21.3 us with 256 threads of four pieces, two fifths of them idle, 16.2 with 320 of two;
-// 4096 x 16384: 317 us with 1024 of four, half of them idle, 185 with 1024 of two), four pieces where sixteen
-// waves would not do.
+// the whole boundary: 25.5 us at 64 lanes, 19.2 at 32); beyond a wave as many waves as two eights a lane ask
+// for (1001 x 5000: 21.3 us with 256 threads of four eights, two fifths of them idle, 16.2 with 320 of two;
+// 4096 x 16384: 317 us with 1024 of four, half of them idle, 185 with 1024 of two), four where sixteen waves
+// would not do.
 template <typename T, typename W>
 void launch(const BlockNorm& p, hipStream_t st) {
-    const int pieces = (p.cols + 7) / 8;
+    const int pieces = (p.cols + 7) / 8;  // a lane holds one, two or four of them
     auto rows_a_wave = [&](int lanes) { return dim3((unsigned)(((int64_t)p.rows * lanes + 255) / 256)); };
-    if (p.cols < 8)
+    if (p.cols < 16 / (int)sizeof(T))
         hipLaunchKernelGGL((block_norm_kernel<T, W, 16, 1, true>), rows_a_wave(16), dim3(256), 0, st, p);
     else if (pieces <= 16)
         hipLaunchKernelGGL((block_norm_kernel<T, W, 16, 1>), rows_a_wave(16), dim3(256), 0, st, p);

@@ -19,12 +19,13 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef f16 f16x2 __attribute__((ext_vector_type(2)));
 
-template <typename T>
-struct Eight {
-    T v[8];
+template <typename T, int N>
+struct Pack {
+    T v[N];
 };
+template <typename T>
+using Eight = Pack<T, 8>;
 
-// 16 bytes at the alignment of a T, in one access
 typedef int i32x4_at2 __attribute__((ext_vector_type(4), aligned(2)));
 typedef int i32x4_at4 __attribute__((ext_vector_type(4), aligned(4)));
 template <typename T>
@@ -38,16 +39,16 @@ __device__ inline void store_16(T* p, i32x4 v) {
     *reinterpret_cast<Unaligned<T>*>(p) = v;
 }
 
-// v moved down by `by` elements (0 .. 8), zeros from above
-template <typename T>
-__device__ inline Eight<T> moved_down(const Eight<T>& v, int by) {
-    constexpr int kWords = sizeof(Eight<T>) / 4;
+// v moved down by `by` elements (0 .. N), zeros from above
+template <typename T, int N>
+__device__ inline Pack<T, N> moved_down(const Pack<T, N>& v, int by) {
+    constexpr int kWords = sizeof(v) / 4;
     struct Words {
-        uint32_t w[kWords + 8];
+        uint32_t w[2 * kWords];
     } x = {};
     __builtin_memcpy(x.w, &v, sizeof(v));
 #pragma unroll
-    for (int bit = 8; bit >= 1; bit >>= 1) {
+    for (int bit = N; bit >= 1; bit >>= 1) {
         const int bytes = bit * sizeof(T);
         if (by & bit) {
 #pragma unroll
@@ -55,62 +56,62 @@ __device__ inline Eight<T> moved_down(const Eight<T>& v, int by) {
                 x.w[i] = bytes >= 4 ? x.w[i + bytes / 4] : __builtin_amdgcn_alignbit(x.w[i + 1], x.w[i], 16);
         }
     }
-    Eight<T> r;
+    Pack<T, N> r;
     __builtin_memcpy(&r, x.w, sizeof(r));
     return r;
 }
 
-// Columns [col, col + 8) of a row of `cols`, zeros behind the last, in two halves so that many loads can
-// be under way before the first is used: fetch_eight reads, without branches, a piece that reaches
-// over the end as the row's last eight; place_eight moves it into place.  NARROW: rows of fewer than
-// eight, a kernel of its own wherever the others would carry its eight loads along.
-template <bool NARROW, typename T>
-__device__ inline Eight<T> fetch_eight(const T* row, int col, int cols) {
-    Eight<T> r;
+// Columns [col, col + N) of a row of `cols`, zeros behind the last, in two halves so that many loads can
+// be under way before the first is used: fetch_pack reads, without branches, a piece that reaches over
+// the end as the row's last N; place_pack moves it into place.  NARROW: rows of fewer than N, a kernel
+// of its own wherever the others would carry its loads along.
+template <bool NARROW, int N, typename T>
+__device__ inline Pack<T, N> fetch_pack(const T* row, int col, int cols) {
+    Pack<T, N> r;
     if constexpr (NARROW) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) r.v[i] = row[min(i, cols - 1)];
+        for (int i = 0; i < N; ++i) r.v[i] = row[min(i, cols - 1)];
     } else {
-        const T* p = row + min(col, cols - 8);
-        if constexpr (sizeof(T) == 2) {
-            r = __builtin_bit_cast(Eight<T>, load_16(p));
-        } else {
-            const i32x4 a = load_16(p), b = load_16(p + 4);
-            r = __builtin_bit_cast(Eight<T>, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+        const T* p = row + min(col, cols - N);
+        constexpr int kEach = 16 / sizeof(T);
+#pragma unroll
+        for (int i = 0; i < N; i += kEach) {
+            const i32x4 part = load_16(p + i);
+            __builtin_memcpy(r.v + i, &part, 16);
         }
     }
     return r;
 }
-template <bool NARROW, typename T>
-__device__ inline Eight<T> place_eight(const Eight<T>& v, int col, int cols) {
+template <bool NARROW, int N, typename T>
+__device__ inline Pack<T, N> place_pack(const Pack<T, N>& v, int col, int cols) {
     if constexpr (NARROW) {
-        Eight<T> r;
+        Pack<T, N> r;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) r.v[i] = col + i < cols ? v.v[i] : T(0);
+        for (int i = 0; i < N; ++i) r.v[i] = col + i < cols ? v.v[i] : T(0);
         return r;
     } else {
-        return col + 8 <= cols ? v : moved_down(v, min(col - (cols - 8), 8));
+        return col + N <= cols ? v : moved_down(v, min(col - (cols - N), N));
     }
 }
-template <bool NARROW, typename T>
-__device__ inline Eight<T> load_eight(const T* row, int col, int cols) {
-    return place_eight<NARROW>(fetch_eight<NARROW>(row, col, cols), col, cols);
+template <bool NARROW, int N, typename T>
+__device__ inline Pack<T, N> load_pack(const T* row, int col, int cols) {
+    return place_pack<NARROW>(fetch_pack<NARROW, N>(row, col, cols), col, cols);
 }
 
-template <typename T>
-__device__ inline void store_eight(T* p, const Eight<T>& r, int valid) {
-    if (valid >= 8) {
-        if constexpr (sizeof(T) == 2) {
-            store_16(p, __builtin_bit_cast(i32x4, r));
-        } else {
-            const i32x8 v = __builtin_bit_cast(i32x8, r);
-            store_16(p, __builtin_shufflevector(v, v, 0, 1, 2, 3));
-            store_16(p + 4, __builtin_shufflevector(v, v, 4, 5, 6, 7));
+template <typename T, int N>
+__device__ inline void store_pack(T* p, const Pack<T, N>& r, int valid) {
+    if (valid >= N) {
+        constexpr int kEach = 16 / sizeof(T);
+#pragma unroll
+        for (int i = 0; i < N; i += kEach) {
+            i32x4 part;
+            __builtin_memcpy(&part, r.v + i, 16);
+            store_16(p + i, part);
         }
         return;
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < N; ++i)
         if (i < valid) p[i] = r.v[i];
 }
 
