@@ -437,11 +437,9 @@ struct Fragments {
 // The wave's 32 rows (x) by 32 * WT columns (w) of accumulators through LDS of its own, so that
 // a row of y leaves in pieces of 16 bytes.  Lane l holds y[m = l % 32][8 * (e / 4) + 4 * (l / 32)
 // + e % 4] of every accumulator; piece q of row m lies at place q ^ m: reads and writes both
-// spread over the banks.  STREAM: past the L2, in the tiles for products whose y is most of their
-// traffic (128 x 256, 8192 x 8192 x 512: 40 us against 43; 55360 x 256 x 768: 13.5 against 15.4; with long
-// sums, where L2 holds the operands, it costs: 256 x 256, 8192 x 8192 x 1024: 66 against 62).
-template <typename T, bool STREAM, int WT>
-__device__ inline void store_rows(const Product& p, const f32x16 (&acc)[WT], const float* bias, uint8_t* lds, int m0, int n0, int lane) {
+// spread over the banks.  `stream`: past the L2.
+template <typename T, int WT>
+__device__ inline void store_rows(const Product& p, bool stream, const f32x16 (&acc)[WT], const float* bias, uint8_t* lds, int m0, int n0, int lane) {
     constexpr int kPieces = 32 * WT * sizeof(T) / 16, kEach = 16 / sizeof(T);
     const int r = lane & 31, half = lane >> 5;
 #pragma unroll
@@ -466,16 +464,16 @@ __device__ inline void store_rows(const Product& p, const f32x16 (&acc)[WT], con
         return *reinterpret_cast<const i32x4*>(lds + row * (kPieces * 16) + ((piece ^ (row & (kPieces - 1))) << 4));
     };
     if (m0 + 32 <= p.rows && n0 + 32 * WT <= p.n) {
-        i32x4 v[32 / kRows];
+        // The empty statements keep the compiler from joining the two loops, which would drop the hint.
+        if (stream) {
+            asm volatile("; past the L2");
 #pragma unroll
-        for (int k = 0; k < 32 / kRows; ++k) v[k] = own(k * kRows + sub);
+            for (int k = 0; k < 32; k += kRows)
+                __builtin_nontemporal_store(own(k + sub), reinterpret_cast<Unaligned<T>*>(y + (int64_t)k * p.n));
+            asm volatile("; past the L2");
+        } else {
 #pragma unroll
-        for (int k = 0; k < 32 / kRows; ++k) {
-            auto* at = reinterpret_cast<Unaligned<T>*>(y + (int64_t)k * kRows * p.n);
-            if (STREAM)
-                __builtin_nontemporal_store(v[k], at);
-            else
-                *at = v[k];
+            for (int k = 0; k < 32; k += kRows) store_16(y + (int64_t)k * p.n, own(k + sub));
         }
         return;
     }
@@ -695,17 +693,23 @@ __global__ __launch_bounds__((Tiling<TM, TN>::kThreads), (Tiling<TM, TN>::kWaves
     constexpr int kOwn = 32 * 32 * WT * 4;
     static_assert(L::kWaves * kOwn <= L::kStages * L::kStage, "the stages hold the waves' parts of y");
     uint8_t* own = lds + wave * kOwn;
+    // The smaller tiles, whose y is most of the traffic, store it past the L2 where its rows are whole lines
+    // (us, 30000 x 1024 x 1000: 28.2 against 31.0 through the L2, 55360 x 256 x 768: 13.9 against 15.8; but rows of 1000,
+    // which share lines: 35.3 against 32.3, and 28.6 against 17.6 for 30000 x 1000 x 128).  The largest leaves L2 to
+    // the operands and y alike (8192 x 8192 x 1024: 66 past it, 62 through it).
+    const int y_size = p.y_type == GLV_F32 ? 4 : 2;
+    const bool stream = TM == 128 && ((reinterpret_cast<uintptr_t>(p.y) | (uintptr_t)p.n * y_size) & 127) == 0;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         f32x16 part[WT];
 #pragma unroll
         for (int i = 0; i < WT; ++i) part[i] = acc[i][j];
         if (p.y_type == GLV_F32)
-            store_rows<float, TM == 128>(p, part, bias + nw, own, m0 + mw + j * 32, n0 + nw, lane);
+            store_rows<float>(p, stream, part, bias + nw, own, m0 + mw + j * 32, n0 + nw, lane);
         else if (p.y_type == GLV_BF16)
-            store_rows<bf16, TM == 128>(p, part, bias + nw, own, m0 + mw + j * 32, n0 + nw, lane);
+            store_rows<bf16>(p, stream, part, bias + nw, own, m0 + mw + j * 32, n0 + nw, lane);
         else
-            store_rows<f16, TM == 128>(p, part, bias + nw, own, m0 + mw + j * 32, n0 + nw, lane);
+            store_rows<f16>(p, stream, part, bias + nw, own, m0 + mw + j * 32, n0 + nw, lane);
         wave_lds_fence();
     }
 }
