@@ -909,23 +909,32 @@ extern "C" int glv_mxfp4_product(const void* x_dev, const uint8_t* x_scales_dev,
         if (rc != GLV_OK) return rc;
         p.xc = codes, p.xs = scales;
     }
-    // Which tile, measured in us for codes that are there already, y in bfloat16:
-    //                        32 x 32   128 x 128   128 x 256   256 x 256   (rows of x times rows of w)
-    //    1000 x 1000 x 1024      5.6         7.7        12.0        13.7
-    //    1024 x 2048 x  256      5.2         5.5         7.5         8.6
-    //    1024 x 2048 x 1024      7.9         7.0        10.0        11.7
-    //    2048 x 2048 x 4096     36.8        15.4        21.4        26.6
-    //   16384 x  256 x 1024     15.3         7.5        10.4        12.6
-    //   55360 x  256 x  512     24.2        13.0        11.9        13.9
-    //   10560 x 4096 x 1024     94.9        34.2        37.0        43.3
-    //    8192 x 8192 x 2048    256          82.4        78.5        84.2
-    //    8192 x 8192 x 4096    481         147         138         135
-    // 32 x 32 spreads small outputs over the chip; 128 x 128 has three workgroups on a CU to hide each
-    // other's ends; with one tile across w, x is read once; long sums on a full chip pay for the largest.
+    // Which tile, measured in us with x and y in bfloat16, quantising x included (in brackets without it):
+    //                            32 x 32    128 x 128     128 x 256     256 x 256   (rows of x times rows of w)
+    //    1000 x 1000 x 1024        (5.6)        (7.7)        (12.0)        (13.7)
+    //    2048 x 2048 x 4096       (36.8)   21.3 (14.6)   26.6 (20.2)   32.5 (25.9)
+    //    2304 x 4096 x 4096                35.5 (28.3)   39.3 (32.2)   34.8 (28.1)
+    //   16384 x  256 x 1024       (15.3)   15.1 ( 8.2)   17.4 (10.1)   19.7 (12.2)
+    //   20000 x  512 x 1024                30.2 (11.1)   22.7 (12.7)   23.8 (14.3)
+    //   55360 x  256 x  512       (24.2)   29.7 (12.8)   23.5 (10.9)   25.1 (12.9)
+    //   30000 x  640 x 1024                35.1 (18.9)   38.6 (24.7)
+    //   10560 x 2048 x  512                19.8 (14.6)   22.2 (17.6)   25.8 (19.9)
+    //   10560 x 4096 x 1024       (94.9)   64.4 (39.7)   47.2 (39.1)   55.3 (45.5)
+    //   10560 x 2048 x 4096                71.9 (54.8)   71.6 (54.4)   77.5 (60.1)
+    //    8192 x 8192 x 1024                73.0 (56.3)   62.1 (55.7)   78.9 (73.0)
+    //    4096 x 4096 x 4096                49.3 (41.2)   47.2 (39.7)   45.3 (37.3)
+    // 32 x 32 spreads small outputs over the chip; 128 x 128 has three workgroups on a CU to hide each other's ends,
+    // but reads twice the LDS bytes of the larger tiles for a product, and where it follows a kernel bound by memory its
+    // draw makes the card lower its clock (10560 x 4096 x 1024: 38 us of zeros, 64 of random values; 41 and 47 for
+    // 128 x 256).  So sums of some length take 128 x 256, if it leaves no CU without work and does not reach much past
+    // w's rows, and so do shorter ones that it finishes in one round of two workgroups a CU.  Long sums take the
+    // largest where its rounds, of one workgroup a CU, are no longer than those of 128 x 256, half as much each.
     if (all * n_out >= (int64_t)2 << 20) {
+        const int64_t rows128 = (all + 127) / 128, narrow = rows128 * ((n_out + 127) / 128), mid = rows128 * ((n_out + 255) / 256);
         const int64_t wide = ((all + 255) / 256) * ((n_out + 255) / 256);
-        if (wide >= 192 && p.taps * p.groups >= 32) return launch_tiled<256, 256>(p, st);
-        if (n_out > 128 && n_out <= 256 && all >= 32768) return launch_tiled<128, 256>(p, st);
+        const int groups = p.taps * p.groups;
+        if (groups >= 32 && 2 * ((wide + 255) / 256) <= (mid + 255) / 256) return launch_tiled<256, 256>(p, st);
+        if (32 * mid <= 17 * narrow && (groups >= 8 ? mid >= 256 : mid > 384 && mid <= 512)) return launch_tiled<128, 256>(p, st);
         return launch_tiled<128, 128>(p, st);
     }
     launch_direct<void>(p, (unsigned)tiles, st);
