@@ -593,6 +593,9 @@ def test_refusals_without_gpu():
         MXFP4Tensor((5, 40), torch.zeros(5 * 68 + 1, dtype=torch.uint8)[1:])
     with pytest.raises(ValueError, match="last dimension"):
         MXFP4Tensor((5, 0), torch.zeros(0, dtype=torch.uint8))
+    for shape in ((0, 1 << 32), (1 << 32, 0, 40)):
+        with pytest.raises(ValueError, match="too large"):
+            MXFP4Tensor(shape, torch.zeros(0, dtype=torch.uint8))
     assert w.codes.shape == (1, 5, 64) and w.scales.shape == (1, 5, 4) and w.to("cpu").shape == (5, 40)
     for name in ("MXFP4Tensor", "Norm", "block_norm", "mxfp4_conv1d", "mxfp4_linear", "mxfp4_quantize"):
         assert name in tts_amd.__all__
@@ -648,6 +651,30 @@ def test_c_entries_validate_before_any_device_call():
         assert norm(**kw) == -1, kw
         assert b"glv_block_norm" in lib.glv_last_error()
     assert norm(rows=0, u=None, y=None) == 0
+
+    # more threads than one launch can hold
+    kw = dict(rows=1 << 24, cols=32768)
+    assert quantize(**kw) == norm(**kw) == lib.glv_mxfp4_dequantize(a, a, kw["rows"], kw["cols"], 0, a, None) == -1
+    assert b"too large for one call" in lib.glv_last_error()
+    for n in (1 << 16, 1 << 18):
+        assert product(kind=3, xs=a, rows=1 << 24, n=n) == -1 and b"too large for one call" in lib.glv_last_error()
+
+
+@gpu
+def test_sizes_that_do_not_fit_the_librarys_ints_are_refused():
+    """Nothing here is allocated at its size: the rows are one row, seen many times."""
+    one = torch.ones(1, 1, 8, device="cuda", dtype=torch.float16)
+    w, wc = mxfp4_quantize(one[0]), mxfp4_quantize(one.expand(1, 3, 8))
+    long, deep = one[0].expand((1 << 32) + 3, 8), one[None].expand(1 << 17, 1 << 16, 3, 8)
+    for call in (lambda: mxfp4_quantize(long), lambda: mxfp4_linear(long, w), lambda: mxfp4_conv1d(long, wc),
+                 lambda: block_norm(long, post=Norm()), lambda: mxfp4_quantize(long[None]), lambda: mxfp4_linear(deep, w)):
+        with pytest.raises(ValueError, match="larger than|hold more than"):
+            call()
+    with pytest.raises(ValueError, match="dilation"):
+        mxfp4_conv1d(one, wc, dilation=(1 << 32) + 1)
+    # 2^32 + 2^16 rows in all, which an int would take for 2^16
+    with pytest.raises(tts_amd._lib.GlvError, match="4295032832 rows"):
+        mxfp4_linear(one.expand(1 << 16, (1 << 16) + 1, 8), w)
 
 
 @gpu

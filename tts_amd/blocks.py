@@ -22,6 +22,7 @@ _MXFP4 = 3
 _ACTIVATIONS = {None: 0, "relu": 1}
 _NORMS = {"layer": 1, "rms": 2}
 _GROUP = 128  # columns that share one dword of scales
+_INT = (1 << 31) - 1  # the library counts in ints; its own limits, which it names, are lower
 
 
 # The calls below take a few microseconds on the host, as much as a small launch on the device, so
@@ -62,8 +63,12 @@ def _vector(t, name, n, index):
 def _rows(x, shape):
     """(tensor, batch, rows, batch stride, row stride) of x as (batch, rows, cols) with a contiguous last
     dimension; a copy only where no view will do."""
+    if max(shape) > _INT:
+        raise ValueError(f"a dimension of {tuple(shape)} is larger than {_INT}")
     dims = len(shape)
     if dims > 3:
+        if shape[:-2].numel() > _INT:
+            raise ValueError(f"the leading dimensions of {tuple(shape)} hold more than {_INT} entries")
         x = x.reshape(-1, shape[-2], shape[-1]) if x.numel() else x.new_empty((0, shape[-2], shape[-1]))
         shape, dims = x.shape, 3
     strides = x.stride()
@@ -95,6 +100,8 @@ class MXFP4Tensor:
         if len(shape) < 1 or shape[-1] < 1:
             raise ValueError(f"an MXFP4 tensor needs a last dimension of at least 1, got {tuple(shape)}")
         rows, groups = shape[:-1].numel(), -(-shape[-1] // _GROUP)
+        if max(shape) > _INT or rows > _INT:
+            raise ValueError(f"an MXFP4 tensor of shape {tuple(shape)} is too large")
         size = groups * rows * 68
         if data.dtype != torch.uint8 or data.shape != (size,) or not data.is_contiguous():
             raise ValueError(f"data must be a contiguous uint8 tensor of shape ({size},), got {data.dtype} "
@@ -199,7 +206,7 @@ def _product(x, weight, bias, taps, dilation, activation, out_dtype):
     if scales is None:
         like, batch, rows, batch_stride, row_stride = _rows(x, shape)
         data = like.data_ptr()
-    if taps == 1 and batch != 1 and batch_stride == rows * row_stride:
+    if taps == 1 and batch != 1 and batch_stride == rows * row_stride and batch * rows <= _INT:
         batch, rows = 1, batch * rows  # rows of a linear layer need no entries
     if out_dtype is None:
         out_dtype, out_kind = (torch.float32, 0) if kind == _MXFP4 else (x.dtype, kind)
@@ -261,8 +268,8 @@ def mxfp4_conv1d(x, weight, bias=None, *, dilation=1, activation=None, out_dtype
         raise ValueError(f"x must be (B, T, C) or (T, C), got {tuple(x.shape)}")
     if weight.shape[1] < 1:
         raise ValueError("weight must have at least one tap")
-    if int(dilation) != dilation or dilation < 1:
-        raise ValueError(f"dilation must be a positive integer, got {dilation!r}")
+    if int(dilation) != dilation or not 1 <= dilation <= _INT:
+        raise ValueError(f"dilation must be a positive integer of at most {_INT}, got {dilation!r}")
     return _product(x, weight, bias, weight.shape[1], int(dilation), activation, out_dtype)
 
 

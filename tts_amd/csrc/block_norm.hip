@@ -186,8 +186,10 @@ __global__ __launch_bounds__(LANES > 0 ? 256 : 1024) void block_norm_kernel(Bloc
 // 4096 x 16384: 317 us with 1024 of four, half of them idle, 185 with 1024 of two), four where sixteen waves
 // would not do.
 template <typename T, typename W>
-void launch(const BlockNorm& p, hipStream_t st) {
+int launch(const BlockNorm& p, hipStream_t st) {
     const int pieces = (p.cols + 7) / 8;  // a lane holds one, two or four of them
+    const int threads = (pieces <= 2048 ? (pieces + 127) / 128 : (pieces + 255) / 256) * 64;  // of a workgroup to itself
+    if (pieces > 128 && too_large(p.rows, threads)) return report(GLV_ERR_INVALID, "glv_block_norm: rows x columns too large for one call");
     auto rows_a_wave = [&](int lanes) { return dim3((unsigned)(((int64_t)p.rows * lanes + 255) / 256)); };
     if (p.cols < 16 / (int)sizeof(T))
         hipLaunchKernelGGL((block_norm_kernel<T, W, 16, 1, true>), rows_a_wave(16), dim3(256), 0, st, p);
@@ -200,9 +202,10 @@ void launch(const BlockNorm& p, hipStream_t st) {
     else if (pieces <= 128)
         hipLaunchKernelGGL((block_norm_kernel<T, W, 64, 2>), rows_a_wave(64), dim3(256), 0, st, p);
     else if (pieces <= 2048)
-        hipLaunchKernelGGL((block_norm_kernel<T, W, 0, 2>), dim3(p.rows), dim3((pieces + 127) / 128 * 64), 0, st, p);
+        hipLaunchKernelGGL((block_norm_kernel<T, W, 0, 2>), dim3(p.rows), dim3(threads), 0, st, p);
     else
-        hipLaunchKernelGGL((block_norm_kernel<T, W, 0, 4>), dim3(p.rows), dim3((pieces + 255) / 256 * 64), 0, st, p);
+        hipLaunchKernelGGL((block_norm_kernel<T, W, 0, 4>), dim3(p.rows), dim3(threads), 0, st, p);
+    return launch_status("block_norm_kernel");
 }
 
 constexpr int kMaxCols = 32768;         // 1024 threads of 32 columns
@@ -249,11 +252,7 @@ extern "C" int glv_block_norm(const void* u_dev, int type, int batch, int rows, 
     p.y = y_dev, p.z = z_dev;
     p.rows = batch * rows, p.T = rows, p.cols = cols;
     hipStream_t st = (hipStream_t)stream;
-    if (type == GLV_F32)
-        launch<float, float>(p, st);
-    else if (type == GLV_BF16)
-        vector_type == GLV_F32 ? launch<bf16, float>(p, st) : launch<bf16, bf16>(p, st);
-    else
-        vector_type == GLV_F32 ? launch<f16, float>(p, st) : launch<f16, f16>(p, st);
-    return launch_status("block_norm_kernel");
+    if (type == GLV_F32) return launch<float, float>(p, st);
+    if (type == GLV_BF16) return vector_type == GLV_F32 ? launch<bf16, float>(p, st) : launch<bf16, bf16>(p, st);
+    return vector_type == GLV_F32 ? launch<f16, float>(p, st) : launch<f16, f16>(p, st);
 }

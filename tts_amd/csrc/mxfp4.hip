@@ -717,7 +717,9 @@ __global__ __launch_bounds__((Tiling<TM, TN>::kThreads), (Tiling<TM, TN>::kWaves
 template <int TM, int TN>
 int launch_tiled(const Product& p, hipStream_t st) {
     using L = Tiling<TM, TN>;
-    const unsigned tiles = (unsigned)((p.rows + TM - 1) / TM) * ((p.n + TN - 1) / TN);
+    const int64_t count = (int64_t)((p.rows + TM - 1) / TM) * ((p.n + TN - 1) / TN);
+    if (too_large(count, L::kThreads)) return report(GLV_ERR_INVALID, "glv_mxfp4_product: rows x n_out too large for one call");
+    const unsigned tiles = (unsigned)count;
     if (p.taps > 1)
         hipLaunchKernelGGL((product_tiled_kernel<true, TM, TN>), dim3(tiles), dim3(L::kThreads), 0, st, p);
     else
@@ -726,11 +728,13 @@ int launch_tiled(const Product& p, hipStream_t st) {
 }
 
 // rows sixteen at a time by groups four at a time
-unsigned span_blocks(int rows, int groups) { return (unsigned)((rows + 15) / 16) * ((groups + 3) / 4); }
+int64_t span_blocks(int rows, int groups) { return (int64_t)((rows + 15) / 16) * ((groups + 3) / 4); }
 
-int quantise(const void* x, int type, Rows xr, int rows, int cols, uint8_t* codes, uint8_t* scales, hipStream_t st) {
+int quantise(const char* what, const void* x, int type, Rows xr, int rows, int cols, uint8_t* codes, uint8_t* scales, hipStream_t st) {
     const int groups = (cols + kGroup - 1) / kGroup;
-    const dim3 grid(span_blocks(rows, groups)), block(256);
+    const int64_t blocks = span_blocks(rows, groups);
+    if (too_large(blocks, 256)) return report(GLV_ERR_INVALID, "%s: rows x columns too large for one call", what);
+    const dim3 grid((unsigned)blocks), block(256);
     auto launch = [&](auto* typed) {
         using T = std::remove_const_t<std::remove_pointer_t<decltype(typed)>>;
         if (cols < 8)
@@ -775,7 +779,7 @@ bool quantised_in_product(int64_t rows, int cols, int n_out, int taps, int dilat
 }
 
 // Row counts and widths are ints in the kernels, row * groups is formed in 64 bits, and every
-// launch counts its workgroups in one 31-bit dimension: these limits keep all of that in range.
+// launch counts its workgroups in one dimension: these limits keep all of that in range.
 constexpr int64_t kMaxRows = 1 << 24;
 constexpr int kMaxCols = 1 << 18;
 
@@ -812,7 +816,7 @@ extern "C" int glv_mxfp4_quantize(const void* x_dev, int x_type, int batch, int 
     if (misaligned(x_dev, x_type == GLV_F32 ? 4 : 2)) return report(GLV_ERR_INVALID, "%s: x is not aligned to its elements", what);
     rc = check_quantised(what, codes_dev, scales_dev);
     if (rc != GLV_OK) return rc;
-    return quantise(x_dev, x_type, Rows{batch_stride, row_stride, rows, batch == 1}, (int)all, cols, codes_dev, scales_dev,
+    return quantise(what, x_dev, x_type, Rows{batch_stride, row_stride, rows, batch == 1}, (int)all, cols, codes_dev, scales_dev,
                     (hipStream_t)stream);
 }
 
@@ -828,7 +832,9 @@ extern "C" int glv_mxfp4_dequantize(const uint8_t* codes_dev, const uint8_t* sca
     rc = check_quantised(what, codes_dev, scales_dev);
     if (rc != GLV_OK) return rc;
     const int groups = (cols + kGroup - 1) / kGroup;
-    const dim3 grid(span_blocks(rows, groups)), block(256);
+    const int64_t blocks = span_blocks(rows, groups);
+    if (too_large(blocks, 256)) return report(GLV_ERR_INVALID, "%s: rows x columns too large for one call", what);
+    const dim3 grid((unsigned)blocks), block(256);
     hipStream_t st = (hipStream_t)stream;
     if (out_type == GLV_F32)
         hipLaunchKernelGGL(dequantise_kernel<float>, grid, block, 0, st, codes_dev, scales_dev, rows, cols, groups, (float*)out_dev);
@@ -883,7 +889,6 @@ extern "C" int glv_mxfp4_product(const void* x_dev, const uint8_t* x_scales_dev,
     p.bias = bias_dev, p.bias_type = bias_type, p.least = activation == GLV_ACT_RELU ? 0.f : -__builtin_huge_valf();
     p.y = y_dev, p.y_type = y_type;
     const int64_t tiles = ((all + 31) / 32) * (int64_t)((n_out + 31) / 32);
-    if (tiles > INT32_MAX) return report(GLV_ERR_INVALID, "%s: rows x n_out too large for one call", what);
     if (x_type == GLV_MXFP4) {
         rc = check_quantised(what, x_dev, x_scales_dev);
         if (rc != GLV_OK) return rc;
@@ -905,7 +910,7 @@ extern "C" int glv_mxfp4_product(const void* x_dev, const uint8_t* x_scales_dev,
         if (misaligned(workspace_dev, 16)) return report(GLV_ERR_INVALID, "%s: the workspace is not 16-byte aligned", what);
         uint8_t* codes = static_cast<uint8_t*>(workspace_dev);
         uint8_t* scales = codes + all * p.groups * kGroupBytes;
-        rc = quantise(x_dev, x_type, Rows{x_batch_stride, x_row_stride, rows, batch == 1}, p.rows, cols, codes, scales, st);
+        rc = quantise(what, x_dev, x_type, Rows{x_batch_stride, x_row_stride, rows, batch == 1}, p.rows, cols, codes, scales, st);
         if (rc != GLV_OK) return rc;
         p.xc = codes, p.xs = scales;
     }

@@ -26,6 +26,9 @@ inline int launch_status(const char* what) {
     return e == hipSuccess ? GLV_OK : report(GLV_ERR_HIP, "%s: launch failed: %s", what, hipGetErrorString(e));
 }
 
+// A launch counts its threads in 32 bits.
+inline bool too_large(int64_t blocks, int threads) { return blocks * threads > UINT32_MAX; }
+
 inline bool float_type(int type) { return type == GLV_F32 || type == GLV_BF16 || type == GLV_F16; }
 
 }  // namespace glv
