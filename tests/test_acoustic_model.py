@@ -214,6 +214,24 @@ def test_mxfp4_blocks_against_the_oracle_and_back():
 
 
 @pytest.mark.gpu
+def test_mxfp4_follows_the_weights_of_a_part_and_of_a_copy():
+    import copy
+    ids = np.random.default_rng(10).integers(1, VOCAB, 20)[None]
+    durations = np.full(ids.shape, np.log(2.0), np.float32)
+    w, other = random_weights(np.random.default_rng(11)), random_weights(np.random.default_rng(12))
+    model = FastSpeechAcousticModel(VOCAB).load_keras_weights(w).cuda().use_mxfp4()
+    want = FastSpeechAcousticModel(VOCAB).load_keras_weights(other)
+    twin = copy.deepcopy(model)
+    first = model((ids, durations))
+    for name, part in want.named_children():
+        getattr(model, name).load_state_dict(part.state_dict())
+    assert torch.equal(model((ids, durations)), want.cuda().use_mxfp4()((ids, durations)))
+    assert torch.equal(twin((ids, durations)), first)
+    torch.nn.ModuleList([twin]).load_state_dict({"0." + k: v for k, v in want.state_dict().items()})
+    assert torch.equal(twin((ids, durations)), want((ids, durations)))
+
+
+@pytest.mark.gpu
 def test_mxfp4_model_feeds_the_vocoder():
     from tts_amd.acoustic import synthesize
     rng = np.random.default_rng(9)

@@ -388,6 +388,25 @@ def test_block_norm_parts(dtype):
 
 
 @gpu
+@pytest.mark.parametrize("rows,cols", [(1, 1), (5, 3), (17, 129), (33, 250), (9, 505), (5, 1001), (3, 4097), (2, 20001)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_block_norm_in_place_of_each_input(dtype, rows, cols):
+    """From C, y may be u, gate or residual itself."""
+    from tts_amd import _lib
+    rng = np.random.default_rng(rows + cols)
+    u, gate, residual = (draw(rng, rows, cols, dtype=dtype) for _ in range(3))
+    want, wantz = block_norm(u, post=Norm(), gate=gate, residual=residual, pre=Norm(kind="rms"))
+    for which in range(3):
+        t = [u.clone(), gate.clone(), residual.clone()]
+        z = torch.empty_like(u)
+        rc = _lib.load().glv_block_norm(
+            t[0].data_ptr(), TYPES.index(dtype), 1, rows, cols, 0, cols, 0, 1, None, None, 1e-5, t[1].data_ptr(), 0, cols, 1, None,
+            1.0, t[2].data_ptr(), 0, cols, 2, None, None, 1e-5, t[which].data_ptr(), z.data_ptr(),
+            torch.cuda.current_stream().cuda_stream)
+        assert rc == 0 and torch.equal(t[which], want) and torch.equal(z, wantz)
+
+
+@gpu
 def test_block_norm_any_strides_and_leading_dimensions():
     rng = np.random.default_rng(12)
     base = draw(rng, 4, 6, 150)

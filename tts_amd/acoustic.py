@@ -72,6 +72,11 @@ class _SequenceConv(nn.Conv1d):
     def __init__(self, in_dim, out_dim, kernel, dilation=1):
         super().__init__(in_dim, out_dim, kernel, padding="same", dilation=dilation)
         self.register_buffer("mxfp4_data", None, persistent=False)
+        self.register_load_state_dict_post_hook(_SequenceConv.refresh)  # of this layer or of a module around it
+
+    def refresh(self, *unused):
+        if self.mxfp4_data is not None:
+            self.quantize(True)
 
     def quantize(self, on):
         self.mxfp4_data = mxfp4_quantize(self.weight.detach().permute(0, 2, 1)).data if on else None
@@ -172,7 +177,6 @@ class FastSpeechAcousticModel(nn.Module):
         self.mel_out = _SequenceConv(hidden_dim, mel_dim, 1)
         self.post_net = PostNet(mel_dim)
         self.last_duration_prediction = None
-        self.register_load_state_dict_post_hook(FastSpeechAcousticModel._refresh_mxfp4)
         self.eval()
 
     @torch.no_grad()
@@ -201,7 +205,7 @@ class FastSpeechAcousticModel(nn.Module):
         in place of torch's products and norms.  The model must be on a ROCm GPU.  The LSTMs, the duration
         predictor's last layer and the post-net, whose five applications of one layer would compound the
         rounding, stay in the model's own type.  The float weights remain; loading weights
-        (`load_keras_weights`, `load_state_dict`) quantises them anew, after other changes to them call
+        (`load_keras_weights`, `load_state_dict` of the model or a part of it) quantises them anew, after other changes to them call
         this again.  ``use_mxfp4(False)`` returns to the float form."""
         for layer in self._mxfp4_layers():
             layer.quantize(on)
@@ -209,11 +213,6 @@ class FastSpeechAcousticModel(nn.Module):
 
     def _mxfp4_layers(self):
         return [m for m in self.modules() if isinstance(m, _SequenceConv)]
-
-    def _refresh_mxfp4(self, *unused):
-        for layer in self._mxfp4_layers():
-            if layer.mxfp4_data is not None:
-                layer.quantize(True)
 
     # -- Keras checkpoint layout ------------------------------------------------------
     def load_keras_weights(self, w):
@@ -259,7 +258,8 @@ class FastSpeechAcousticModel(nn.Module):
             norm(self.post_net.bnorm1, "post_bn")
             self.post_net.bnorm1.running_mean.copy_(t(w["post_bn_mean"]))
             self.post_net.bnorm1.running_var.copy_(t(w["post_bn_var"]))
-        self._refresh_mxfp4()
+        for layer in self._mxfp4_layers():
+            layer.refresh()
         return self
 
 
