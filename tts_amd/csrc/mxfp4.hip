@@ -259,11 +259,48 @@ __device__ inline f32x16 step(i32x4 w, i32x4 x, int wscale, int xscale, f32x16 a
     return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(widen(w), widen(x), acc, 4, 4, S, wscale, S, xscale);
 }
 
+// The workgroup quantises rows first .. first + span - 1 of x, whatever entries they belong to, into LDS:
+//   codes [group][row][64], piece q of 16 bytes of row i at place q ^ (i / 4 % 4);  scales [group][row][4]
+// Sixteen lanes that read one piece of sixteen rows in a run then touch each of the 64 banks once.
+template <typename X, int THREADS>
+__device__ inline void quantise_rows(const Product& p, int first, int span, uint32_t* codes, uint8_t* scales) {
+    constexpr int kTeams = THREADS / 16, kDeep = sizeof(X) == 4 ? 4 : 8;  // sixteen lanes a row and group
+    const int team = threadIdx.x >> 4, piece = threadIdx.x & 15, units = span * p.groups;
+    // unit u is group u % groups of row u / groups; one team's units are kTeams apart
+    struct Unit {
+        int i, gx;
+    };
+    const int step_i = kTeams / p.groups, step_gx = kTeams - step_i * p.groups;
+    auto next = [&](Unit u) {
+        u.i += step_i, u.gx += step_gx;
+        const bool over = u.gx >= p.groups;
+        return Unit{u.i + over, over ? u.gx - p.groups : u.gx};
+    };
+    Unit at{team / p.groups, team % p.groups};
+    for (int u0 = team; u0 < units; u0 += kTeams * kDeep) {
+        Eight<X> v[kDeep];  // all loads before the first use
+        Unit u = at;
+#pragma unroll
+        for (int k = 0; k < kDeep; ++k, u = next(u)) {
+            if (u0 + k * kTeams >= units) break;
+            v[k] = fetch_pack<false, 8>(static_cast<const X*>(p.x) + row_offset(p.xr, first + u.i), u.gx * kGroup + piece * 8, p.cols);
+        }
+#pragma unroll
+        for (int k = 0; k < kDeep; ++k, at = next(at)) {
+            if (u0 + k * kTeams >= units) break;
+            int byte;
+            const uint32_t c = quantise_eight(place_pack<false>(v[k], at.gx * kGroup + piece * 8, p.cols), &byte);
+            const int row = at.gx * span + at.i;
+            codes[(row * 4 + (((piece >> 2) ^ (at.i >> 2)) & 3)) * 4 + (piece & 3)] = c;
+            if ((piece & 3) == 0) scales[row * 4 + (piece >> 2)] = (uint8_t)byte;
+        }
+    }
+}
+
 // One 32 x 32 tile of y a workgroup; the waves deal the groups out among themselves and their sums meet
 // in LDS in a fixed order.  X is `void` for activations that are quantised already; otherwise the
 // workgroup first quantises the rows of x that its tile reaches, all groups of them, into LDS, so that
 // a small product is one launch, and every tap of a convolution finds them there.
-//   codes in LDS  [group][row][64], piece q of 16 bytes of row i at place q ^ (i / 4 % 4);  scales [group][row][4]
 template <typename X, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void product_direct_kernel(Product p) {
     constexpr bool kOwn = !std::is_void_v<X>;
@@ -296,37 +333,7 @@ __global__ __launch_bounds__(WAVES * 64) void product_direct_kernel(Product p) {
     uint32_t* const codes = reinterpret_cast<uint32_t*>(held);
     uint8_t* const scales = held + span * p.groups * kGroupBytes;
     if constexpr (kOwn) {
-        constexpr int kTeams = WAVES * 4, kDeep = sizeof(X) == 4 ? 4 : 8;  // sixteen lanes a row and group
-        const int team = threadIdx.x >> 4, piece = threadIdx.x & 15, units = span * p.groups;
-        // unit u is group u % groups of row u / groups; one team's units are kTeams apart
-        struct Unit {
-            int i, gx;
-        };
-        const int step_i = kTeams / p.groups, step_gx = kTeams - step_i * p.groups;
-        auto next = [&](Unit u) {
-            u.i += step_i, u.gx += step_gx;
-            const bool over = u.gx >= p.groups;
-            return Unit{u.i + over, over ? u.gx - p.groups : u.gx};
-        };
-        Unit at{team / p.groups, team % p.groups};
-        for (int u0 = team; u0 < units; u0 += kTeams * kDeep) {
-            Eight<X> v[kDeep];  // all loads before the first use
-            Unit u = at;
-#pragma unroll
-            for (int k = 0; k < kDeep; ++k, u = next(u)) {
-                if (u0 + k * kTeams >= units) break;
-                v[k] = fetch_pack<false, 8>(static_cast<const X*>(p.x) + row_offset(p.xr, first + u.i), u.gx * kGroup + piece * 8, p.cols);
-            }
-#pragma unroll
-            for (int k = 0; k < kDeep; ++k, at = next(at)) {
-                if (u0 + k * kTeams >= units) break;
-                int byte;
-                const uint32_t c = quantise_eight(place_pack<false>(v[k], at.gx * kGroup + piece * 8, p.cols), &byte);
-                const int row = at.gx * span + at.i;
-                codes[(row * 4 + (((piece >> 2) ^ (at.i >> 2)) & 3)) * 4 + (piece & 3)] = c;
-                if ((piece & 3) == 0) scales[row * 4 + (piece >> 2)] = (uint8_t)byte;
-            }
-        }
+        quantise_rows<X, WAVES * 64>(p, first, span, codes, scales);
         __syncthreads();
     }
 
@@ -373,18 +380,25 @@ __global__ __launch_bounds__(WAVES * 64) void product_direct_kernel(Product p) {
 // the product, large: tiles staged through LDS
 // ---------------------------------------------------------------------------
 // A workgroup's tile has TN rows of w and TM of x; a wave multiplies half of the w rows by 64 of x.
-template <int TM, int TN>
+// OWN (X is a float type): the workgroup quantises what its tile reaches of x into LDS before the first product.
+constexpr int kHeldUnits = 392;  // pairs of a row and a group: what three workgroups of 128 x 128 find room for
+template <int TM, int TN, bool OWN>
 struct Tiling {
     static constexpr int kWaves = TM / 32, kThreads = 64 * kWaves, kWt = TN / 64;
     static constexpr int kStages = TM == 256 ? 4 : 3;
     static constexpr int kWavesPerSimd = TN == 128 ? 3 : 2;
+    static constexpr int kStagedX = OWN ? 0 : TM;
     // one stage: the codes of one group of every row of w and of x, then their scales
-    static constexpr int kW = 0, kX = TN * kGroupBytes, kWs = kX + TM * kGroupBytes, kXs = kWs + TN * 4;
-    static constexpr int kStage = kXs + TM * 4;
+    static constexpr int kW = 0, kX = TN * kGroupBytes, kWs = kX + kStagedX * kGroupBytes, kXs = kWs + TN * 4;
+    static constexpr int kStage = kXs + kStagedX * 4;
     // a wave's loads for a stage: pieces of 16 rows of w and x, scales of 64 rows
-    static constexpr int kLoadsW = TN / 16 / kWaves, kLoadsX = TM / 16 / kWaves;
-    static constexpr int kLoadsS = ((TN + TM) / 64 + kWaves - 1) / kWaves;
+    static constexpr int kLoadsW = TN / 16 / kWaves, kLoadsX = kStagedX / 16 / kWaves;
+    static constexpr int kLoadsS = ((TN + kStagedX) / 64 + kWaves - 1) / kWaves;
     static constexpr int kLoads = kLoadsW + kLoadsX + kLoadsS;
+    // OWN: behind the stages the codes of x, a unit of zeros, and their scales
+    static constexpr int kHeld = kStages * kStage, kHeldScales = kHeld + (kHeldUnits + 1) * kGroupBytes;
+    static constexpr int kBytes = OWN ? kHeldScales + (kHeldUnits + 1) * 4 : kHeld;
+    static_assert(kHeld % kGroupBytes == 0, "the two pieces of a lane differ in one bit of their address");
 };
 
 template <int FROM, int TO, typename F>
@@ -504,11 +518,12 @@ __device__ inline void arrive_and_wait() {  // all but the N youngest loads are 
 // r at place q ^ (r / 4 % 4): sixteen lanes that read one piece of sixteen rows then touch each of the
 // 64 banks once.  One stage is multiplied while the others are on their way.  A stage is two steps; the
 // barrier stands early in the second, whose products hide the first reads of the next stage.
-template <bool CONV, int TM, int TN>
-__global__ __launch_bounds__((Tiling<TM, TN>::kThreads), (Tiling<TM, TN>::kWavesPerSimd)) void product_tiled_kernel(Product p) {
-    using L = Tiling<TM, TN>;
+template <typename X, bool CONV, int TM, int TN>
+__global__ __launch_bounds__((Tiling<TM, TN, !std::is_void_v<X>>::kThreads), (Tiling<TM, TN, !std::is_void_v<X>>::kWavesPerSimd)) void product_tiled_kernel(Product p) {
+    constexpr bool OWN = !std::is_void_v<X>;
+    using L = Tiling<TM, TN, OWN>;
     constexpr int WT = L::kWt;
-    __shared__ __align__(1024) uint8_t lds[L::kStages * L::kStage];
+    __shared__ __align__(1024) uint8_t lds[L::kBytes];
     __shared__ __align__(16) float bias[TN];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 31, half = lane >> 5;
@@ -521,8 +536,8 @@ __global__ __launch_bounds__((Tiling<TM, TN>::kThreads), (Tiling<TM, TN>::kWaves
     // Load i of a wave fills 16 rows from (i * waves + wave) * 16 on, lane l the place l % 4 of row l / 4.
     // Rows behind the last repeat it.
     const int place = ((lane & 3) ^ (lane >> 4)) * 16;
-    uint32_t woff[L::kLoadsW], xoff[L::kLoadsX], soff[L::kLoadsS];
-    int xt[L::kLoadsX], st = 0;
+    uint32_t woff[L::kLoadsW], xoff[OWN ? 1 : L::kLoadsX], soff[L::kLoadsS];
+    int xt[OWN ? 1 : L::kLoadsX], st = 0;
 #pragma unroll
     for (int i = 0; i < L::kLoadsW; ++i)
         woff[i] = min(n0 + (i * L::kWaves + wave) * 16 + (lane >> 2), p.n - 1) * p.taps * kGroupBytes + place;
@@ -534,8 +549,11 @@ __global__ __launch_bounds__((Tiling<TM, TN>::kThreads), (Tiling<TM, TN>::kWaves
     }
     // Scales, 64 rows a load: with one load a wave the first TN / 64 waves bring w's, the others x's; with two
     // every wave brings w's and then x's (four waves for two loads of x: two of them the same).
-    const bool first_w = L::kLoadsS == 2 || wave < TN / 64;
-    {
+    const bool first_w = OWN || L::kLoadsS == 2 || wave < TN / 64;
+    const int swave = OWN ? wave & (TN / 64 - 1) : wave;
+    if constexpr (OWN) {
+        soff[0] = min(n0 + swave * 64 + lane, p.n - 1) * p.taps * 4;
+    } else {
         const int m = min(m0 + (L::kLoadsS == 1 ? wave - TN / 64 : wave & (TM / 64 - 1)) * 64 + lane, p.rows - 1);
         if (first_w) soff[0] = min(n0 + wave * 64 + lane, p.n - 1) * p.taps * 4;
         if (!first_w || L::kLoadsS == 2) {
@@ -570,8 +588,8 @@ __global__ __launch_bounds__((Tiling<TM, TN>::kThreads), (Tiling<TM, TN>::kWaves
             }
         } else {
             // with one load a wave, x's scales follow w's as the waves follow each other
-            const bool of_w = L::kLoadsS == 1 ? first_w : si == 0;
-            const uint32_t to = dst + (si == 0 ? L::kWs + wave * 256 : L::kXs + (wave & (TM / 64 - 1)) * 256);
+            const bool of_w = OWN || (L::kLoadsS == 1 ? first_w : si == 0);
+            const uint32_t to = dst + (si == 0 ? L::kWs + swave * 256 : L::kXs + (wave & (TM / 64 - 1)) * 256);
             const uint8_t* from = si == 0 ? sbase + sat : p.xs + xrow * 4;
             if (CONV) {
                 // of w the tap's own scales; of x those of the shifted row
@@ -595,12 +613,39 @@ __global__ __launch_bounds__((Tiling<TM, TN>::kThreads), (Tiling<TM, TN>::kWaves
 #pragma unroll
     for (int c = 0; c < L::kStages; ++c)
         if (c < all) each<0, L::kLoads>([&](auto part) { stage_part(c, part); });
+    const int nw = (wave & 1) * 32 * WT, mw = (wave >> 1) * 64;
+    // OWN: where this lane's two rows of x lie, and the unit that the next reads of them come from (its first
+    // piece; the second is the neighbour)
+    int xi[2] = {}, xe[2] = {}, span = 0;
+    uint32_t xat[2] = {};
+    int rtap = 0, rgx = 0;
+    auto seek = [&]() {
+        const int shift = CONV ? rtap * p.dilation - p.left : 0;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const bool inside = !CONV || (unsigned)(xe[j] + shift) < (unsigned)p.T;
+            const int i = xi[j] + shift, unit = inside ? rgx * span + i : kHeldUnits;
+            xat[j] = L::kHeld + unit * kGroupBytes + ((half * 2 ^ (i >> 2)) & 3) * 16;
+        }
+    };
+    if constexpr (OWN) {
+        const int first = max(m0 - p.left, 0);
+        span = min(min(m0 + TM, p.rows) - 1 + (p.taps - 1) * p.dilation - p.left, p.rows - 1) - first + 1;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int m = min(m0 + mw + j * 32 + r, p.rows - 1);
+            xi[j] = m - first, xe[j] = CONV ? m % p.T : 0;
+        }
+        quantise_rows<X, L::kThreads>(p, first, span, reinterpret_cast<uint32_t*>(lds + L::kHeld), lds + L::kHeldScales);
+        if (threadIdx.x < kGroupBytes / 4) reinterpret_cast<uint32_t*>(lds + L::kHeld + kHeldUnits * kGroupBytes)[threadIdx.x] = 0;
+        if (threadIdx.x == 0) reinterpret_cast<uint32_t*>(lds + L::kHeldScales)[kHeldUnits] = 0;
+        seek();
+    }
     // asked for here, used behind the loop: no wait of its own
     static_assert(L::kThreads >= TN, "a thread for every bias");
     float own_bias = 0.f;
     if (p.bias && n0 + (int)threadIdx.x < p.n && threadIdx.x < TN) own_bias = load_float(p.bias, p.bias_type, n0 + threadIdx.x);
 
-    const int nw = (wave & 1) * 32 * WT, mw = (wave >> 1) * 64;
     // lane l takes, of row l % 32, the blocks 2 * (l / 32) and + 1 in the two steps
     uint32_t at[2];
 #pragma unroll
@@ -611,7 +656,8 @@ __global__ __launch_bounds__((Tiling<TM, TN>::kThreads), (Tiling<TM, TN>::kWaves
     auto fetch = [&](uint32_t base, int k, auto q, Fragments<WT>& f) {
         constexpr bool x = q == 1 || q == WT + 1;
         constexpr int i = q == 0 ? 0 : x ? q / (WT + 1) : q - 1;
-        const i32x4 v = *reinterpret_cast<const i32x4*>(lds + base + (x ? xr : wr) + at[k] + i * 32 * kGroupBytes);
+        const uint32_t from = OWN && x ? xat[x ? i : 0] ^ (k * 16) : base + (x ? xr : wr) + at[k] + i * 32 * kGroupBytes;
+        const i32x4 v = *reinterpret_cast<const i32x4*>(lds + from);
         if constexpr (x)
             f.x[i] = v;
         else
@@ -623,7 +669,8 @@ __global__ __launch_bounds__((Tiling<TM, TN>::kThreads), (Tiling<TM, TN>::kWaves
 #pragma unroll
         for (int i = 0; i < WT; ++i) wnext[i] = *reinterpret_cast<const int*>(lds + base + wsr + i * 128);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) xnext[j] = *reinterpret_cast<const int*>(lds + base + xsr + j * 128);
+        for (int j = 0; j < 2; ++j)
+            xnext[j] = *reinterpret_cast<const int*>(lds + (OWN ? L::kHeldScales + (xat[j] - L::kHeld) / kGroupBytes * 4 : base + xsr + j * 128));
     };
     f32x16 acc[WT][2] = {};
     auto multiply = [&](auto S, auto q, const Fragments<WT>& f) {
@@ -669,6 +716,11 @@ __global__ __launch_bounds__((Tiling<TM, TN>::kThreads), (Tiling<TM, TN>::kWaves
                     arrive_and_wait<0>();
                 slot = slot == L::kStages - 1 ? 0 : slot + 1;
                 base = slot * L::kStage;
+                if constexpr (OWN) {
+                    rgx = rgx == p.groups - 1 ? 0 : rgx + 1;
+                    if (CONV) rtap = rgx > 0 ? rtap : rtap == p.taps - 1 ? 0 : rtap + 1;
+                    seek();
+                }
             }
             // then the next stage's first reads (behind the last stage: of whatever lies there, and nothing
             // uses them), its scales, and the loads into the stage that is free now, over the products left
@@ -691,7 +743,7 @@ __global__ __launch_bounds__((Tiling<TM, TN>::kThreads), (Tiling<TM, TN>::kWaves
     __syncthreads();
     // every read of the stages lies behind: each wave takes a part of them
     constexpr int kOwn = 32 * 32 * WT * 4;
-    static_assert(L::kWaves * kOwn <= L::kStages * L::kStage, "the stages hold the waves' parts of y");
+    static_assert(L::kWaves * kOwn <= L::kBytes, "the stages (and x) hold the waves' parts of y");
     uint8_t* own = lds + wave * kOwn;
     // The smaller tiles, whose y is most of the traffic, store it past the L2 where its rows are whole lines
     // (us, 30000 x 1024 x 1000: 28.2 against 31.0 through the L2, 55360 x 256 x 768: 13.9 against 15.8; but rows of 1000,
@@ -714,16 +766,16 @@ __global__ __launch_bounds__((Tiling<TM, TN>::kThreads), (Tiling<TM, TN>::kWaves
     }
 }
 
-template <int TM, int TN>
+template <int TM, int TN, typename X = void>
 int launch_tiled(const Product& p, hipStream_t st) {
-    using L = Tiling<TM, TN>;
+    using L = Tiling<TM, TN, !std::is_void_v<X>>;
     const int64_t count = (int64_t)((p.rows + TM - 1) / TM) * ((p.n + TN - 1) / TN);
     if (too_large(count, L::kThreads)) return report(GLV_ERR_INVALID, "glv_mxfp4_product: rows x n_out too large for one call");
     const unsigned tiles = (unsigned)count;
     if (p.taps > 1)
-        hipLaunchKernelGGL((product_tiled_kernel<true, TM, TN>), dim3(tiles), dim3(L::kThreads), 0, st, p);
+        hipLaunchKernelGGL((product_tiled_kernel<X, true, TM, TN>), dim3(tiles), dim3(L::kThreads), 0, st, p);
     else
-        hipLaunchKernelGGL((product_tiled_kernel<false, TM, TN>), dim3(tiles), dim3(L::kThreads), 0, st, p);
+        hipLaunchKernelGGL((product_tiled_kernel<X, false, TM, TN>), dim3(tiles), dim3(L::kThreads), 0, st, p);
     return launch_status("product_tiled_kernel");
 }
 
@@ -751,31 +803,42 @@ int quantise(const char* what, const void* x, int type, Rows xr, int rows, int c
     return launch_status("quantise_kernel");
 }
 
-// Rows of x that one tile of 32 rows of y reaches, at most.
-int64_t reached_rows(int64_t rows, int taps, int dilation) {
-    const int64_t span = 32 + (int64_t)(taps - 1) * dilation;
+// Rows of x that one tile of `tile` rows of y reaches, at most.
+int64_t reached_rows(int64_t rows, int tile, int taps, int dilation) {
+    const int64_t span = tile + (int64_t)(taps - 1) * dilation;
     return span < rows ? span : rows;
 }
 
 // Four waves where there are no more groups than that, else eight.
 template <typename X>
-void launch_direct(const Product& p, unsigned tiles, hipStream_t st) {
-    const size_t held = std::is_void_v<X> ? 0 : reached_rows(p.rows, p.taps, p.dilation) * p.groups * (kGroupBytes + 4);
+int launch_direct(const Product& p, unsigned tiles, hipStream_t st) {
+    const size_t held = std::is_void_v<X> ? 0 : reached_rows(p.rows, 32, p.taps, p.dilation) * p.groups * (kGroupBytes + 4);
     if (p.taps * p.groups <= 4)
         hipLaunchKernelGGL((product_direct_kernel<X, 4>), dim3(tiles), dim3(256), held, st, p);
     else
         hipLaunchKernelGGL((product_direct_kernel<X, 8>), dim3(tiles), dim3(512), held, st, p);
+    return launch_status("product_direct_kernel");
 }
 
-// Whether a product quantises its activations itself: every tile of 32 x 32 of y does so anew with the
-// rows it reaches, against a launch and a workspace less.  It does while those are at most 256 pairs
-// of a row and a group (us, bfloat16, device: 32 x 4096 x 1024, 256 pairs, 5.7 against 5.8 in two launches; 32 x
-// 1024 x 2048, 512 pairs, 8.2 against 6.3; 165 rows, 256 -> 256, 5 taps, 80 pairs, 4.2 against 5.6) and at most 8 M
-// elements in all tiles together (865 x 256 x 1024, 7 M, 5.8 against 6.6; 2000 x 500 x 500, 16 M, 9.7 against 7.9).
-bool quantised_in_product(int64_t rows, int cols, int n_out, int taps, int dilation) {
-    const int64_t pairs = reached_rows(rows, taps, dilation) * ((cols + kGroup - 1) / kGroup);
-    const int64_t tiles = ((rows + 31) / 32) * ((n_out + 31) / 32);
-    return cols >= 8 && pairs <= 256 && tiles * pairs * kGroup <= (int64_t)8 << 20;
+// The tile in which a product quantises its activations itself (columns of y; 0: it does not): every tile
+// does so anew with the rows it reaches, against a launch and a workspace less (us, bfloat16, device).
+// 32 x 32, while those are at most 256 pairs of a row and a group (32 x 4096 x 1024, 256 pairs, 5.7 against 5.8
+// in two launches; 32 x 1024 x 2048, 512 pairs, 8.2 against 6.3; 165 rows, 256 -> 256, 5 taps, 80 pairs, 4.2
+// against 5.6) and at most 8 M elements in all tiles together (865 x 256 x 1024, 7 M, 5.8 against 6.6; 2000 x 500 x
+// 500, 16 M, 9.7 against 7.9).
+// 128 x 128 and 128 x 256, where one tile spans w's rows, so that x is still read once, and x fits beside the
+// stages: for narrow w from a tile a CU on (55360 x 80 x 256: 12.9 against 15.3, 120000 x 128 x 384: 26.0 against 30.6;
+// 16384 x 80 x 256: 10.4 against 9.1), for wider w in one round of two a CU (55360 rows, 256 -> 256, 3 taps: 19.3
+// against 21.3, 65500 x 256 x 384: 18.7 against 22.4; 32768 x 200 x 384: 17.9 against 16.4, 120000 x 200 x 384: 40.4
+// against 38.2), for a workgroup's reading, multiplying and writing follow each other.
+int own_tile(int64_t rows, int cols, int n_out, int taps, int dilation) {
+    if (cols < 8) return 0;
+    const int64_t groups = (cols + kGroup - 1) / kGroup, pairs = reached_rows(rows, 32, taps, dilation) * groups;
+    const int64_t tiles = ((rows + 31) / 32) * ((n_out + 31) / 32), high = (rows + 127) / 128;
+    if (pairs <= 256 && tiles * pairs * kGroup <= (int64_t)8 << 20) return 32;
+    if (reached_rows(rows, 128, taps, dilation) * groups > kHeldUnits) return 0;
+    if (n_out <= 128) return high >= 256 ? 128 : 0;
+    return n_out <= 256 && high > 384 && high <= 512 ? 256 : 0;
 }
 
 // Row counts and widths are ints in the kernels, row * groups is formed in 64 bits, and every
@@ -848,7 +911,7 @@ extern "C" int glv_mxfp4_dequantize(const uint8_t* codes_dev, const uint8_t* sca
 extern "C" int64_t glv_mxfp4_product_workspace(int x_type, int batch, int rows, int cols, int n_out, int taps, int dilation) {
     if (batch < 0 || rows < 0 || n_out < 0 || taps < 1 || dilation < 1 || cols < 1 || cols > kMaxCols) return -1;
     if ((int64_t)batch * rows > kMaxRows || !(float_type(x_type) || x_type == GLV_MXFP4)) return -1;
-    if (x_type == GLV_MXFP4 || quantised_in_product((int64_t)batch * rows, cols, n_out, taps, dilation)) return 0;
+    if (x_type == GLV_MXFP4 || own_tile((int64_t)batch * rows, cols, n_out, taps, dilation)) return 0;
     return quantised_bytes((int64_t)batch * rows, (cols + kGroup - 1) / kGroup);
 }
 
@@ -893,15 +956,16 @@ extern "C" int glv_mxfp4_product(const void* x_dev, const uint8_t* x_scales_dev,
         rc = check_quantised(what, x_dev, x_scales_dev);
         if (rc != GLV_OK) return rc;
         p.xc = static_cast<const uint8_t*>(x_dev), p.xs = x_scales_dev;
-    } else if (quantised_in_product(all, cols, n_out, taps, dilation)) {
+    } else if (const int tile = own_tile(all, cols, n_out, taps, dilation)) {
         p.x = x_dev, p.xr = Rows{x_batch_stride, x_row_stride, rows, batch == 1}, p.cols = cols;
-        if (x_type == GLV_F32)
-            launch_direct<float>(p, (unsigned)tiles, st);
-        else if (x_type == GLV_BF16)
-            launch_direct<bf16>(p, (unsigned)tiles, st);
-        else
-            launch_direct<f16>(p, (unsigned)tiles, st);
-        return launch_status("product_direct_kernel");
+        auto launch = [&](auto* typed) {
+            using X = std::remove_pointer_t<decltype(typed)>;
+            if (tile == 256) return launch_tiled<128, 256, X>(p, st);
+            if (tile == 128) return launch_tiled<128, 128, X>(p, st);
+            return launch_direct<X>(p, (unsigned)tiles, st);
+        };
+        if (x_type == GLV_F32) return launch((float*)nullptr);
+        return x_type == GLV_BF16 ? launch((bf16*)nullptr) : launch((f16*)nullptr);
     } else {
         const int64_t need = quantised_bytes(all, p.groups);
         if (!workspace_dev || workspace_bytes < need)
@@ -942,6 +1006,5 @@ extern "C" int glv_mxfp4_product(const void* x_dev, const uint8_t* x_scales_dev,
         if (32 * mid <= 17 * narrow && (groups >= 8 ? mid >= 256 : mid > 384 && mid <= 512)) return launch_tiled<128, 256>(p, st);
         return launch_tiled<128, 128>(p, st);
     }
-    launch_direct<void>(p, (unsigned)tiles, st);
-    return launch_status("product_direct_kernel");
+    return launch_direct<void>(p, (unsigned)tiles, st);
 }
