@@ -297,6 +297,19 @@ __device__ inline void quantise_rows(const Product& p, int first, int span, uint
     }
 }
 
+// Workgroup ids go round the eight XCDs; each XCD gets a contiguous run of tiles, and a run walks
+// eight rows of tiles at a time, so that what an XCD's L2 holds is used by several of its CUs.
+struct Tile {
+    int m, n;
+};
+__device__ inline Tile tile_of(int id, int total, int m_tiles, int n_tiles) {
+    const int q = total >> 3, rem = total & 7, xcd = id & 7;
+    id = xcd * q + min(xcd, rem) + (id >> 3);
+    const int band = id / (8 * n_tiles), first = band * 8, high = min(m_tiles - first, 8);
+    id -= band * 8 * n_tiles;
+    return Tile{first + id % high, id / high};
+}
+
 // One 32 x 32 tile of y a workgroup; the waves deal the groups out among themselves and their sums meet
 // in LDS in a fixed order.  X is `void` for activations that are quantised already; otherwise the
 // workgroup first quantises the rows of x that its tile reaches, all groups of them, into LDS, so that
@@ -309,8 +322,8 @@ __global__ __launch_bounds__(WAVES * 64) void product_direct_kernel(Product p) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int r = lane & 31, half = lane >> 5;
     const int n_tiles = (p.n + 31) / 32;
-    const int m_tile = blockIdx.x / n_tiles;
-    const int n0 = (blockIdx.x - m_tile * n_tiles) * 32, m0 = m_tile * 32;
+    const Tile tile = tile_of(blockIdx.x, gridDim.x, (p.rows + 31) / 32, n_tiles);
+    const int n0 = tile.n * 32, m0 = tile.m * 32;
     const int n = min(n0 + r, p.n - 1), m = min(m0 + r, p.rows - 1);  // rows beyond the ends: computed, not stored
     const int rows = min(32, p.rows - m0);
     const int t = p.taps == 1 ? 0 : m % p.T;
@@ -421,19 +434,6 @@ __device__ inline void to_lds(const uint8_t* base, uint32_t offset, uint32_t dst
 }
 __device__ inline void to_lds(const uint8_t* src, uint32_t dst) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(dst), "v"(src) : "memory");
-}
-
-// Workgroup ids go round the eight XCDs; each XCD gets a contiguous run of tiles, and a run walks
-// eight rows of tiles at a time, so that what an XCD's L2 holds is used by several of its CUs.
-struct Tile {
-    int m, n;
-};
-__device__ inline Tile tile_of(int id, int total, int m_tiles, int n_tiles) {
-    const int q = total >> 3, rem = total & 7, xcd = id & 7;
-    id = xcd * q + min(xcd, rem) + (id >> 3);
-    const int band = id / (8 * n_tiles), first = band * 8, high = min(m_tiles - first, 8);
-    id -= band * 8 * n_tiles;
-    return Tile{first + id % high, id / high};
 }
 
 __device__ inline void dword_to_lds(const uint8_t* base, uint32_t offset, uint32_t dst) {
@@ -992,16 +992,20 @@ extern "C" int glv_mxfp4_product(const void* x_dev, const uint8_t* x_scales_dev,
     //   10560 x 2048 x 4096                71.9 (54.8)   71.6 (54.4)   77.5 (60.1)
     //    8192 x 8192 x 1024                73.0 (56.3)   62.1 (55.7)   78.9 (73.0)
     //    4096 x 4096 x 4096                49.3 (41.2)   47.2 (39.7)   45.3 (37.3)
-    // 32 x 32 spreads small outputs over the chip; 128 x 128 has three workgroups on a CU to hide each other's ends,
-    // but reads twice the LDS bytes of the larger tiles for a product, and where it follows a kernel bound by memory its
-    // draw makes the card lower its clock (10560 x 4096 x 1024: 38 us of zeros, 64 of random values; 41 and 47 for
-    // 128 x 256).  So sums of some length take 128 x 256, if it leaves no CU without work and does not reach much past
-    // w's rows, and so do shorter ones that it finishes in one round of two workgroups a CU.  Long sums take the
-    // largest where its rounds, of one workgroup a CU, are no longer than those of 128 x 256, half as much each.
-    if (all * n_out >= (int64_t)2 << 20) {
+    // 32 x 32 spreads small outputs over the chip, and takes about 3 us and 0.27 for a thousand tiles and groups; a
+    // workgroup of 128 x 128 alone on its CU 5 and 0.3 a group: the rule below fits where the two meet (2900
+    // tiles of 32 x 32 for one group, 1900 for five, 1300 for 25, 1140 for 68: 1203 x 1830 x 4429, 2204 tiles, 22.8 us
+    // against 16.0; 187 x 8779 x 655, 1650 tiles, 7.5 against 7.6; 1814 x 327 x 6961, 627 tiles, 13.2 against 19.8).
+    // 128 x 128 has three workgroups on a CU to hide each other's ends, but reads twice the LDS bytes of the larger
+    // tiles for a product, and where it follows a kernel bound by memory its draw makes the card lower its clock
+    // (10560 x 4096 x 1024: 38 us of zeros, 64 of random values; 41 and 47 for 128 x 256).  So sums of some length take
+    // 128 x 256, if it leaves no CU without work and does not reach much past w's rows, and so do shorter ones
+    // that it finishes in one round of two workgroups a CU.  Long sums take the largest where its rounds, of one
+    // workgroup a CU, are no longer than those of 128 x 256, half as much each.
+    const int64_t groups = (int64_t)p.taps * p.groups;
+    if ((tiles - 1050) * (2 * groups + 5) > 13000) {
         const int64_t rows128 = (all + 127) / 128, narrow = rows128 * ((n_out + 127) / 128), mid = rows128 * ((n_out + 255) / 256);
         const int64_t wide = ((all + 255) / 256) * ((n_out + 255) / 256);
-        const int groups = p.taps * p.groups;
         if (groups >= 32 && 2 * ((wide + 255) / 256) <= (mid + 255) / 256) return launch_tiled<256, 256>(p, st);
         if (32 * mid <= 17 * narrow && (groups >= 8 ? mid >= 256 : mid > 384 && mid <= 512)) return launch_tiled<128, 256>(p, st);
         return launch_tiled<128, 128>(p, st);
