@@ -67,20 +67,82 @@ struct Row {
 };
 
 // A lane holds V pieces of N columns: 16 bytes of a stream each, so that what the lanes of a row touch
-// at once is one run of memory.
-//
-// x <- Norm(x), zeros behind `cols`
+// at once is one run of memory.  A piece that reaches over the row's end is the row's last N columns instead,
+// of which the first are another lane's: its elements [lo, hi) count, and no value has to be moved into place (which
+// cost a tenth of the time at 1001 x 5000).
+// NARROW: rows of fewer than N columns.
+template <int N, bool NARROW>
+struct Piece {
+    int at, lo, hi;  // element i is column at + i
+
+    __device__ Piece(int col, int cols) {
+        if constexpr (NARROW)
+            at = 0, lo = col == 0 ? 0 : N, hi = cols;
+        else
+            at = min(col, cols - N), lo = min(col - at, N), hi = N;
+    }
+    __device__ bool whole() const { return lo == 0 && hi == N; }
+    template <typename T>
+    __device__ Pack<T, N> fetch(const T* row) const {
+        return fetch_pack<NARROW, N>(row, at, NARROW ? hi : at + N);
+    }
+    template <typename T>
+    __device__ void store(T* row, const Pack<T, N>& r) const {
+        if (whole()) {
+            store_pack(row + at, r, N);
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (i >= lo && i < hi) row[at + i] = r.v[i];
+    }
+    // zeros for what does not count
+    __device__ void mask(float (&x)[N]) const {
+        if (whole()) return;
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = i >= lo && i < hi ? x[i] : 0.f;
+    }
+};
+
+// Keeps a pack as it was loaded until here: the compiler would convert it to float at its load, and hold twice the
+// registers over all the sums (1001 x 5000 float16, the whole boundary: 13.8 us against 15.4).
+template <typename T, int N>
+__device__ inline void as_loaded(Pack<T, N>& r) {
+    if constexpr (sizeof(T) == 2) {
+        i32x4 w;
+        static_assert(sizeof(w) == sizeof(r));
+        __builtin_memcpy(&w, &r, sizeof(w));
+        asm volatile("" : "+v"(w));
+        __builtin_memcpy(&r, &w, sizeof(w));
+    }
+}
+
+// Whether what meets the row after its sums is under way while they are formed, or is read when they are done:
+// early, but for float32 rows of several waves, whose registers would leave a CU room for fewer rows (us, the whole
+// boundary, early against late: 1001 x 5000 26.2 and 18.2, 4000 x 9000 185 and 154; a wave a row, 55360 x 900, 189 and
+// 200), and for four eights a lane, whose would spill (8000 x 20000 float32: 1380 and 672).
+template <int LANES, int EIGHTS, int N>
+constexpr bool early() {
+    return EIGHTS <= 2 && (LANES > 0 || N == 8);
+}
+
+// x <- Norm(x)
 template <typename W, int LANES, int V, int N, bool NARROW>
 __device__ inline void normalise(float (&x)[V][N], int kind, const void* weight, const void* bias, float eps, int cols,
                                  const Row<LANES>& row, int use) {
     const float inv = 1.f / (float)cols;
+    auto piece = [&](int v) { return Piece<N, NARROW>((v * row.lanes + row.lane) * N, cols); };
+    constexpr bool kEarly = early<LANES, V * N / 8, N>();
     Pack<W, N> w[V], b[V];
+    auto fetch = [&](int v) {
+        if (weight) w[v] = piece(v).fetch(static_cast<const W*>(weight));
+        if (bias) b[v] = piece(v).fetch(static_cast<const W*>(bias));
+    };
+    if constexpr (kEarly)
 #pragma unroll
-    for (int v = 0; v < V; ++v) {  // under way while the sums are formed
-        const int col = (v * row.lanes + row.lane) * N;
-        if (weight) w[v] = fetch_pack<NARROW, N>(static_cast<const W*>(weight), col, cols);
-        if (bias) b[v] = fetch_pack<NARROW, N>(static_cast<const W*>(bias), col, cols);
-    }
+        for (int v = 0; v < V; ++v) fetch(v);
+#pragma unroll
+    for (int v = 0; v < V; ++v) piece(v).mask(x[v]);
     if (kind == GLV_NORM_LAYER) {
         float s = 0.f;
 #pragma unroll
@@ -89,10 +151,11 @@ __device__ inline void normalise(float (&x)[V][N], int kind, const void* weight,
             for (int i = 0; i < N; ++i) s += x[v][i];
         const float mean = row.sum(s, use) * inv;
 #pragma unroll
-        for (int v = 0; v < V; ++v)
+        for (int v = 0; v < V; ++v) {
 #pragma unroll
-            for (int i = 0; i < N; ++i)
-                x[v][i] = (v * row.lanes + row.lane) * N + i < cols ? x[v][i] - mean : 0.f;
+            for (int i = 0; i < N; ++i) x[v][i] -= mean;
+            piece(v).mask(x[v]);
+        }
     }
     float q = 0.f;
 #pragma unroll
@@ -102,9 +165,9 @@ __device__ inline void normalise(float (&x)[V][N], int kind, const void* weight,
     const float r = rsqrtf(row.sum(q, use + 1) * inv + eps);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        const int col = (v * row.lanes + row.lane) * N;
-        if (weight) w[v] = place_pack<NARROW>(w[v], col, cols);
-        if (bias) b[v] = place_pack<NARROW>(b[v], col, cols);
+        if constexpr (!kEarly) fetch(v);
+        if (weight) as_loaded(w[v]);
+        if (bias) as_loaded(b[v]);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             float t = x[v][i] * r;
@@ -130,32 +193,35 @@ __global__ __launch_bounds__(LANES > 0 ? 256 : 1024) void block_norm_kernel(Bloc
     const T* gate = p.gate ? static_cast<const T*>(p.gate) + b * p.gate_batch + t * p.gate_row : nullptr;
     const T* res = p.residual ? static_cast<const T*>(p.residual) + b * p.res_batch + t * p.res_row : nullptr;
     const int64_t out = (int64_t)at * p.cols;
-    const int cols = p.cols, store_cols = index < p.rows ? p.cols : 0;
+    const int cols = p.cols;
+    const bool stored = index < p.rows;
+    auto piece = [&](int v) { return Piece<N, NARROW>((v * row.lanes + row.lane) * N, cols); };
 
     Pack<T, N> ur[V], gr[V], rr[V];
+    constexpr bool kEarly = early<LANES, EIGHTS, N>();
+    auto fetch = [&](int v) {
+        if (gate && p.gate_col) gr[v] = piece(v).fetch(gate);
+        if (res) rr[v] = piece(v).fetch(res);
+    };
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        const int col = (v * row.lanes + row.lane) * N;
-        ur[v] = fetch_pack<NARROW, N>(u, col, cols);
-        if (gate && p.gate_col) gr[v] = fetch_pack<NARROW, N>(gate, col, cols);
-        if (res) rr[v] = fetch_pack<NARROW, N>(res, col, cols);
+        ur[v] = piece(v).fetch(u);
+        if constexpr (kEarly) fetch(v);
     }
     const float row_factor = p.scale * (gate && !p.gate_col ? (float)gate[0] : 1.f);
     float x[V][N];
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-        const Pack<T, N> placed = place_pack<NARROW>(ur[v], (v * row.lanes + row.lane) * N, cols);
+    for (int v = 0; v < V; ++v)
 #pragma unroll
-        for (int i = 0; i < N; ++i) x[v][i] = (float)placed.v[i];
-    }
+        for (int i = 0; i < N; ++i) x[v][i] = (float)ur[v].v[i];
     if (p.post) normalise<W, LANES, V, N, NARROW>(x, p.post, p.post_w, p.post_b, p.post_eps, cols, row, 0);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        const int col = (v * row.lanes + row.lane) * N;
+        if constexpr (!kEarly) fetch(v);
         Pack<W, N> sv;
-        if (p.scale_vec) sv = load_pack<NARROW, N>(static_cast<const W*>(p.scale_vec), col, cols);
-        if (gate && p.gate_col) gr[v] = place_pack<NARROW>(gr[v], col, cols);
-        if (res) rr[v] = place_pack<NARROW>(rr[v], col, cols);
+        if (p.scale_vec) sv = piece(v).fetch(static_cast<const W*>(p.scale_vec));
+        if (gate && p.gate_col) as_loaded(gr[v]);
+        if (res) as_loaded(rr[v]);
         Pack<T, N> o;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
@@ -163,32 +229,30 @@ __global__ __launch_bounds__(LANES > 0 ? 256 : 1024) void block_norm_kernel(Bloc
             if (gate && p.gate_col) k *= (float)gr[v].v[i];
             if (p.scale_vec) k *= (float)sv.v[i];
             if (res) k += (float)rr[v].v[i];
-            x[v][i] = col + i < cols ? k : 0.f;
+            x[v][i] = k;
             o.v[i] = (T)k;
         }
-        store_pack(static_cast<T*>(p.y) + out + col, o, store_cols - col);
+        if (stored) piece(v).store(static_cast<T*>(p.y) + out, o);
     }
     if (!p.pre) return;
     normalise<W, LANES, V, N, NARROW>(x, p.pre, p.pre_w, p.pre_b, p.pre_eps, cols, row, 2);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        const int col = (v * row.lanes + row.lane) * N;
         Pack<T, N> o;
 #pragma unroll
         for (int i = 0; i < N; ++i) o.v[i] = (T)x[v][i];
-        store_pack(static_cast<T*>(p.z) + out + col, o, store_cols - col);
+        if (stored) piece(v).store(static_cast<T*>(p.z) + out, o);
     }
 }
 
-// The fewest lanes that hold a row: 16 or 32 leave room for the other rows of a wave (32768 x 256 fp16,
-// the whole boundary: 25.5 us at 64 lanes, 19.2 at 32); beyond a wave as many waves as two eights a lane ask
-// for (1001 x 5000: 21.3 us with 256 threads of four eights, two fifths of them idle, 16.2 with 320 of two;
-// 4096 x 16384: 317 us with 1024 of four, half of them idle, 185 with 1024 of two), four where sixteen waves
-// would not do.
+// The fewest lanes that hold a row: 16 or 32 leave room for the other rows of a wave (us, the whole boundary in
+// float16: 32768 x 256 26.8 at 64 lanes, 19.0 at 32); beyond a wave as many waves as two eights a lane ask for (1001 x 3000
+// 8.8, with four eights 11.3; 4000 x 9000 94 and 113) up to twelve, of which a CU holds two workgroups (4000 x 12200 125
+// and 141), then four eights (4000 x 12400 137, with two 153).
 template <typename T, typename W>
 int launch(const BlockNorm& p, hipStream_t st) {
     const int pieces = (p.cols + 7) / 8;  // a lane holds one, two or four of them
-    const int threads = (pieces <= 2048 ? (pieces + 127) / 128 : (pieces + 255) / 256) * 64;  // of a workgroup to itself
+    const int threads = (pieces <= 1536 ? (pieces + 127) / 128 : (pieces + 255) / 256) * 64;  // of a workgroup to itself
     if (pieces > 128 && too_large(p.rows, threads)) return report(GLV_ERR_INVALID, "glv_block_norm: rows x columns too large for one call");
     auto rows_a_wave = [&](int lanes) { return dim3((unsigned)(((int64_t)p.rows * lanes + 255) / 256)); };
     if (p.cols < 16 / (int)sizeof(T))
@@ -201,7 +265,7 @@ int launch(const BlockNorm& p, hipStream_t st) {
         hipLaunchKernelGGL((block_norm_kernel<T, W, 64, 1>), rows_a_wave(64), dim3(256), 0, st, p);
     else if (pieces <= 128)
         hipLaunchKernelGGL((block_norm_kernel<T, W, 64, 2>), rows_a_wave(64), dim3(256), 0, st, p);
-    else if (pieces <= 2048)
+    else if (pieces <= 1536)
         hipLaunchKernelGGL((block_norm_kernel<T, W, 0, 2>), dim3(p.rows), dim3(threads), 0, st, p);
     else
         hipLaunchKernelGGL((block_norm_kernel<T, W, 0, 4>), dim3(p.rows), dim3(threads), 0, st, p);

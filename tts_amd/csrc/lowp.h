@@ -93,11 +93,6 @@ __device__ inline Pack<T, N> place_pack(const Pack<T, N>& v, int col, int cols) 
         return col + N <= cols ? v : moved_down(v, min(col - (cols - N), N));
     }
 }
-template <bool NARROW, int N, typename T>
-__device__ inline Pack<T, N> load_pack(const T* row, int col, int cols) {
-    return place_pack<NARROW>(fetch_pack<NARROW, N>(row, col, cols), col, cols);
-}
-
 template <typename T, int N>
 __device__ inline void store_pack(T* p, const Pack<T, N>& r, int valid) {
     if (valid >= N) {
