@@ -289,11 +289,37 @@ class Norm:
 
 def _norm_vector(t, name, cols, index, kind, seen, held):
     """(pointer, number of its type) of a weight, bias or scale; all of a call share one type."""
-    t, k = _vector(t, name, cols, index)
-    if (k != 0 and k != kind) or (seen is not None and seen != k):
+    k = _check(t, name, index)
+    if t.shape != (cols,):
+        raise ValueError(f"{name} must have shape ({cols},), got {tuple(t.shape)}")
+    if k != seen and (seen is not None or (k != 0 and k != kind)):
         raise ValueError(f"weights, biases and scale must all be float32 or all of u's type, got {t.dtype}")
-    held.append(t)
+    if t.stride(0) != 1 and cols != 1:
+        t = t.contiguous()
+        held.append(t)
     return t.data_ptr(), k
+
+
+def _broadcast(gate, shape, batch, rows, cols):
+    """(tensor, [batch, row and column stride]) of a gate that broadcasts to `shape`, u's, taken as (batch,
+    rows, cols)."""
+    g = gate
+    if len(shape) > 3:  # leading dimensions that a broadcast gate need not collapse like u's
+        try:
+            g = g.expand(shape)
+        except RuntimeError:
+            raise ValueError(f"gate of shape {tuple(gate.shape)} does not broadcast to {tuple(shape)}") from None
+        g = g.reshape(batch, rows, cols) if g.numel() else g.new_empty((batch, rows, cols))
+    full = (batch, rows, cols)[-len(shape):]
+    if g.dim() > len(full) or any(a != 1 and a != b for a, b in zip(reversed(g.shape), reversed(full))):
+        raise ValueError(f"gate of shape {tuple(gate.shape)} does not broadcast to {tuple(shape)}")
+    if g.dim() and g.shape[-1] != 1 and g.stride(-1) != 1:
+        g = g.contiguous()
+    strides = [0, 0, 0]
+    for i, (size, stride) in enumerate(zip(reversed(g.shape), reversed(g.stride()))):
+        if size != 1:
+            strides[2 - i] = stride
+    return g, strides
 
 
 def block_norm(u, *, post=None, gate=None, scale=None, residual=None, pre=None):
@@ -308,7 +334,7 @@ def block_norm(u, *, post=None, gate=None, scale=None, residual=None, pre=None):
     pre       `Norm` the next block starts with, or None
 
     Statistics are 32 bits; y enters `pre` before it is rounded to u's type.  C is at most 32768."""
-    kind, shape, index, dtype = _check(u, "u"), u.shape, u.get_device(), u.dtype
+    kind, shape, index = _check(u, "u"), u.shape, u.get_device()
     if len(shape) < 1 or shape[-1] < 1:
         raise ValueError(f"u must have a last dimension of at least 1, got {tuple(shape)}")
     if _current_device() != index:
@@ -317,15 +343,16 @@ def block_norm(u, *, post=None, gate=None, scale=None, residual=None, pre=None):
     cols = shape[-1]
     v, batch, rows, u_batch, u_row = _rows(u, shape)
     held, sides, vector_kind = [], [], None  # contiguous copies live until the launch
-    for side, norm in (("post", post), ("pre", pre)):
+    for norm, side, weight_name, bias_name in ((post, "post", "post.weight", "post.bias"),
+                                               (pre, "pre", "pre.weight", "pre.bias")):
         if norm is None:
             sides.append((0, None, None, 0.0))
         elif isinstance(norm, Norm):
             weight, bias = norm.weight, norm.bias
             if weight is not None:
-                weight, vector_kind = _norm_vector(weight, f"{side}.weight", cols, index, kind, vector_kind, held)
+                weight, vector_kind = _norm_vector(weight, weight_name, cols, index, kind, vector_kind, held)
             if bias is not None:
-                bias, vector_kind = _norm_vector(bias, f"{side}.bias", cols, index, kind, vector_kind, held)
+                bias, vector_kind = _norm_vector(bias, bias_name, cols, index, kind, vector_kind, held)
             sides.append((_NORMS[norm.kind], weight, bias, norm.eps))
         else:
             raise ValueError(f"{side} must be a Norm or None, got {type(norm).__name__}")
@@ -336,32 +363,19 @@ def block_norm(u, *, post=None, gate=None, scale=None, residual=None, pre=None):
         factor = float(scale)
     gate_ptr, gate_strides = None, (0, 0, 1)
     if gate is not None:
-        _check(gate, "gate", index)
-        if gate.dtype != dtype:
-            raise ValueError(f"gate must be {dtype} like u, got {gate.dtype}")
-        g = gate
-        if len(shape) > 3:  # leading dimensions that a broadcast gate need not collapse like u's
-            try:
-                g = g.expand(shape)
-            except RuntimeError:
-                raise ValueError(f"gate of shape {tuple(gate.shape)} does not broadcast to {tuple(shape)}") from None
-            g = g.reshape(batch, rows, cols) if g.numel() else g.new_empty((batch, rows, cols))
-        full = (batch, rows, cols)[-len(shape):]
-        if g.dim() > len(full) or any(a != 1 and a != b for a, b in zip(reversed(g.shape), reversed(full))):
-            raise ValueError(f"gate of shape {tuple(gate.shape)} does not broadcast to {tuple(shape)}")
-        if g.dim() and g.shape[-1] != 1 and g.stride(-1) != 1:
-            g = g.contiguous()
-        gate_strides = [0, 0, 0]
-        for i, (size, stride) in enumerate(zip(reversed(g.shape), reversed(g.stride()))):
-            if size != 1:
-                gate_strides[2 - i] = stride
+        if _check(gate, "gate", index) != kind:
+            raise ValueError(f"gate must be {u.dtype} like u, got {gate.dtype}")
+        if gate.shape == shape:
+            g, _, _, *gate_strides = _rows(gate, shape)
+            gate_strides.append(1)
+        else:
+            g, gate_strides = _broadcast(gate, shape, batch, rows, cols)
         gate_ptr = g.data_ptr()
         held.append(g)
     res_ptr, res_batch, res_row = None, 0, 0
     if residual is not None:
-        _check(residual, "residual", index)
-        if residual.dtype != dtype or residual.shape != shape:
-            raise ValueError(f"residual must be {dtype} {tuple(shape)} like u, got {residual.dtype} "
+        if _check(residual, "residual", index) != kind or residual.shape != shape:
+            raise ValueError(f"residual must be {u.dtype} {tuple(shape)} like u, got {residual.dtype} "
                              f"{tuple(residual.shape)}")
         r, _, _, res_batch, res_row = _rows(residual, shape)
         res_ptr = r.data_ptr()
