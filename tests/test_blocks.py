@@ -222,7 +222,8 @@ LARGE = [(512, 512, 1), (1000, 300, 129), (255, 2049, 385), (4100, 70, 640), (30
          (513, 6200, 100), (3100, 1100, 385), (12300, 257, 1001), (16500, 1030, 1100), (700, 8200, 1500), (260000, 9, 300),
          (33000, 129, 1), (40000, 200, 385), (32769, 256, 600), (16500, 1030, 4100), (100000, 70, 4200),
          (33000, 129, 1100), (50000, 250, 130), (12900, 1000, 1025), (8500, 1001, 4100), (4100, 2300, 4200),
-         (33000, 128, 384), (50001, 100, 131), (50001, 255, 257)]
+         (33000, 128, 384), (50001, 100, 131), (50001, 255, 257),
+         (3100, 1100, 300), (1000, 2000, 2900), (1250, 1500, 140)]
 
 
 @gpu
@@ -244,7 +245,7 @@ def test_linear_of_many_rows_and_columns(dtype, m, n, k):
     (2, 600, 300, 250, 2, 1), (64, 200, 256, 256, 3, 1), (3, 4100, 80, 300, 5, 2), (5000, 3, 130, 257, 4, 1), (130, 130, 60, 1030, 17, 20), (64, 700, 130, 200, 3, 2),
     (11000, 3, 40, 250, 4, 1), (130, 130, 60, 1030, 33, 3), (5500, 3, 100, 1000, 33, 1),
     (72, 700, 130, 200, 3, 2), (330, 100, 8, 80, 5, 7), (65, 505, 300, 128, 3, 1), (70, 705, 256, 250, 4, 5), (50001, 1, 384, 256, 1, 1),
-    (25001, 2, 40, 33, 7, 2), (11000, 3, 40, 250, 9, 1), (130, 65, 60, 1001, 33, 3), (3000, 3, 100, 1000, 33, 1)])
+    (25001, 2, 40, 33, 7, 2), (8, 500, 130, 515, 3, 1), (3, 1300, 100, 600, 5, 2), (5, 801, 260, 300, 3, 7), (11000, 3, 40, 250, 9, 1), (130, 65, 60, 1001, 33, 3), (3000, 3, 100, 1000, 33, 1)])
 def test_conv1d_of_many_rows(batch, time, c, n, taps, dilation):
     rng = np.random.default_rng(batch + time + c)
     x, w, bias = draw(rng, batch, time, c), draw(rng, n, taps, c, scale=(taps * c) ** -0.5), draw(rng, n)

@@ -393,6 +393,7 @@ __global__ __launch_bounds__(WAVES * 64) void product_direct_kernel(Product p) {
 // the product, large: tiles staged through LDS
 // ---------------------------------------------------------------------------
 // A workgroup's tile has TN rows of w and TM of x; a wave multiplies half of the w rows by 64 of x.
+// TEAMS: as many such sets of waves share the groups out, each with stages of its own, and add up at the end.
 // OWN (X is a float type): the workgroup quantises what its tile reaches of x into LDS before the first product.
 constexpr int kHeldUnits = 392;  // pairs of a row and a group: what three workgroups of 128 x 128 find room for
 template <int TM, int TN, bool OWN>
@@ -518,20 +519,23 @@ __device__ inline void arrive_and_wait() {  // all but the N youngest loads are 
 // r at place q ^ (r / 4 % 4): sixteen lanes that read one piece of sixteen rows then touch each of the
 // 64 banks once.  One stage is multiplied while the others are on their way.  A stage is two steps; the
 // barrier stands early in the second, whose products hide the first reads of the next stage.
-template <typename X, bool CONV, int TM, int TN>
-__global__ __launch_bounds__((Tiling<TM, TN, !std::is_void_v<X>>::kThreads), (Tiling<TM, TN, !std::is_void_v<X>>::kWavesPerSimd)) void product_tiled_kernel(Product p) {
+template <typename X, bool CONV, int TM, int TN, int TEAMS>
+__global__ __launch_bounds__((Tiling<TM, TN, !std::is_void_v<X>>::kThreads * TEAMS), (TEAMS > 1 ? 2 : Tiling<TM, TN, !std::is_void_v<X>>::kWavesPerSimd)) void product_tiled_kernel(Product p) {
     constexpr bool OWN = !std::is_void_v<X>;
     using L = Tiling<TM, TN, OWN>;
     constexpr int WT = L::kWt;
-    __shared__ __align__(1024) uint8_t lds[L::kBytes];
+    __shared__ __align__(1024) uint8_t lds[L::kBytes * TEAMS];
     __shared__ __align__(16) float bias[TN];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, id = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int team = TEAMS > 1 ? id / L::kWaves : 0, wave = id - team * L::kWaves;
     const int r = lane & 31, half = lane >> 5;
     const int m_tiles = (p.rows + TM - 1) / TM, n_tiles = (p.n + TN - 1) / TN;
     const Tile tile = tile_of(blockIdx.x, gridDim.x, m_tiles, n_tiles);
     const int n0 = tile.n * TN, m0 = tile.m * TM;
-    const int all = p.taps * p.groups;
-    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
+    // the team's groups: g0 .. g0 + all - 1
+    const int longest = (p.taps * p.groups + TEAMS - 1) / TEAMS, g0 = team * longest;
+    const int all = TEAMS > 1 ? min(longest, p.taps * p.groups - g0) : longest;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds + team * L::kBytes;
 
     // Load i of a wave fills 16 rows from (i * waves + wave) * 16 on, lane l the place l % 4 of row l / 4.
     // Rows behind the last repeat it.
@@ -562,13 +566,13 @@ __global__ __launch_bounds__((Tiling<TM, TN, !std::is_void_v<X>>::kThreads), (Ti
         }
     }
     // the next stage to be loaded: tap, group, and where their rows begin (counted in rows)
-    int tap = 0, gx = 0;
-    int64_t wrow = 0, xrow = 0;
+    int tap = TEAMS > 1 && CONV ? g0 / p.groups : 0, gx = g0 - tap * p.groups;
     const int64_t wstep = (int64_t)p.n * p.taps;
+    int64_t wrow = gx * wstep + tap, xrow = (int64_t)gx * p.rows;
     // first scale load of this wave: base, bytes to the current group, bytes of a group
     const uint8_t* sbase = first_w ? p.ws : p.xs;
     const int64_t sstep = (first_w ? wstep : p.rows) * 4;
-    int64_t sat = 0;
+    int64_t sat = gx * sstep;
     // the loads in order: w, x, scales; after the last one on to the next group; no branches
     auto stage_part = [&](int slot, auto part) {
         constexpr int i = part, xi = i - L::kLoadsW, si = xi - L::kLoadsX;
@@ -650,7 +654,8 @@ __global__ __launch_bounds__((Tiling<TM, TN, !std::is_void_v<X>>::kThreads), (Ti
     uint32_t at[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) at[k] = ((half * 2 + k) ^ ((r >> 2) & 3)) * 16;
-    const uint32_t wr = L::kW + (nw + r) * kGroupBytes, xr = L::kX + (mw + r) * kGroupBytes;
+    const uint32_t first_byte = team * L::kBytes;
+    const uint32_t wr = first_byte + L::kW + (nw + r) * kGroupBytes, xr = first_byte + L::kX + (mw + r) * kGroupBytes;
     // the reads of a step in the order of their use: w0 x0 w1 .. x1
     constexpr int kReads = WT + 2, kProducts = WT * 2;
     auto fetch = [&](uint32_t base, int k, auto q, Fragments<WT>& f) {
@@ -664,7 +669,7 @@ __global__ __launch_bounds__((Tiling<TM, TN, !std::is_void_v<X>>::kThreads), (Ti
             f.w[i] = v;
     };
     int ws[WT], xs[2], wnext[WT], xnext[2];
-    const uint32_t wsr = L::kWs + (nw + r) * 4, xsr = L::kXs + (mw + r) * 4;
+    const uint32_t wsr = first_byte + L::kWs + (nw + r) * 4, xsr = first_byte + L::kXs + (mw + r) * 4;
     auto fetch_scales = [&](uint32_t base) {
 #pragma unroll
         for (int i = 0; i < WT; ++i) wnext[i] = *reinterpret_cast<const int*>(lds + base + wsr + i * 128);
@@ -738,24 +743,45 @@ __global__ __launch_bounds__((Tiling<TM, TN, !std::is_void_v<X>>::kThreads), (Ti
     int c = 0;
     for (; c < all - L::kStages; ++c) chunk(std::true_type{});
     for (; c < all; ++c) chunk(std::false_type{});
+    if (TEAMS > 1 && all < longest) arrive_and_wait<0>();  // the other team's last barrier
 
     if (threadIdx.x < TN) bias[threadIdx.x] = own_bias;
     __syncthreads();
     // every read of the stages lies behind: each wave takes a part of them
     constexpr int kOwn = 32 * 32 * WT * 4;
     static_assert(L::kWaves * kOwn <= L::kBytes, "the stages (and x) hold the waves' parts of y");
-    uint8_t* own = lds + wave * kOwn;
+    uint8_t* own = lds + id * kOwn;
     // The smaller tiles, whose y is most of the traffic, store it past the L2 where its rows are whole lines
     // (us, 30000 x 1024 x 1000: 28.2 against 31.0 through the L2, 55360 x 256 x 768: 13.9 against 15.8; but rows of 1000,
     // which share lines: 35.3 against 32.3, and 28.6 against 17.6 for 30000 x 1000 x 128).  The largest leaves L2 to
     // the operands and y alike (8192 x 8192 x 1024: 66 past it, 62 through it).
     const int y_size = p.y_type == GLV_F32 ? 4 : 2;
     const bool stream = TM == 128 && ((reinterpret_cast<uintptr_t>(p.y) | (uintptr_t)p.n * y_size) & 127) == 0;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    // 32 rows of the wave's 64: of two teams each takes its half of both sums
+    auto finish = [&](auto J) {
+        constexpr int j = J;
         f32x16 part[WT];
 #pragma unroll
         for (int i = 0; i < WT; ++i) part[i] = acc[i][j];
+        if constexpr (TEAMS > 1) {
+            f32x4* const to = reinterpret_cast<f32x4*>(own);
+            const f32x4* const from = reinterpret_cast<const f32x4*>(lds + (id ^ L::kWaves) * kOwn);
+#pragma unroll
+            for (int i = 0; i < WT; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    to[(i * 4 + q) * 64 + lane] = f32x4{acc[i][1 - j][4 * q], acc[i][1 - j][4 * q + 1], acc[i][1 - j][4 * q + 2], acc[i][1 - j][4 * q + 3]};
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < WT; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const f32x4 v = from[(i * 4 + q) * 64 + lane];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) part[i][4 * q + e] += v[e];
+                }
+            __syncthreads();
+        }
         if (p.y_type == GLV_F32)
             store_rows<float>(p, stream, part, bias + nw, own, m0 + mw + j * 32, n0 + nw, lane);
         else if (p.y_type == GLV_BF16)
@@ -763,19 +789,21 @@ __global__ __launch_bounds__((Tiling<TM, TN, !std::is_void_v<X>>::kThreads), (Ti
         else
             store_rows<f16>(p, stream, part, bias + nw, own, m0 + mw + j * 32, n0 + nw, lane);
         wave_lds_fence();
-    }
+    };
+    if (TEAMS == 1 || team == 0) finish(std::integral_constant<int, 0>{});
+    if (TEAMS == 1 || team == 1) finish(std::integral_constant<int, 1>{});
 }
 
-template <int TM, int TN, typename X = void>
+template <int TM, int TN, int TEAMS = 1, typename X = void>
 int launch_tiled(const Product& p, hipStream_t st) {
     using L = Tiling<TM, TN, !std::is_void_v<X>>;
     const int64_t count = (int64_t)((p.rows + TM - 1) / TM) * ((p.n + TN - 1) / TN);
-    if (too_large(count, L::kThreads)) return report(GLV_ERR_INVALID, "glv_mxfp4_product: rows x n_out too large for one call");
+    if (too_large(count, L::kThreads * TEAMS)) return report(GLV_ERR_INVALID, "glv_mxfp4_product: rows x n_out too large for one call");
     const unsigned tiles = (unsigned)count;
     if (p.taps > 1)
-        hipLaunchKernelGGL((product_tiled_kernel<X, true, TM, TN>), dim3(tiles), dim3(L::kThreads), 0, st, p);
+        hipLaunchKernelGGL((product_tiled_kernel<X, true, TM, TN, TEAMS>), dim3(tiles), dim3(L::kThreads * TEAMS), 0, st, p);
     else
-        hipLaunchKernelGGL((product_tiled_kernel<X, false, TM, TN>), dim3(tiles), dim3(L::kThreads), 0, st, p);
+        hipLaunchKernelGGL((product_tiled_kernel<X, false, TM, TN, TEAMS>), dim3(tiles), dim3(L::kThreads * TEAMS), 0, st, p);
     return launch_status("product_tiled_kernel");
 }
 
@@ -960,8 +988,8 @@ extern "C" int glv_mxfp4_product(const void* x_dev, const uint8_t* x_scales_dev,
         p.x = x_dev, p.xr = Rows{x_batch_stride, x_row_stride, rows, batch == 1}, p.cols = cols;
         auto launch = [&](auto* typed) {
             using X = std::remove_pointer_t<decltype(typed)>;
-            if (tile == 256) return launch_tiled<128, 256, X>(p, st);
-            if (tile == 128) return launch_tiled<128, 128, X>(p, st);
+            if (tile == 256) return launch_tiled<128, 256, 1, X>(p, st);
+            if (tile == 128) return launch_tiled<128, 128, 1, X>(p, st);
             return launch_direct<X>(p, (unsigned)tiles, st);
         };
         if (x_type == GLV_F32) return launch((float*)nullptr);
@@ -980,8 +1008,8 @@ extern "C" int glv_mxfp4_product(const void* x_dev, const uint8_t* x_scales_dev,
     }
     // Which tile, measured in us with x and y in bfloat16, quantising x included (in brackets without it):
     //                            32 x 32    128 x 128     128 x 256     256 x 256   (rows of x times rows of w)
-    //    1000 x 1000 x 1024        (5.6)        (7.7)        (12.0)        (13.7)
-    //    2048 x 2048 x 4096       (36.8)   21.3 (14.6)   26.6 (20.2)   32.5 (25.9)
+    //    1000 x 1000 x 1024        (5.6)        (6.7)        (12.0)        (13.7)
+    //    2048 x 2048 x 4096       (36.8)   19.4 (12.9)   26.6 (20.2)   32.5 (25.9)
     //    2304 x 4096 x 4096                35.5 (28.3)   39.3 (32.2)   34.8 (28.1)
     //   16384 x  256 x 1024       (15.3)   15.1 ( 8.2)   17.4 (10.1)   19.7 (12.2)
     //   20000 x  512 x 1024                30.2 (11.1)   22.7 (12.7)   23.8 (14.3)
@@ -993,9 +1021,12 @@ extern "C" int glv_mxfp4_product(const void* x_dev, const uint8_t* x_scales_dev,
     //    8192 x 8192 x 1024                73.0 (56.3)   62.1 (55.7)   78.9 (73.0)
     //    4096 x 4096 x 4096                49.3 (41.2)   47.2 (39.7)   45.3 (37.3)
     // 32 x 32 spreads small outputs over the chip, and takes about 3 us and 0.27 for a thousand tiles and groups; a
-    // workgroup of 128 x 128 alone on its CU 5 and 0.3 a group: the rule below fits where the two meet (2900
-    // tiles of 32 x 32 for one group, 1900 for five, 1300 for 25, 1140 for 68: 1203 x 1830 x 4429, 2204 tiles, 22.8 us
-    // against 16.0; 187 x 8779 x 655, 1650 tiles, 7.5 against 7.6; 1814 x 327 x 6961, 627 tiles, 13.2 against 19.8).
+    // workgroup of 128 x 128 and two teams alone on its CU 5 and 0.2 a group: the rule below fits where the two meet
+    // (1700 tiles of 32 x 32 for two groups, 1300 for seven, 1100 for 19, 1000 for 64: 283 x 4812 x 2061, 1359 tiles,
+    // 9.8 us against 8.7; 960 tiles, 158 x 6144 x 1749, 6.8 against 7.6; 1163 x 1807 x 160, 2109 tiles, 6.6 against 6.1).
+    // Two teams a tile, while there is a CU for every tile: a wave a SIMD alone reaches half the rate (340 x 7567 x
+    // 5126, 180 tiles: 16.4 us against 19.2 with one team, 15164 x 151 x 490, 238 tiles, 6.9 against 7.6; 18227 x 187 x
+    // 1375, 286 tiles, 13.7 against 11.3).
     // 128 x 128 has three workgroups on a CU to hide each other's ends, but reads twice the LDS bytes of the larger
     // tiles for a product, and where it follows a kernel bound by memory its draw makes the card lower its clock
     // (10560 x 4096 x 1024: 38 us of zeros, 64 of random values; 41 and 47 for 128 x 256).  So sums of some length take
@@ -1003,11 +1034,12 @@ extern "C" int glv_mxfp4_product(const void* x_dev, const uint8_t* x_scales_dev,
     // that it finishes in one round of two workgroups a CU.  Long sums take the largest where its rounds, of one
     // workgroup a CU, are no longer than those of 128 x 256, half as much each.
     const int64_t groups = (int64_t)p.taps * p.groups;
-    if ((tiles - 1050) * (2 * groups + 5) > 13000) {
+    if ((tiles - 940) * (2 * groups + 5) > 6800) {
         const int64_t rows128 = (all + 127) / 128, narrow = rows128 * ((n_out + 127) / 128), mid = rows128 * ((n_out + 255) / 256);
         const int64_t wide = ((all + 255) / 256) * ((n_out + 255) / 256);
         if (groups >= 32 && 2 * ((wide + 255) / 256) <= (mid + 255) / 256) return launch_tiled<256, 256>(p, st);
         if (32 * mid <= 17 * narrow && (groups >= 8 ? mid >= 256 : mid > 384 && mid <= 512)) return launch_tiled<128, 256>(p, st);
+        if (narrow <= 256) return launch_tiled<128, 128, 2>(p, st);
         return launch_tiled<128, 128>(p, st);
     }
     return launch_direct<void>(p, (unsigned)tiles, st);
