@@ -168,6 +168,15 @@ def test_mxfp4_needs_a_gpu_and_leaves_the_state_dict_alone():
     assert model.use_mxfp4(False) is model
 
 
+def quantised(weights):
+    return FastSpeechAcousticModel(VOCAB).load_keras_weights(weights).cuda().use_mxfp4()
+
+
+def same_layers(model, other):
+    pairs = list(zip(model._mxfp4_layers(), other._mxfp4_layers(), strict=True))
+    return all(torch.equal(a.mxfp4_data, b.mxfp4_data) for a, b in pairs)
+
+
 @pytest.mark.gpu
 def test_mxfp4_blocks_against_the_oracle_and_back():
     from oracle import blocks_oracle as O
@@ -206,29 +215,28 @@ def test_mxfp4_blocks_against_the_oracle_and_back():
     assert mel.shape == plain.shape and torch.isfinite(mel).all() and not torch.equal(mel, plain)
     # loading weights quantises them anew
     other = random_weights(np.random.default_rng(8))
-    again = FastSpeechAcousticModel(VOCAB).load_keras_weights(other).cuda().use_mxfp4()((ids, durations))
-    assert torch.equal(model.load_keras_weights(other)((ids, durations)), again)
+    assert same_layers(model.load_keras_weights(other), quantised(other))
     model.load_state_dict(FastSpeechAcousticModel(VOCAB).load_keras_weights(w).state_dict())
-    assert torch.equal(model((ids, durations)), mel)
-    assert torch.equal(model.use_mxfp4(False)((ids, durations)), plain)
+    assert same_layers(model, quantised(w)) and not same_layers(model, quantised(other))
+    model.use_mxfp4(False)
+    assert all(layer.mxfp4_data is None for layer in model._mxfp4_layers())
+    # float32 is within 1e-4 of float64 (above), so two runs of it are within twice that of each other: the
+    # libraries behind it may choose another algorithm from call to call
+    assert (model((ids, durations)) - plain).norm() < 2e-4 * plain.norm()
 
 
 @pytest.mark.gpu
 def test_mxfp4_follows_the_weights_of_a_part_and_of_a_copy():
     import copy
-    ids = np.random.default_rng(10).integers(1, VOCAB, 20)[None]
-    durations = np.full(ids.shape, np.log(2.0), np.float32)
     w, other = random_weights(np.random.default_rng(11)), random_weights(np.random.default_rng(12))
-    model = FastSpeechAcousticModel(VOCAB).load_keras_weights(w).cuda().use_mxfp4()
+    model = quantised(w)
     want = FastSpeechAcousticModel(VOCAB).load_keras_weights(other)
     twin = copy.deepcopy(model)
-    first = model((ids, durations))
     for name, part in want.named_children():
         getattr(model, name).load_state_dict(part.state_dict())
-    assert torch.equal(model((ids, durations)), want.cuda().use_mxfp4()((ids, durations)))
-    assert torch.equal(twin((ids, durations)), first)
+    assert same_layers(model, quantised(other)) and same_layers(twin, quantised(w))
     torch.nn.ModuleList([twin]).load_state_dict({"0." + k: v for k, v in want.state_dict().items()})
-    assert torch.equal(twin((ids, durations)), want((ids, durations)))
+    assert same_layers(twin, model)
 
 
 @pytest.mark.gpu
