@@ -413,7 +413,9 @@ int glv_plan_drawn_phase(glv_plan* plan, uint64_t seed, int batch, int frames_st
  * with fixed weights, each followed by a norm).  They need no plan, allocate nothing and wait for
  * nothing; they run on the current device, on which every array must lie, and may be captured
  * into a graph.  Float arrays are of one of the types below and aligned to their elements; the
- * last dimension is contiguous, strides are counted in elements, outputs are contiguous.
+ * last dimension is contiguous, strides are counted in elements, outputs are contiguous.  Arguments
+ * come in a struct that is read before the call returns (a binding then fills one buffer: twenty and
+ * more arguments, each converted by itself, cost a Python caller 2 to 3 us).
  * Zero rows (or columns of output) are answered with GLV_OK before any pointer is looked at.
  */
 enum {
@@ -432,14 +434,19 @@ enum {
  *   codes_dev   (groups, rows, 64) bytes, the even column in the low half; 16-byte aligned
  *   scales_dev  (groups, rows, 4) bytes; 4-byte aligned
  * where rows counts batch * rows.  At most 2^24 rows and 2^18 columns.
- *   glv_mxfp4_quantize:   x_dev (batch, rows, cols), x[b, r, :] at b * batch_stride + r * row_stride.
- *   glv_mxfp4_dequantize: out_dev (rows, cols); exact in float32 and bfloat16, and in float16 wherever
- *                         that type can hold the value.
+ *   glv_mxfp4_quantize:   reads data_dev, data[b, r, :] at b * batch_stride + r * row_stride.
+ *   glv_mxfp4_dequantize: writes data_dev, contiguous (the strides are not used); exact in float32 and
+ *                         bfloat16, and in float16 wherever that type can hold the value.
  */
-int glv_mxfp4_quantize(const void* x_dev, int x_type, int batch, int rows, int cols, int64_t batch_stride,
-                       int64_t row_stride, uint8_t* codes_dev, uint8_t* scales_dev, void* stream);
-int glv_mxfp4_dequantize(const uint8_t* codes_dev, const uint8_t* scales_dev, int rows, int cols, int out_type,
-                         void* out_dev, void* stream);
+typedef struct glv_mxfp4_array {
+    void* data_dev; /* (batch, rows, cols) of `type`, a float type */
+    uint8_t* codes_dev;
+    uint8_t* scales_dev;
+    int64_t batch_stride, row_stride;
+    int type, batch, rows, cols;
+} glv_mxfp4_array;
+int glv_mxfp4_quantize(const glv_mxfp4_array* array, void* stream);
+int glv_mxfp4_dequantize(const glv_mxfp4_array* array, void* stream);
 
 /*
  * y[b, t, n] = act(sum_{j, c} q(x)[b, t + j * dilation - left, c] * w[n, j, c] + bias[n]),
@@ -456,12 +463,16 @@ int glv_mxfp4_dequantize(const uint8_t* codes_dev, const uint8_t* scales_dev, in
  * taps * cols and n_out are at most 2^18, n_out * taps and (taps - 1) * dilation at most 2^24.
  */
 enum { GLV_ACT_NONE = 0, GLV_ACT_RELU = 1 };
-int64_t glv_mxfp4_product_workspace(int x_type, int batch, int rows, int cols, int n_out, int taps, int dilation);
-int glv_mxfp4_product(const void* x_dev, const uint8_t* x_scales_dev, int x_type, int batch, int rows, int cols,
-                      int64_t x_batch_stride, int64_t x_row_stride, const uint8_t* w_codes_dev,
-                      const uint8_t* w_scales_dev, int n_out, int taps, int dilation, const void* bias_dev,
-                      int bias_type, int activation, void* y_dev, int y_type, void* workspace_dev,
-                      int64_t workspace_bytes, void* stream);
+typedef struct glv_mxfp4_product_args {
+    const void* x_dev;
+    const uint8_t *x_scales_dev, *w_codes_dev, *w_scales_dev;
+    const void* bias_dev;
+    void* y_dev;
+    int64_t x_batch_stride, x_row_stride;
+    int x_type, batch, rows, cols, n_out, taps, dilation, bias_type, activation, y_type;
+} glv_mxfp4_product_args;
+int64_t glv_mxfp4_product_workspace(const glv_mxfp4_product_args* args); /* looks at the sizes and x_type alone */
+int glv_mxfp4_product(const glv_mxfp4_product_args* args, void* workspace_dev, int64_t workspace_bytes, void* stream);
 
 /*
  * The end of a block and the start of the next, row by row:
@@ -479,13 +490,15 @@ int glv_mxfp4_product(const void* x_dev, const uint8_t* x_scales_dev, int x_type
  * At most 2^24 rows and 32768 columns.
  */
 enum { GLV_NORM_NONE = 0, GLV_NORM_LAYER = 1, GLV_NORM_RMS = 2 };
-int glv_block_norm(const void* u_dev, int type, int batch, int rows, int cols, int64_t u_batch_stride,
-                   int64_t u_row_stride, int vector_type, int post_kind, const void* post_weight_dev,
-                   const void* post_bias_dev, float post_eps, const void* gate_dev, int64_t gate_batch_stride,
-                   int64_t gate_row_stride, int gate_col_stride, const void* scale_dev, float scale,
-                   const void* residual_dev, int64_t residual_batch_stride, int64_t residual_row_stride,
-                   int pre_kind, const void* pre_weight_dev, const void* pre_bias_dev, float pre_eps, void* y_dev,
-                   void* z_dev, void* stream);
+typedef struct glv_block_norm_args {
+    const void *u_dev, *gate_dev, *residual_dev;
+    const void *post_weight_dev, *post_bias_dev, *scale_dev, *pre_weight_dev, *pre_bias_dev;
+    void *y_dev, *z_dev;
+    int64_t u_batch_stride, u_row_stride, gate_batch_stride, gate_row_stride, residual_batch_stride, residual_row_stride;
+    int type, batch, rows, cols, vector_type, post_kind, pre_kind, gate_col_stride;
+    float post_eps, pre_eps, scale;
+} glv_block_norm_args;
+int glv_block_norm(const glv_block_norm_args* args, void* stream);
 
 const char* glv_last_error(void);
 

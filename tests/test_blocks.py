@@ -1,7 +1,9 @@
 """The MXFP4 and block operators (tts_amd/blocks.py) against the float64 oracle, their refusals, and
 their use on other streams and in graphs."""
-import ctypes
 import itertools
+import os
+import struct
+import subprocess
 
 import numpy as np
 import pytest
@@ -402,10 +404,9 @@ def test_block_norm_in_place_of_each_input(dtype, rows, cols):
     for which in range(3):
         t = [u.clone(), gate.clone(), residual.clone()]
         z = torch.empty_like(u)
-        rc = _lib.load().glv_block_norm(
-            t[0].data_ptr(), TYPES.index(dtype), 1, rows, cols, 0, cols, 0, 1, None, None, 1e-5, t[1].data_ptr(), 0, cols, 1, None,
-            1.0, t[2].data_ptr(), 0, cols, 2, None, None, 1e-5, t[which].data_ptr(), z.data_ptr(),
-            torch.cuda.current_stream().cuda_stream)
+        args = _lib.block_norm_args(*(v.data_ptr() for v in t), 0, 0, 0, 0, 0, t[which].data_ptr(), z.data_ptr(), 0, cols, 0, cols,
+                                    0, cols, TYPES.index(dtype), 1, rows, cols, 0, 1, 2, 1, 1e-5, 1e-5, 1.0)
+        rc = _lib.load().glv_block_norm(args, torch.cuda.current_stream().cuda_stream)
         assert rc == 0 and torch.equal(t[which], want) and torch.equal(z, wantz)
 
 
@@ -623,60 +624,87 @@ def test_refusals_without_gpu():
         assert name in tts_amd.__all__
 
 
+def test_packed_arguments_are_the_headers_structs(tmp_path):
+    from tts_amd import _lib
+    # (struct, last field, its size) and the packed form with that field alone set
+    structs = [("glv_mxfp4_array", "cols", 4, _lib.mxfp4_array(*[0] * 8, 1)),
+               ("glv_mxfp4_product_args", "y_type", 4, _lib.mxfp4_product_args(*[0] * 17, 1)),
+               ("glv_block_norm_args", "scale", 4, _lib.block_norm_args(*[0] * 26, 1.0))]
+    source = "#include <stddef.h>\n#include \"glvoc.h\"\n"
+    for name, last, size, packed in structs:
+        at = next(i for i in range(0, len(packed), 4) if any(packed[i:i + 4]))
+        source += f"_Static_assert(sizeof({name}) == {len(packed)} && offsetof({name}, {last}) == {at}, \"{name}\");\n"
+    (tmp_path / "structs.c").write_text(source)
+    include = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include")
+    subprocess.run(["gcc", "-std=c11", "-fsyntax-only", "-I", include, str(tmp_path / "structs.c")], check=True)
+    with pytest.raises(struct.error):
+        _lib.mxfp4_array(0, 0, 0, 0, 0, 0, 1, 1 << 32, 1)
+
+
 def test_c_entries_validate_before_any_device_call():
     from tts_amd import _lib
     lib = _lib.load()
-    a, odd = ctypes.c_void_p(4096), ctypes.c_void_p(4097)  # never looked at: every call below is refused first
+    a, odd = 4096, 4097  # never looked at: every call below is refused first
 
     def quantize(x=a, kind=0, batch=1, rows=4, cols=32, codes=a, scales=a):
-        return lib.glv_mxfp4_quantize(x, kind, batch, rows, cols, rows * cols, cols, codes, scales, None)
+        return lib.glv_mxfp4_quantize(_lib.mxfp4_array(x or 0, codes or 0, scales or 0, rows * cols, cols, kind, batch, rows, cols), None)
 
     for kw in (dict(x=None), dict(codes=None), dict(scales=None), dict(kind=3), dict(kind=-1), dict(cols=0), dict(rows=-1),
                dict(batch=-1), dict(cols=1 << 19), dict(rows=(1 << 24) + 1), dict(batch=1 << 12, rows=1 << 13),
-               dict(codes=ctypes.c_void_p(4104)), dict(scales=ctypes.c_void_p(4098)), dict(x=odd)):
+               dict(codes=4104), dict(scales=4098), dict(x=odd)):
         assert quantize(**kw) == -1, kw
         assert b"glv_mxfp4_quantize" in lib.glv_last_error()
     assert quantize(rows=0) == 0 and quantize(batch=0, x=None, codes=None, scales=None) == 0
+
+    def dequantize(codes, scales, rows, cols, kind, out):
+        return lib.glv_mxfp4_dequantize(_lib.mxfp4_array(out or 0, codes or 0, scales or 0, 0, 0, kind, 1, rows, cols), None)
+
     for kw in ((None, a, 4, 32, 0, a), (a, None, 4, 32, 0, a), (a, a, 4, 32, 0, None), (a, a, 4, 32, 3, a), (a, a, -1, 32, 0, a),
-               (a, a, 4, 0, 0, a), (a, a, 4, 32, 0, odd), (ctypes.c_void_p(4104), a, 4, 32, 0, a)):
-        assert lib.glv_mxfp4_dequantize(*kw, None) == -1
-    assert lib.glv_mxfp4_dequantize(None, None, 0, 32, 0, None, None) == 0
+               (a, a, 4, 0, 0, a), (a, a, 4, 32, 0, odd), (4104, a, 4, 32, 0, a)):
+        assert dequantize(*kw) == -1
+    assert dequantize(None, None, 0, 32, 0, None) == 0
 
     def product(x=a, xs=None, kind=0, batch=1, rows=4, cols=32, wc=a, ws=a, n=8, taps=1, dilation=1, bias=None, bias_kind=0,
                 act=0, y=a, y_kind=0, work=a, size=1 << 20):
-        return lib.glv_mxfp4_product(x, xs, kind, batch, rows, cols, rows * cols, cols, wc, ws, n, taps, dilation, bias,
-                                     bias_kind, act, y, y_kind, work, size, None)
+        args = _lib.mxfp4_product_args(x or 0, xs or 0, wc or 0, ws or 0, bias or 0, y or 0, rows * cols, cols, kind, batch, rows, cols,
+                                       n, taps, dilation, bias_kind, act, y_kind)
+        return lib.glv_mxfp4_product(args, work, size, None)
 
     for kw in (dict(x=None), dict(wc=None), dict(ws=None), dict(y=None), dict(rows=64, cols=4096, work=None), dict(rows=64, cols=4096, size=8),
                dict(kind=4),
                dict(kind=3), dict(y_kind=3), dict(act=2), dict(taps=0), dict(dilation=0), dict(n=-1), dict(cols=0), dict(rows=-1),
                dict(taps=1 << 14), dict(taps=2, dilation=(1 << 24) + 1), dict(n=(1 << 18) + 1), dict(y=odd), dict(bias=odd), dict(x=odd),
-               dict(bias=a, bias_kind=3), dict(wc=ctypes.c_void_p(4104)),
-               dict(rows=64, cols=4096, work=ctypes.c_void_p(4104)),
-               dict(kind=3, xs=a, x=ctypes.c_void_p(4104)), dict(taps=128, n=1 << 18)):
+               dict(bias=a, bias_kind=3), dict(wc=4104),
+               dict(rows=64, cols=4096, work=4104),
+               dict(kind=3, xs=a, x=4104), dict(taps=128, n=1 << 18)):
         assert product(**kw) == -1, kw
         assert b"glv_mxfp4_product" in lib.glv_last_error()
     assert product(rows=0, x=None, y=None, work=None) == 0 and product(n=0, wc=None) == 0
-    size = lib.glv_mxfp4_product_workspace
+    assert lib.glv_mxfp4_product(None, None, 0, None) == lib.glv_mxfp4_quantize(None, None) == lib.glv_block_norm(None, None) == -1
+
+    def size(*shape):
+        return lib.glv_mxfp4_product_workspace(_lib.mxfp4_product_args(0, 0, 0, 0, 0, 0, 0, 0, *shape, 0, 0, 0))
+
     assert size(0, 1, 64, 4096, 8, 1, 1) > 0 and size(3, 1, 64, 4096, 8, 1, 1) == 0
     assert size(9, 1, 4, 32, 8, 1, 1) == -1 and size(0, 1, 4, 0, 8, 1, 1) == -1 and size(0, 1 << 13, 1 << 13, 32, 8, 1, 1) == -1
     assert size(0, 1, 4, 32, 8, 1, 0) == -1 and size(0, 1, 4, 32, 8, 0, 1) == -1
 
     def norm(u=a, kind=0, batch=1, rows=4, cols=32, vkind=0, post=1, pw=None, eps=1e-5, gate=None, gate_col=1, scale=None, res=None,
              pre=0, y=a, z=None):
-        return lib.glv_block_norm(u, kind, batch, rows, cols, rows * cols, cols, vkind, post, pw, None, eps, gate, 0, 0, gate_col,
-                                  scale, 1.0, res, 0, 0, pre, None, None, eps, y, z, None)
+        return lib.glv_block_norm(_lib.block_norm_args(
+            u or 0, gate or 0, res or 0, pw or 0, 0, scale or 0, 0, 0, y or 0, z or 0, rows * cols, cols, 0, 0, 0, 0, kind, batch, rows,
+            cols, vkind, post, pre, gate_col, eps, eps, 1.0), None)
 
     for kw in (dict(u=None), dict(y=None), dict(pre=2), dict(kind=3), dict(vkind=1), dict(post=3), dict(pre=-1), dict(eps=-1.0),
                dict(eps=float("nan")), dict(gate_col=2), dict(cols=0), dict(cols=32769), dict(rows=-1), dict(batch=1 << 13, rows=1 << 13),
-               dict(u=odd), dict(gate=odd), dict(res=odd), dict(pw=ctypes.c_void_p(4098)), dict(scale=odd)):
+               dict(u=odd), dict(gate=odd), dict(res=odd), dict(pw=4098), dict(scale=odd)):
         assert norm(**kw) == -1, kw
         assert b"glv_block_norm" in lib.glv_last_error()
     assert norm(rows=0, u=None, y=None) == 0
 
     # more threads than one launch can hold
     kw = dict(rows=1 << 24, cols=32768)
-    assert quantize(**kw) == norm(**kw) == lib.glv_mxfp4_dequantize(a, a, kw["rows"], kw["cols"], 0, a, None) == -1
+    assert quantize(**kw) == norm(**kw) == dequantize(a, a, kw["rows"], kw["cols"], 0, a) == -1
     assert b"too large for one call" in lib.glv_last_error()
     for n in (1 << 16, 1 << 18):
         assert product(kind=3, xs=a, rows=1 << 24, n=n) == -1 and b"too large for one call" in lib.glv_last_error()

@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # GLVOC_LIB selects another build of the same library (kernel tuning experiments)
@@ -88,25 +89,20 @@ SIGNATURES = {
     "glv_shard_last_run_form": (ctypes.c_int, [ctypes.c_void_p]),
     "glv_plan_drawn_phase": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_uint64, ctypes.c_int, ctypes.c_int,
                                             ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p]),
-    "glv_mxfp4_quantize": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int,
-                                          ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p,
-                                          ctypes.c_void_p]),
-    "glv_mxfp4_dequantize": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_int,
-                                            ctypes.c_void_p, ctypes.c_void_p]),
-    "glv_mxfp4_product_workspace": (ctypes.c_int64, [ctypes.c_int] * 7),
-    "glv_mxfp4_product": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_int,
-                                         ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p,
-                                         ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
-                                         ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p,
-                                         ctypes.c_int64, ctypes.c_void_p]),
-    "glv_block_norm": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int,
-                                      ctypes.c_int64, ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
-                                      ctypes.c_void_p, ctypes.c_float, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64,
-                                      ctypes.c_int, ctypes.c_void_p, ctypes.c_float, ctypes.c_void_p, ctypes.c_int64,
-                                      ctypes.c_int64, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_float,
-                                      ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
+    "glv_mxfp4_quantize": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_void_p]),
+    "glv_mxfp4_dequantize": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_void_p]),
+    "glv_mxfp4_product_workspace": (ctypes.c_int64, [ctypes.c_char_p]),
+    "glv_mxfp4_product": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]),
+    "glv_block_norm": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_void_p]),
     "glv_last_error": (ctypes.c_char_p, []),
 }
+
+
+# The argument structs of glvoc.h, packed: one buffer costs a call less than twenty converted arguments, and a
+# value that does not fit its field is an error.
+mxfp4_array = struct.Struct("3P2q4i").pack
+mxfp4_product_args = struct.Struct("6P2q10i").pack
+block_norm_args = struct.Struct("10P6q8i3f4x").pack
 
 
 class GlvError(RuntimeError):

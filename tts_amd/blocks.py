@@ -143,8 +143,8 @@ class MXFP4Tensor:
                 return self.dequantize(dtype)
         out = data.new_empty(shape, dtype=dtype)
         codes, scales = self._pointers()
-        rc = _lib.load().glv_mxfp4_dequantize(codes, scales, self.rows, shape[-1], kind, out.data_ptr(),
-                                              _current_stream(index))
+        array = _lib.mxfp4_array(out.data_ptr(), codes, scales, 0, 0, kind, 1, self.rows, shape[-1])
+        rc = _lib.load().glv_mxfp4_dequantize(array, _current_stream(index))
         if rc:
             _lib.check(rc)
         return out
@@ -171,8 +171,8 @@ def mxfp4_quantize(x):
     q.shape, q.rows, q.groups = shape, batch * rows, -(-cols // _GROUP)
     q.data = x.new_empty(q.rows * q.groups * 68, dtype=torch.uint8)
     codes, scales = q._pointers()
-    rc = _lib.load().glv_mxfp4_quantize(v.data_ptr(), kind, batch, rows, cols, batch_stride, row_stride, codes, scales,
-                                        _current_stream(index))
+    array = _lib.mxfp4_array(v.data_ptr(), codes, scales, batch_stride, row_stride, kind, batch, rows, cols)
+    rc = _lib.load().glv_mxfp4_quantize(array, _current_stream(index))
     if rc:
         _lib.check(rc)
     return q
@@ -187,7 +187,7 @@ def _product(x, weight, bias, taps, dilation, activation, out_dtype):
     if _current_device() != index:
         with torch.cuda.device(index):
             return _product(x, weight, bias, taps, dilation, activation, out_dtype)
-    scales, batch_stride, row_stride = None, 0, 0
+    scales, batch_stride, row_stride = 0, 0, 0
     if isinstance(x, MXFP4Tensor):
         like, shape = x.data, x.shape
         if like.get_device() < 0:
@@ -203,7 +203,7 @@ def _product(x, weight, bias, taps, dilation, activation, out_dtype):
             raise ValueError("x must have at least one dimension")
     if shape[-1] != cols:
         raise ValueError(f"x has {shape[-1]} columns but the weight {cols}")
-    if scales is None:
+    if kind != _MXFP4:
         like, batch, rows, batch_stride, row_stride = _rows(x, shape)
         data = like.data_ptr()
     if taps == 1 and batch != 1 and batch_stride == rows * row_stride and batch * rows <= _INT:
@@ -214,21 +214,20 @@ def _product(x, weight, bias, taps, dilation, activation, out_dtype):
         out_kind = _TYPES.get(out_dtype)
         if out_kind is None:
             raise ValueError(f"out_dtype must be float32, bfloat16 or float16, got {out_dtype}")
-    bias_ptr, bias_kind = None, 0
+    bias_ptr, bias_kind = 0, 0
     if bias is not None:
         bias, bias_kind = _vector(bias, "bias", n, index)
         bias_ptr = bias.data_ptr()
     lib = _lib.load()
     y = like.new_empty((*shape[:-1], n), dtype=out_dtype)
-    need = lib.glv_mxfp4_product_workspace(kind, batch, rows, cols, n, taps, dilation)
+    args = _lib.mxfp4_product_args(data, scales, *weight._pointers(), bias_ptr, y.data_ptr(), batch_stride, row_stride, kind,
+                                   batch, rows, cols, n, taps, dilation, bias_kind, act, out_kind)
+    need = lib.glv_mxfp4_product_workspace(args)
     work_ptr = None
     if need > 0:
         work = like.new_empty(need, dtype=torch.uint8)
         work_ptr = work.data_ptr()
-    w_codes, w_scales = weight._pointers()
-    rc = lib.glv_mxfp4_product(data, scales, kind, batch, rows, cols, batch_stride, row_stride, w_codes, w_scales, n, taps,
-                               dilation, bias_ptr, bias_kind, act, y.data_ptr(), out_kind, work_ptr,
-                               need if need > 0 else 0, _current_stream(index))
+    rc = lib.glv_mxfp4_product(args, work_ptr, need, _current_stream(index))
     if rc:
         _lib.check(rc)
     return y
@@ -346,22 +345,22 @@ def block_norm(u, *, post=None, gate=None, scale=None, residual=None, pre=None):
     for norm, side, weight_name, bias_name in ((post, "post", "post.weight", "post.bias"),
                                                (pre, "pre", "pre.weight", "pre.bias")):
         if norm is None:
-            sides.append((0, None, None, 0.0))
+            sides.append((0, 0, 0, 0.0))
         elif isinstance(norm, Norm):
-            weight, bias = norm.weight, norm.bias
-            if weight is not None:
-                weight, vector_kind = _norm_vector(weight, weight_name, cols, index, kind, vector_kind, held)
-            if bias is not None:
-                bias, vector_kind = _norm_vector(bias, bias_name, cols, index, kind, vector_kind, held)
+            weight = bias = 0
+            if norm.weight is not None:
+                weight, vector_kind = _norm_vector(norm.weight, weight_name, cols, index, kind, vector_kind, held)
+            if norm.bias is not None:
+                bias, vector_kind = _norm_vector(norm.bias, bias_name, cols, index, kind, vector_kind, held)
             sides.append((_NORMS[norm.kind], weight, bias, norm.eps))
         else:
             raise ValueError(f"{side} must be a Norm or None, got {type(norm).__name__}")
-    scale_ptr, factor = None, 1.0
+    scale_ptr, factor = 0, 1.0
     if isinstance(scale, torch.Tensor):
         scale_ptr, vector_kind = _norm_vector(scale, "scale", cols, index, kind, vector_kind, held)
     elif scale is not None:
         factor = float(scale)
-    gate_ptr, gate_strides = None, (0, 0, 1)
+    gate_ptr, gate_strides = 0, (0, 0, 1)
     if gate is not None:
         if _check(gate, "gate", index) != kind:
             raise ValueError(f"gate must be {u.dtype} like u, got {gate.dtype}")
@@ -372,7 +371,7 @@ def block_norm(u, *, post=None, gate=None, scale=None, residual=None, pre=None):
             g, gate_strides = _broadcast(gate, shape, batch, rows, cols)
         gate_ptr = g.data_ptr()
         held.append(g)
-    res_ptr, res_batch, res_row = None, 0, 0
+    res_ptr, res_batch, res_row = 0, 0, 0
     if residual is not None:
         if _check(residual, "residual", index) != kind or residual.shape != shape:
             raise ValueError(f"residual must be {u.dtype} {tuple(shape)} like u, got {residual.dtype} "
@@ -384,10 +383,11 @@ def block_norm(u, *, post=None, gate=None, scale=None, residual=None, pre=None):
     z = v.new_empty(shape) if pre is not None else None
     post_kind, post_w, post_b, post_eps = sides[0]
     pre_kind, pre_w, pre_b, pre_eps = sides[1]
-    rc = _lib.load().glv_block_norm(v.data_ptr(), kind, batch, rows, cols, u_batch, u_row, vector_kind or 0, post_kind,
-                                    post_w, post_b, post_eps, gate_ptr, gate_strides[0], gate_strides[1], gate_strides[2],
-                                    scale_ptr, factor, res_ptr, res_batch, res_row, pre_kind, pre_w, pre_b, pre_eps,
-                                    y.data_ptr(), None if z is None else z.data_ptr(), _current_stream(index))
+    args = _lib.block_norm_args(v.data_ptr(), gate_ptr, res_ptr, post_w, post_b, scale_ptr, pre_w, pre_b, y.data_ptr(),
+                                0 if z is None else z.data_ptr(), u_batch, u_row, gate_strides[0], gate_strides[1],
+                                res_batch, res_row, kind, batch, rows, cols, vector_kind or 0, post_kind, pre_kind,
+                                gate_strides[2], post_eps, pre_eps, factor)
+    rc = _lib.load().glv_block_norm(args, _current_stream(index))
     if rc:
         _lib.check(rc)
     return y if z is None else (y, z)

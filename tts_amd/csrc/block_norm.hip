@@ -280,14 +280,12 @@ bool norm_kind(int k) { return k == GLV_NORM_NONE || k == GLV_NORM_LAYER || k ==
 
 }  // namespace
 
-extern "C" int glv_block_norm(const void* u_dev, int type, int batch, int rows, int cols, int64_t u_batch_stride,
-                              int64_t u_row_stride, int vector_type, int post_kind, const void* post_weight_dev,
-                              const void* post_bias_dev, float post_eps, const void* gate_dev, int64_t gate_batch_stride,
-                              int64_t gate_row_stride, int gate_col_stride, const void* scale_dev, float scale,
-                              const void* residual_dev, int64_t residual_batch_stride, int64_t residual_row_stride,
-                              int pre_kind, const void* pre_weight_dev, const void* pre_bias_dev, float pre_eps, void* y_dev,
-                              void* z_dev, void* stream) {
+extern "C" int glv_block_norm(const glv_block_norm_args* a, void* stream) {
     const char* what = "glv_block_norm";
+    if (!a) return report(GLV_ERR_INVALID, "%s: null argument", what);
+    const auto [u_dev, gate_dev, residual_dev, post_weight_dev, post_bias_dev, scale_dev, pre_weight_dev, pre_bias_dev, y_dev, z_dev,
+                u_batch_stride, u_row_stride, gate_batch_stride, gate_row_stride, residual_batch_stride, residual_row_stride, type, batch,
+                rows, cols, vector_type, post_kind, pre_kind, gate_col_stride, post_eps, pre_eps, scale] = *a;
     if (batch < 0 || rows < 0 || (int64_t)batch * rows > kMaxRows)
         return report(GLV_ERR_INVALID, "%s: %d x %d rows outside [0, %lld]", what, batch, rows, (long long)kMaxRows);
     if (cols < 1 || cols > kMaxCols) return report(GLV_ERR_INVALID, "%s: cols %d outside [1, %d]", what, cols, kMaxCols);

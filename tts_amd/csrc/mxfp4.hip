@@ -894,34 +894,37 @@ int64_t quantised_bytes(int64_t rows, int64_t groups) { return rows * groups * (
 
 }  // namespace
 
-extern "C" int glv_mxfp4_quantize(const void* x_dev, int x_type, int batch, int rows, int cols, int64_t batch_stride,
-                                  int64_t row_stride, uint8_t* codes_dev, uint8_t* scales_dev, void* stream) {
-    const char* what = "glv_mxfp4_quantize";
-    if (batch < 0 || rows < 0) return report(GLV_ERR_INVALID, "%s: negative batch or rows", what);
-    const int64_t all = (int64_t)batch * rows;
-    int rc = check_shape(what, all, cols);
+// What both directions ask of an array; GLV_OK with *all = 0: nothing to do.
+static int check_array(const char* what, const glv_mxfp4_array* a, int64_t* all) {
+    if (!a) return report(GLV_ERR_INVALID, "%s: null argument", what);
+    if (a->batch < 0 || a->rows < 0) return report(GLV_ERR_INVALID, "%s: negative batch or rows", what);
+    *all = (int64_t)a->batch * a->rows;
+    const int rc = check_shape(what, *all, a->cols);
     if (rc != GLV_OK) return rc;
-    if (!float_type(x_type)) return report(GLV_ERR_INVALID, "%s: unknown element type %d", what, x_type);
-    if (all == 0) return GLV_OK;
-    if (!x_dev || !codes_dev || !scales_dev) return report(GLV_ERR_INVALID, "%s: null argument", what);
-    if (misaligned(x_dev, x_type == GLV_F32 ? 4 : 2)) return report(GLV_ERR_INVALID, "%s: x is not aligned to its elements", what);
-    rc = check_quantised(what, codes_dev, scales_dev);
-    if (rc != GLV_OK) return rc;
-    return quantise(what, x_dev, x_type, Rows{batch_stride, row_stride, rows, batch == 1}, (int)all, cols, codes_dev, scales_dev,
-                    (hipStream_t)stream);
+    if (!float_type(a->type)) return report(GLV_ERR_INVALID, "%s: unknown element type %d", what, a->type);
+    if (*all == 0) return GLV_OK;
+    if (!a->data_dev || !a->codes_dev || !a->scales_dev) return report(GLV_ERR_INVALID, "%s: null argument", what);
+    if (misaligned(a->data_dev, a->type == GLV_F32 ? 4 : 2)) return report(GLV_ERR_INVALID, "%s: data is not aligned to its elements", what);
+    return check_quantised(what, a->codes_dev, a->scales_dev);
 }
 
-extern "C" int glv_mxfp4_dequantize(const uint8_t* codes_dev, const uint8_t* scales_dev, int rows, int cols, int out_type,
-                                    void* out_dev, void* stream) {
+extern "C" int glv_mxfp4_quantize(const glv_mxfp4_array* a, void* stream) {
+    const char* what = "glv_mxfp4_quantize";
+    int64_t all = 0;
+    const int rc = check_array(what, a, &all);
+    if (rc != GLV_OK || all == 0) return rc;
+    return quantise(what, a->data_dev, a->type, Rows{a->batch_stride, a->row_stride, a->rows, a->batch == 1}, (int)all, a->cols,
+                    a->codes_dev, a->scales_dev, (hipStream_t)stream);
+}
+
+extern "C" int glv_mxfp4_dequantize(const glv_mxfp4_array* a, void* stream) {
     const char* what = "glv_mxfp4_dequantize";
-    int rc = check_shape(what, rows, cols);
-    if (rc != GLV_OK) return rc;
-    if (!float_type(out_type)) return report(GLV_ERR_INVALID, "%s: unknown element type %d", what, out_type);
-    if (rows == 0) return GLV_OK;
-    if (!codes_dev || !scales_dev || !out_dev) return report(GLV_ERR_INVALID, "%s: null argument", what);
-    if (misaligned(out_dev, out_type == GLV_F32 ? 4 : 2)) return report(GLV_ERR_INVALID, "%s: out is not aligned to its elements", what);
-    rc = check_quantised(what, codes_dev, scales_dev);
-    if (rc != GLV_OK) return rc;
+    int64_t all = 0;
+    const int rc = check_array(what, a, &all);
+    if (rc != GLV_OK || all == 0) return rc;
+    const int rows = (int)all, cols = a->cols, out_type = a->type;
+    const uint8_t *codes_dev = a->codes_dev, *scales_dev = a->scales_dev;
+    void* out_dev = a->data_dev;
     const int groups = (cols + kGroup - 1) / kGroup;
     const int64_t blocks = span_blocks(rows, groups);
     if (too_large(blocks, 256)) return report(GLV_ERR_INVALID, "%s: rows x columns too large for one call", what);
@@ -936,19 +939,19 @@ extern "C" int glv_mxfp4_dequantize(const uint8_t* codes_dev, const uint8_t* sca
     return launch_status("dequantise_kernel");
 }
 
-extern "C" int64_t glv_mxfp4_product_workspace(int x_type, int batch, int rows, int cols, int n_out, int taps, int dilation) {
-    if (batch < 0 || rows < 0 || n_out < 0 || taps < 1 || dilation < 1 || cols < 1 || cols > kMaxCols) return -1;
-    if ((int64_t)batch * rows > kMaxRows || !(float_type(x_type) || x_type == GLV_MXFP4)) return -1;
-    if (x_type == GLV_MXFP4 || own_tile((int64_t)batch * rows, cols, n_out, taps, dilation)) return 0;
-    return quantised_bytes((int64_t)batch * rows, (cols + kGroup - 1) / kGroup);
+extern "C" int64_t glv_mxfp4_product_workspace(const glv_mxfp4_product_args* a) {
+    if (!a || a->batch < 0 || a->rows < 0 || a->n_out < 0 || a->taps < 1 || a->dilation < 1 || a->cols < 1 || a->cols > kMaxCols) return -1;
+    const int64_t all = (int64_t)a->batch * a->rows;
+    if (all > kMaxRows || !(float_type(a->x_type) || a->x_type == GLV_MXFP4)) return -1;
+    if (a->x_type == GLV_MXFP4 || own_tile(all, a->cols, a->n_out, a->taps, a->dilation)) return 0;
+    return quantised_bytes(all, (a->cols + kGroup - 1) / kGroup);
 }
 
-extern "C" int glv_mxfp4_product(const void* x_dev, const uint8_t* x_scales_dev, int x_type, int batch, int rows, int cols,
-                                 int64_t x_batch_stride, int64_t x_row_stride, const uint8_t* w_codes_dev,
-                                 const uint8_t* w_scales_dev, int n_out, int taps, int dilation, const void* bias_dev,
-                                 int bias_type, int activation, void* y_dev, int y_type, void* workspace_dev,
-                                 int64_t workspace_bytes, void* stream) {
+extern "C" int glv_mxfp4_product(const glv_mxfp4_product_args* a, void* workspace_dev, int64_t workspace_bytes, void* stream) {
     const char* what = "glv_mxfp4_product";
+    if (!a) return report(GLV_ERR_INVALID, "%s: null argument", what);
+    const auto [x_dev, x_scales_dev, w_codes_dev, w_scales_dev, bias_dev, y_dev, x_batch_stride, x_row_stride, x_type, batch, rows, cols,
+                n_out, taps, dilation, bias_type, activation, y_type] = *a;
     if (batch < 0 || rows < 0) return report(GLV_ERR_INVALID, "%s: negative batch or rows", what);
     const int64_t all = (int64_t)batch * rows;
     int rc = check_shape(what, all, cols);
