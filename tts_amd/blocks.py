@@ -219,7 +219,8 @@ def _product(x, weight, bias, taps, dilation, activation, out_dtype):
         bias, bias_kind = _vector(bias, "bias", n, index)
         bias_ptr = bias.data_ptr()
     lib = _lib.load()
-    y = like.new_empty((*shape[:-1], n), dtype=out_dtype)
+    shape = (*shape[:-1], n)
+    y = like.new_empty(shape) if out_kind == kind else like.new_empty(shape, dtype=out_dtype)
     args = _lib.mxfp4_product_args(data, scales, *weight._pointers(), bias_ptr, y.data_ptr(), batch_stride, row_stride, kind,
                                    batch, rows, cols, n, taps, dilation, bias_kind, act, out_kind)
     need = lib.glv_mxfp4_product_workspace(args)
@@ -379,8 +380,12 @@ def block_norm(u, *, post=None, gate=None, scale=None, residual=None, pre=None):
         r, _, _, res_batch, res_row = _rows(residual, shape)
         res_ptr = r.data_ptr()
         held.append(r)
-    y = v.new_empty(shape)
-    z = v.new_empty(shape) if pre is not None else None
+    if u.is_contiguous():  # the shorter call, which would keep other strides
+        y = torch.empty_like(u)
+        z = torch.empty_like(u) if pre is not None else None
+    else:
+        y = u.new_empty(shape)
+        z = u.new_empty(shape) if pre is not None else None
     post_kind, post_w, post_b, post_eps = sides[0]
     pre_kind, pre_w, pre_b, pre_eps = sides[1]
     args = _lib.block_norm_args(v.data_ptr(), gate_ptr, res_ptr, post_w, post_b, scale_ptr, pre_w, pre_b, y.data_ptr(),
