@@ -310,15 +310,13 @@ def _broadcast(gate, shape, batch, rows, cols):
         except RuntimeError:
             raise ValueError(f"gate of shape {tuple(gate.shape)} does not broadcast to {tuple(shape)}") from None
         g = g.reshape(batch, rows, cols) if g.numel() else g.new_empty((batch, rows, cols))
-    full = (batch, rows, cols)[-len(shape):]
-    if g.dim() > len(full) or any(a != 1 and a != b for a, b in zip(reversed(g.shape), reversed(full))):
+    dims = g.dim()
+    sizes = (1, 1, 1)[dims:] + g.shape
+    if dims > len(shape) or dims > 3 or sizes[0] not in (1, batch) or sizes[1] not in (1, rows) or sizes[2] not in (1, cols):
         raise ValueError(f"gate of shape {tuple(gate.shape)} does not broadcast to {tuple(shape)}")
-    if g.dim() and g.shape[-1] != 1 and g.stride(-1) != 1:
+    if sizes[2] != 1 and g.stride(-1) != 1:
         g = g.contiguous()
-    strides = [0, 0, 0]
-    for i, (size, stride) in enumerate(zip(reversed(g.shape), reversed(g.stride()))):
-        if size != 1:
-            strides[2 - i] = stride
+    strides = [0 if size == 1 else stride for size, stride in zip(sizes, (0, 0, 0)[dims:] + g.stride())]
     return g, strides
 
 
