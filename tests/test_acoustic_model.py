@@ -248,3 +248,41 @@ def test_mxfp4_model_feeds_the_vocoder():
     durations = np.log(rng.integers(2, 5, ids.shape).astype(np.float64)).astype(np.float32)
     audio, mel = synthesize(model, ids, durations, -61.6, 20.4, return_mel=True, n_iter=4, init_phase=1)
     assert torch.isfinite(audio).all() and audio.shape == (256 * (mel.shape[0] - 1),)
+
+
+def held_in_mxfp4(model):
+    """The state of a model that was moved to the host after use_mxfp4(): its buffers come along."""
+    for layer in model._mxfp4_layers():
+        n, c, taps = layer.weight.shape
+        layer.mxfp4_data = torch.zeros(n * taps * -(-c // 128) * 68, dtype=torch.uint8)
+    return model
+
+
+@pytest.mark.parametrize("how", ["state_dict", "keras", "assign"])
+def test_mxfp4_model_on_the_host_loads_weights_whole(how):
+    w = random_weights(np.random.default_rng(13))
+    model, want = held_in_mxfp4(FastSpeechAcousticModel(VOCAB)), FastSpeechAcousticModel(VOCAB).load_keras_weights(w)
+    if how == "keras":
+        model.load_keras_weights(w)
+    else:
+        model.load_state_dict(want.state_dict(), assign=how == "assign")
+    got = model.state_dict()
+    assert all(torch.equal(got[k], v) for k, v in want.state_dict().items())
+    assert all(layer.stale for layer in model._mxfp4_layers())
+    # what was quantised before does not stand for these weights
+    with pytest.raises(ValueError, match="cannot be quantised"):
+        model((np.array([[3, 4]]), np.zeros((1, 2), np.float32)))
+    assert all(layer.stale for layer in model.float()._mxfp4_layers())
+    inputs = np.array([[3, 4, 5]]), np.ones((1, 3), np.float32)
+    assert torch.equal(model.use_mxfp4(False)(inputs), want(inputs))
+
+
+@pytest.mark.gpu
+def test_mxfp4_weights_loaded_on_the_host_or_in_another_type_are_quantised_on_the_way_back():
+    w, other = random_weights(np.random.default_rng(14)), random_weights(np.random.default_rng(15))
+    state = FastSpeechAcousticModel(VOCAB).load_keras_weights(other).state_dict()
+    for there, back in (("cpu", "cuda"), (torch.float64, torch.float32)):
+        model = quantised(w).to(there)
+        model.load_state_dict(state)
+        assert all(layer.stale for layer in model._mxfp4_layers())
+        assert same_layers(model.to(back), quantised(other)) and not any(layer.stale for layer in model._mxfp4_layers())

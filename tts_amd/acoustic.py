@@ -67,7 +67,11 @@ class _MaskedBiLSTM(nn.Module):
 class _SequenceConv(nn.Conv1d):
     """Conv1D(padding='same') whose weight can be held in MXFP4 beside the float one.  The quantised
     copy lies in a buffer outside the state dict: it moves with the module, and checkpoints stay what
-    they were."""
+    they were.  Weights that are loaded where they cannot be quantised (another device or type) leave it
+    `stale`: the load goes on, the layer refuses to run on it, and it is made anew when the module has
+    moved to where that can be done."""
+
+    stale = False
 
     def __init__(self, in_dim, out_dim, kernel, dilation=1):
         super().__init__(in_dim, out_dim, kernel, padding="same", dilation=dilation)
@@ -75,16 +79,29 @@ class _SequenceConv(nn.Conv1d):
         self.register_load_state_dict_post_hook(_SequenceConv.refresh)  # of this layer or of a module around it
 
     def refresh(self, *unused):
-        if self.mxfp4_data is not None:
+        if self.mxfp4_data is None:
+            return
+        self.stale = not self.weight.is_cuda or self.weight.dtype not in (torch.float32, torch.bfloat16, torch.float16)
+        if not self.stale:
             self.quantize(True)
+
+    def _apply(self, *args, **kwargs):  # what to(), cuda(), float() and their like end in
+        super()._apply(*args, **kwargs)
+        if self.stale:
+            self.refresh()
+        return self
 
     def quantize(self, on):
         self.mxfp4_data = mxfp4_quantize(self.weight.detach().permute(0, 2, 1)).data if on else None
+        self.stale = False
 
     def sequence(self, x, relu=False):  # (B, T, C)
         if self.mxfp4_data is None:
             y = self(x.transpose(1, 2))
             return (F.relu(y) if relu else y).transpose(1, 2)
+        if self.stale:
+            raise ValueError("the weights were loaded where they cannot be quantised: move the module to a ROCm GPU "
+                             "in float32, bfloat16 or float16 and call use_mxfp4() again")
         n, c, taps = self.weight.shape
         weight = MXFP4Tensor((n, taps, c) if taps > 1 else (n, c), self.mxfp4_data)
         activation = "relu" if relu else None
@@ -205,8 +222,9 @@ class FastSpeechAcousticModel(nn.Module):
         in place of torch's products and norms.  The model must be on a ROCm GPU.  The LSTMs, the duration
         predictor's last layer and the post-net, whose five applications of one layer would compound the
         rounding, stay in the model's own type.  The float weights remain; loading weights
-        (`load_keras_weights`, `load_state_dict` of the model or a part of it) quantises them anew, after other changes to them call
-        this again.  ``use_mxfp4(False)`` returns to the float form."""
+        (`load_keras_weights`, `load_state_dict` of the model or a part of it) quantises them anew (on the host:
+        when the model is back on the GPU), after other changes to them call this again.
+        ``use_mxfp4(False)`` returns to the float form."""
         for layer in self._mxfp4_layers():
             layer.quantize(on)
         return self
