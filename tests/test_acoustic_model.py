@@ -286,3 +286,38 @@ def test_mxfp4_weights_loaded_on_the_host_or_in_another_type_are_quantised_on_th
         model.load_state_dict(state)
         assert all(layer.stale for layer in model._mxfp4_layers())
         assert same_layers(model.to(back), quantised(other)) and not any(layer.stale for layer in model._mxfp4_layers())
+
+
+def test_mxfp4_weights_are_quantised_anew_in_place(monkeypatch):
+    from types import SimpleNamespace
+    from tts_amd import acoustic
+    made = iter((1, 2))
+    monkeypatch.setattr(acoustic, "mxfp4_quantize", lambda w: SimpleNamespace(data=torch.full((68,), next(made), dtype=torch.uint8)))
+    layer = FastSpeechAcousticModel(VOCAB).mel_out
+    layer.quantize(True)
+    kept = layer.mxfp4_data
+    layer.quantize(True)
+    assert layer.mxfp4_data is kept and (kept == 2).all()
+
+
+@pytest.mark.gpu
+def test_mxfp4_graph_follows_the_weights():
+    w, other = random_weights(np.random.default_rng(16)), random_weights(np.random.default_rng(17))
+    model, want = quantised(w), quantised(other)
+    blocks = [(m.encoder.block1, m.duration_predictor.blocks[0]) for m in (model, want)]
+    x = torch.randn(2, 30, 256, device="cuda")
+    with torch.no_grad():
+        [b(x) for b in blocks[0]]
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = [b(x) for b in blocks[0]]
+        for load in (lambda: None, lambda: model.load_keras_weights(other), lambda: model.load_keras_weights(w),
+                     lambda: model.load_state_dict(want.state_dict())):
+            load()
+            eager = [b(x) for b in blocks[0]]
+            for out in outs:
+                out.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(outs, eager))
+        assert all(torch.equal(a, b(x)) for a, b in zip(outs, blocks[1]))

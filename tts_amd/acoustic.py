@@ -92,7 +92,11 @@ class _SequenceConv(nn.Conv1d):
         return self
 
     def quantize(self, on):
+        old = self.mxfp4_data
         self.mxfp4_data = mxfp4_quantize(self.weight.detach().permute(0, 2, 1)).data if on else None
+        if on and old is not None and old.device == self.mxfp4_data.device and not old.is_inference():
+            # where it was: a graph that was captured with the old weights reads the new ones, as of the float weights
+            self.mxfp4_data = old.copy_(self.mxfp4_data)
         self.stale = False
 
     def sequence(self, x, relu=False):  # (B, T, C)
