@@ -321,3 +321,13 @@ def test_mxfp4_graph_follows_the_weights():
             torch.cuda.synchronize()
             assert all(torch.equal(a, b) for a, b in zip(outs, eager))
         assert all(torch.equal(a, b(x)) for a, b in zip(outs, blocks[1]))
+
+
+def test_mxfp4_copy_does_not_outlive_a_keras_load_that_ends_early():
+    w = random_weights(np.random.default_rng(18))
+    model = held_in_mxfp4(FastSpeechAcousticModel(VOCAB))
+    del w["post_bn_var"]
+    with pytest.raises(KeyError):
+        model.load_keras_weights(w)
+    assert np.array_equal(model.mel_out.bias.detach().numpy(), w["mel_out_bias"])
+    assert all(layer.stale for layer in model._mxfp4_layers())

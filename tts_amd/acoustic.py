@@ -253,6 +253,8 @@ class FastSpeechAcousticModel(nn.Module):
 
         def conv(mod, name):
             mod.weight.copy_(t(np.transpose(w[name + "_kernel"], (2, 1, 0))))
+            if isinstance(mod, _SequenceConv):  # now, not at the end, which a missing name keeps the load from
+                mod.refresh()
             mod.bias.copy_(t(w[name + "_bias"]))
 
         def norm(mod, name):
@@ -280,8 +282,6 @@ class FastSpeechAcousticModel(nn.Module):
             norm(self.post_net.bnorm1, "post_bn")
             self.post_net.bnorm1.running_mean.copy_(t(w["post_bn_mean"]))
             self.post_net.bnorm1.running_var.copy_(t(w["post_bn_var"]))
-        for layer in self._mxfp4_layers():
-            layer.refresh()
         return self
 
 
