@@ -331,3 +331,59 @@ def test_mxfp4_copy_does_not_outlive_a_keras_load_that_ends_early():
         model.load_keras_weights(w)
     assert np.array_equal(model.mel_out.bias.detach().numpy(), w["mel_out_bias"])
     assert all(layer.stale for layer in model._mxfp4_layers())
+
+
+def test_convolutions_can_be_replaced():
+    """A layer of another kind, of one's own or of a library, in the place of one of the model's."""
+    model = FastSpeechAcousticModel(VOCAB).load_keras_weights(random_weights(np.random.default_rng(19)))
+    inputs = np.array([[3, 4, 5]]), np.ones((1, 3), np.float32)
+    want = model(inputs)
+
+    def plain(conv):
+        other = torch.nn.Conv1d(conv.in_channels, conv.out_channels, conv.kernel_size, padding="same", dilation=conv.dilation)
+        other.load_state_dict(conv.state_dict())
+        return other
+
+    model.mel_out, model.encoder.block2.conv = plain(model.mel_out), plain(model.encoder.block2.conv)
+    assert torch.equal(model(inputs), want)
+
+
+def through(model, modules, run):
+    """What forward hooks on the modules see while `run` runs."""
+    seen = {}
+    hooks = [m.register_forward_hook(lambda m, args, out: seen.__setitem__(m, (args[0], out))) for m in modules]
+    out = run()
+    for h in hooks:
+        h.remove()
+    return out, [seen.get(m) for m in modules]
+
+
+def test_hooks_on_convolutions_fire_in_mxfp4(monkeypatch):
+    from tts_amd import acoustic
+
+    def product(x, weight, bias, dilation=1, activation=None):
+        y = bias + x.sum(-1, keepdim=True) * (-1.0) ** torch.arange(len(bias))
+        return torch.relu(y) if activation else y
+
+    for name in ("mxfp4_conv1d", "mxfp4_linear"):
+        monkeypatch.setattr(acoustic, name, product)
+    monkeypatch.setattr(acoustic, "block_norm", lambda u, post: u)
+    model = held_in_mxfp4(FastSpeechAcousticModel(VOCAB))
+    inputs = np.array([[3, 4, 5]]), np.ones((1, 3), np.float32)
+    want, convs = model(inputs), model._mxfp4_layers()
+    out, seen = through(model, convs, lambda: model(inputs))
+    assert torch.equal(out, want) and None not in seen
+    for conv, (x, y) in zip(convs, seen):
+        # (B, C, T), and before the rectifier, as in the float form
+        assert torch.equal(y, product(x.transpose(1, 2), None, conv.bias).transpose(1, 2)) and (y < 0).any()
+
+
+@pytest.mark.gpu
+def test_hooks_on_convolutions_change_nothing_in_mxfp4():
+    model = quantised(random_weights(np.random.default_rng(20)))
+    block, x = model.encoder.block1, torch.randn(2, 30, 256, device="cuda")
+    with torch.no_grad():
+        want = block(x)
+        out, [(given, y)] = through(block, [block.conv], lambda: block(x))
+        assert torch.equal(out, want) and torch.equal(given.transpose(1, 2), x) and (y < 0).any()
+        assert torch.equal(torch.relu(y), block.conv(given, relu=True))

@@ -99,19 +99,33 @@ class _SequenceConv(nn.Conv1d):
             self.mxfp4_data = old.copy_(self.mxfp4_data)
         self.stale = False
 
-    def sequence(self, x, relu=False):  # (B, T, C)
+    def forward(self, x, relu=False):  # (B, C, T)
         if self.mxfp4_data is None:
-            y = self(x.transpose(1, 2))
-            return (F.relu(y) if relu else y).transpose(1, 2)
+            y = super().forward(x)
+            return F.relu(y) if relu else y
         if self.stale:
             raise ValueError("the weights were loaded where they cannot be quantised: move the module to a ROCm GPU "
                              "in float32, bfloat16 or float16 and call use_mxfp4() again")
         n, c, taps = self.weight.shape
         weight = MXFP4Tensor((n, taps, c) if taps > 1 else (n, c), self.mxfp4_data)
-        activation = "relu" if relu else None
+        x, activation = x.transpose(-1, -2), "relu" if relu else None
         if taps == 1:
-            return mxfp4_linear(x, weight, self.bias, activation=activation)
-        return mxfp4_conv1d(x, weight, self.bias, dilation=self.dilation[0], activation=activation)
+            y = mxfp4_linear(x, weight, self.bias, activation=activation)
+        else:
+            y = mxfp4_conv1d(x, weight, self.bias, dilation=self.dilation[0], activation=activation)
+        return y.transpose(-1, -2)
+
+    def joins_relu(self):
+        """Whether the product may rectify its own output: a hook sees the layer's output before that."""
+        return self.mxfp4_data is not None and not self._forward_hooks and not nn.modules.module._global_forward_hooks
+
+
+def _along_time(layer, x, relu=False):
+    """`layer`, a convolution of (B, C, T), over (B, T, C)."""
+    if relu and isinstance(layer, _SequenceConv) and layer.joins_relu():
+        return layer(x.transpose(1, 2), relu=True).transpose(1, 2)
+    y = layer(x.transpose(1, 2))
+    return (F.relu(y) if relu else y).transpose(1, 2)
 
 
 class _ConvNorm(nn.Module):
@@ -123,8 +137,8 @@ class _ConvNorm(nn.Module):
         self.norm = nn.LayerNorm(out_dim, eps=_KERAS_EPS)
 
     def forward(self, x):  # (B, T, C)
-        y = self.conv.sequence(x, relu=True)
-        if self.conv.mxfp4_data is None:
+        y = _along_time(self.conv, x, relu=True)
+        if getattr(self.conv, "mxfp4_data", None) is None:
             return self.norm(y)
         return block_norm(y, post=Norm(self.norm.weight, self.norm.bias, eps=_KERAS_EPS))
 
@@ -216,7 +230,7 @@ class FastSpeechAcousticModel(nn.Module):
         x = self.encoder(x, lengths)
         self.last_duration_prediction = self.duration_predictor(x)
         x = length_regulate(x, durations)
-        mel_output = self.mel_out.sequence(x)
+        mel_output = _along_time(self.mel_out, x)
         return mel_output + self.post_net(mel_output)
 
     # -- MXFP4 ------------------------------------------------------------------------
