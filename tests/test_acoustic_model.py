@@ -387,3 +387,32 @@ def test_hooks_on_convolutions_change_nothing_in_mxfp4():
         out, [(given, y)] = through(block, [block.conv], lambda: block(x))
         assert torch.equal(out, want) and torch.equal(given.transpose(1, 2), x) and (y < 0).any()
         assert torch.equal(torch.relu(y), block.conv(given, relu=True))
+
+
+def test_norms_are_called_as_modules_with_their_own_eps(monkeypatch):
+    from tts_amd import acoustic
+    calls = []
+
+    def end(u, post):
+        calls.append(post)
+        return torch.nn.functional.layer_norm(u, u.shape[-1:], post.weight, post.bias, post.eps)
+
+    monkeypatch.setattr(acoustic, "block_norm", end)
+    # without convolutions of a kind that the host cannot run
+    monkeypatch.setattr(acoustic._SequenceConv, "quantize", lambda self, on: None)
+    model = FastSpeechAcousticModel(VOCAB)
+    inputs = np.array([[3, 4, 5]]), np.ones((1, 3), np.float32)
+    norms = [model.encoder.block1.norm, model.encoder.block2.norm, *(b.norm for b in model.duration_predictor.blocks)]
+    for n, norm in enumerate(norms):
+        norm.eps = 1e-3 * 2 ** n
+    want, plain = through(model, norms, lambda: model(inputs))
+    assert not calls
+    got, seen = through(model, norms, lambda: model.use_mxfp4()(inputs))
+    assert [c.eps for c in calls] == [norm.eps for norm in norms] and torch.equal(got, want)
+    assert all(torch.equal(a[1], b[1]) for a, b in zip(seen, plain))
+    model.encoder.block1.norm = torch.nn.Identity()
+    model(inputs)
+    assert len(calls) == 9
+    calls.clear()
+    model.use_mxfp4(False)(inputs)
+    assert not calls

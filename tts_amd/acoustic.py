@@ -128,19 +128,27 @@ def _along_time(layer, x, relu=False):
     return (F.relu(y) if relu else y).transpose(1, 2)
 
 
+class _RowNorm(nn.LayerNorm):
+    """LayerNorm that `block_norm` runs while `fused` is set, beside convolutions in MXFP4."""
+
+    fused = False
+
+    def forward(self, x):
+        if self.fused:
+            return block_norm(x, post=Norm(self.weight, self.bias, eps=self.eps))
+        return super().forward(x)
+
+
 class _ConvNorm(nn.Module):
     """Conv1D(padding='same', activation='relu') followed by LayerNormalization."""
 
     def __init__(self, in_dim, out_dim, kernel, dilation=1):
         super().__init__()
         self.conv = _SequenceConv(in_dim, out_dim, kernel, dilation)
-        self.norm = nn.LayerNorm(out_dim, eps=_KERAS_EPS)
+        self.norm = _RowNorm(out_dim, eps=_KERAS_EPS)
 
     def forward(self, x):  # (B, T, C)
-        y = _along_time(self.conv, x, relu=True)
-        if getattr(self.conv, "mxfp4_data", None) is None:
-            return self.norm(y)
-        return block_norm(y, post=Norm(self.norm.weight, self.norm.bias, eps=_KERAS_EPS))
+        return self.norm(_along_time(self.conv, x, relu=True))
 
 
 class Encoder(nn.Module):
@@ -245,6 +253,9 @@ class FastSpeechAcousticModel(nn.Module):
         ``use_mxfp4(False)`` returns to the float form."""
         for layer in self._mxfp4_layers():
             layer.quantize(on)
+        for norm in self.modules():
+            if isinstance(norm, _RowNorm):
+                norm.fused = on
         return self
 
     def _mxfp4_layers(self):
