@@ -776,3 +776,45 @@ def test_refusals_on_the_device():
             call()
     with pytest.raises(tts_amd._lib.GlvError, match="cols 32769"):
         block_norm(torch.ones(1, 32769, device="cuda"), post=Norm())
+
+
+def test_forward_mode_derivatives_are_refused():
+    """A dual tensor has requires_grad False and memory of its own; the tangent would be lost without a word."""
+    import torch.autograd.forward_ad as forward_ad
+    calls = (lambda x: mxfp4_quantize(x), lambda x: block_norm(x, post=Norm()))
+    with forward_ad.dual_level():
+        x = forward_ad.make_dual(torch.ones(3, 40), torch.ones(3, 40))
+        for call in calls:
+            for mode in (torch.enable_grad, torch.no_grad):
+                with mode(), pytest.raises(ValueError, match="forward-mode derivative"):
+                    call(x)
+            with pytest.raises(ValueError, match="ROCm GPU"):  # one without a tangent gets as far as any other
+                call(torch.ones(3, 40))
+    for call in calls:
+        with pytest.raises((ValueError, RuntimeError), match="forward-mode derivative"):
+            torch.func.jvp(call, (torch.ones(3, 40),), (torch.ones(3, 40),))
+
+
+def test_tracing_is_refused():
+    for call in (lambda x: mxfp4_quantize(x).dequantize(), lambda x: packed((3, 40)).dequantize(), lambda x: block_norm(x, post=Norm())):
+        with pytest.raises(ValueError, match="traced"):
+            torch.jit.trace(call, torch.ones(3, 40), check_trace=False)
+
+
+@gpu
+def test_derivatives_and_traces_of_products_are_refused():
+    import torch.autograd.forward_ad as forward_ad
+    x, bias = torch.ones(3, 40, device="cuda"), torch.ones(5, device="cuda")
+    w, wc = mxfp4_quantize(torch.ones(5, 40, device="cuda")), mxfp4_quantize(torch.ones(5, 3, 40, device="cuda"))
+    xq = mxfp4_quantize(x)
+    with forward_ad.dual_level():
+        dual, dual_bias = forward_ad.make_dual(x, x), forward_ad.make_dual(bias, bias)
+        for call in (lambda: mxfp4_linear(dual, w), lambda: mxfp4_conv1d(dual, wc), lambda: mxfp4_linear(x, w, dual_bias),
+                     lambda: mxfp4_linear(xq, w, dual_bias), lambda: block_norm(x, gate=dual), lambda: block_norm(x, residual=dual),
+                     lambda: block_norm(x, post=Norm(dual[0])), lambda: block_norm(x, scale=dual[0])):
+            with pytest.raises(ValueError, match="forward-mode derivative"):
+                call()
+        assert mxfp4_linear(x, w).shape == (3, 5)
+    for call in (lambda x: mxfp4_linear(x, w), lambda x: mxfp4_conv1d(x, wc), lambda x: mxfp4_linear(xq, w, x[0, :5])):
+        with pytest.raises(ValueError, match="traced"):
+            torch.jit.trace(call, x, check_trace=False)

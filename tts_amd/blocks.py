@@ -7,11 +7,14 @@ The reference's acoustic model is a stack of products with fixed weights, each f
 All arithmetic runs in libglvoc.so; torch owns the memory and the stream.  The functions enqueue
 work on torch's current stream of the inputs' device, allocate their outputs and workspace from
 torch (so they can be captured into a graph) and return without synchronising.  They are for
-inference: a tensor that asks for a gradient is refused while gradients are recorded.
+inference: a tensor that asks for a gradient is refused while gradients are recorded, one that carries a
+forward-mode derivative always, and so is every call under `torch.jit.trace`, which would keep the outputs'
+allocation and lose the work.
 """
 from __future__ import annotations
 
 import torch
+import torch.autograd.forward_ad as _forward_ad
 
 from . import _lib
 
@@ -33,6 +36,13 @@ _current_device = torch.cuda.current_device
 _current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
+_is_tracing = torch._C._is_tracing
+
+
+def _no_trace():
+    if _is_tracing():
+        raise ValueError("this operator cannot be traced: torch.jit.trace records torch's own operators alone")
+
 
 def _check(t, name, index=None):
     """The element type's number, after the checks that every float input passes; `index` is the device
@@ -42,6 +52,8 @@ def _check(t, name, index=None):
     kind = _TYPES.get(t.dtype)
     if kind is None:
         raise ValueError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
+    if _forward_ad._current_level >= 0 and _forward_ad.unpack_dual(t).tangent is not None:
+        raise ValueError(f"{name} carries a forward-mode derivative: this operator is for inference and would drop it")
     at = t.get_device()
     if at < 0:
         raise ValueError(f"{name} must be on a ROCm GPU (there is no CPU fallback), got {t.device}")
@@ -134,6 +146,7 @@ class MXFP4Tensor:
         kind = _TYPES.get(dtype)
         if kind is None:
             raise ValueError(f"dtype must be float32, bfloat16 or float16, got {dtype}")
+        _no_trace()
         data, shape = self.data, self.shape
         index = data.get_device()
         if index < 0:
@@ -158,6 +171,7 @@ def mxfp4_quantize(x):
     at least 2 ** -127; an element goes to the nearest code, ties to the even one, beyond 6 to 6.  A block
     that holds an infinity or a NaN reads back as NaN.  Any strides; a last dimension that is not
     contiguous is copied first."""
+    _no_trace()
     kind, shape = _check(x, "x"), x.shape
     if len(shape) < 1 or shape[-1] < 1:
         raise ValueError(f"x must have a last dimension of at least 1, got {tuple(shape)}")
@@ -179,6 +193,7 @@ def mxfp4_quantize(x):
 
 
 def _product(x, weight, bias, taps, dilation, activation, out_dtype):
+    _no_trace()
     act = _ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"activation must be None or 'relu', got {activation!r}")
@@ -332,6 +347,7 @@ def block_norm(u, *, post=None, gate=None, scale=None, residual=None, pre=None):
     pre       `Norm` the next block starts with, or None
 
     Statistics are 32 bits; y enters `pre` before it is rounded to u's type.  C is at most 32768."""
+    _no_trace()
     kind, shape, index = _check(u, "u"), u.shape, u.get_device()
     if len(shape) < 1 or shape[-1] < 1:
         raise ValueError(f"u must have a last dimension of at least 1, got {tuple(shape)}")
