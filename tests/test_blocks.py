@@ -818,3 +818,34 @@ def test_derivatives_and_traces_of_products_are_refused():
     for call in (lambda x: mxfp4_linear(x, w), lambda x: mxfp4_conv1d(x, wc), lambda x: mxfp4_linear(xq, w, x[0, :5])):
         with pytest.raises(ValueError, match="traced"):
             torch.jit.trace(call, x, check_trace=False)
+
+
+def negated(*shape, device="cpu"):
+    """Values whose memory holds their opposites: the imaginary part of a conjugated tensor."""
+    v = torch.arange(1.0, 1 + int(np.prod(shape)), device=device).reshape(shape)
+    x = torch.complex(torch.zeros_like(v), -v).conj().imag
+    assert x.is_neg() and torch.equal(x, v)
+    return x
+
+
+@pytest.mark.parametrize("shape", [(5, 3), (5, 1), (1, 1), (2, 4, 1), (1,), (4,), (2, 2, 2, 1), (2, 2, 2, 3)])
+def test_pending_negations_are_resolved_on_the_way(shape):
+    from tts_amd import blocks
+    x = negated(*shape)
+    t, batch, rows, batch_stride, row_stride = blocks._rows(x, x.shape)
+    assert not t.is_neg() and torch.equal(t.as_strided((batch, rows, shape[-1]), (batch_stride, row_stride, 1)), x.reshape(batch, rows, -1))
+    g, strides = blocks._broadcast(negated(4, 1), torch.Size((2, 4, 3)), 2, 4, 3)
+    assert not g.is_neg() and torch.equal(g.as_strided((2, 4, 3), strides)[0, :, 2], torch.arange(1.0, 5))
+
+
+@gpu
+def test_pending_negations_reach_the_kernels_resolved():
+    for n in (1, 3):
+        x, w = negated(4, n, device="cuda"), mxfp4_quantize(torch.ones(n, n, device="cuda"))
+        v = negated(n, device="cuda")
+        plain, pv = x.resolve_neg(), v.resolve_neg()
+        for got, want in ((mxfp4_quantize(x).dequantize(), mxfp4_quantize(plain).dequantize()), (mxfp4_linear(x, w, v), mxfp4_linear(plain, w, pv)),
+                          (block_norm(x, gate=x, residual=x, scale=v), block_norm(plain, gate=plain, residual=plain, scale=pv)),
+                          (block_norm(x, post=Norm(v, v), gate=x[:, :1]), block_norm(plain, post=Norm(pv, pv), gate=plain[:, :1]))):
+            assert torch.equal(got, want) and not got.is_neg()
+        assert (mxfp4_linear(x, w) > 0).all()

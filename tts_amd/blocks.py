@@ -69,12 +69,14 @@ def _vector(t, name, n, index):
     kind = _check(t, name, index)
     if t.shape != (n,):
         raise ValueError(f"{name} must have shape ({n},), got {tuple(t.shape)}")
-    return (t if t.stride(0) == 1 or n == 1 else t.contiguous()), kind
+    return (t if t.stride(0) == 1 and n != 1 else t.resolve_neg().contiguous()), kind
 
 
 def _rows(x, shape):
     """(tensor, batch, rows, batch stride, row stride) of x as (batch, rows, cols) with a contiguous last
-    dimension; a copy only where no view will do."""
+    dimension; a copy only where no view will do.  The imaginary part of a conjugated tensor is such a case: its
+    memory holds the values before a negation.  Those are two elements apart, so that any copy for the last
+    dimension's sake resolves them, and only a single column has to be looked at."""
     if max(shape) > _INT:
         raise ValueError(f"a dimension of {tuple(shape)} is larger than {_INT}")
     dims = len(shape)
@@ -84,7 +86,10 @@ def _rows(x, shape):
         x = x.reshape(-1, shape[-2], shape[-1]) if x.numel() else x.new_empty((0, shape[-2], shape[-1]))
         shape, dims = x.shape, 3
     strides = x.stride()
-    if strides[-1] != 1 and shape[-1] > 1:
+    if shape[-1] == 1:
+        x = x.resolve_neg()
+        strides = x.stride()
+    elif strides[-1] != 1:
         x = x.contiguous()
         strides = x.stride()
     if dims == 2:
@@ -309,8 +314,8 @@ def _norm_vector(t, name, cols, index, kind, seen, held):
         raise ValueError(f"{name} must have shape ({cols},), got {tuple(t.shape)}")
     if k != seen and (seen is not None or (k != 0 and k != kind)):
         raise ValueError(f"weights, biases and scale must all be float32 or all of u's type, got {t.dtype}")
-    if t.stride(0) != 1 and cols != 1:
-        t = t.contiguous()
+    if t.stride(0) != 1 or cols == 1:
+        t = t.resolve_neg().contiguous()
         held.append(t)
     return t.data_ptr(), k
 
@@ -329,7 +334,9 @@ def _broadcast(gate, shape, batch, rows, cols):
     sizes = (1, 1, 1)[dims:] + g.shape
     if dims > len(shape) or dims > 3 or sizes[0] not in (1, batch) or sizes[1] not in (1, rows) or sizes[2] not in (1, cols):
         raise ValueError(f"gate of shape {tuple(gate.shape)} does not broadcast to {tuple(shape)}")
-    if sizes[2] != 1 and g.stride(-1) != 1:
+    if sizes[2] == 1:
+        g = g.resolve_neg()
+    elif g.stride(-1) != 1:
         g = g.contiguous()
     strides = [0 if size == 1 else stride for size, stride in zip(sizes, (0, 0, 0)[dims:] + g.stride())]
     return g, strides
