@@ -459,8 +459,10 @@ int glv_mxfp4_dequantize(const glv_mxfp4_array* array, void* stream);
  *   y_dev                       (batch, rows, n_out) of y_type
  *   workspace_dev               glv_mxfp4_product_workspace() bytes, 16-byte aligned, free to use
  *                               until the work on the stream is done (NULL when that is 0);
- *                               the function returns -1 for a shape that the product refuses.
- * taps * cols and n_out are at most 2^18, n_out * taps and (taps - 1) * dilation at most 2^24.
+ *                               the function returns -1 (and glv_last_error() says why) for sizes or
+ *                               an x_type that the product refuses.
+ * taps * cols and n_out are at most 2^18, n_out * taps and (taps - 1) * dilation at most 2^24; x to be
+ * quantised has fewer than 2^37 elements and y than 2^38, rounded up to whole tiles.
  */
 enum { GLV_ACT_NONE = 0, GLV_ACT_RELU = 1 };
 typedef struct glv_mxfp4_product_args {

@@ -849,3 +849,34 @@ def test_pending_negations_reach_the_kernels_resolved():
                           (block_norm(x, post=Norm(v, v), gate=x[:, :1]), block_norm(plain, post=Norm(pv, pv), gate=plain[:, :1]))):
             assert torch.equal(got, want) and not got.is_neg()
         assert (mxfp4_linear(x, w) > 0).all()
+
+
+def test_workspace_refuses_what_the_product_refuses():
+    from tts_amd import _lib
+    lib = _lib.load()
+    a = 4096  # never looked at: every call below is refused first
+    shapes = [  # (x_type, batch, rows, cols, n_out, taps, dilation)
+        (0, 1, 64, 4096, (1 << 18) + 1, 1, 1), (0, 1, 64, 4096, 8, 1 << 14, 1), (0, 1, 4, 32, 8, 2, (1 << 24) + 1), (0, 1, 4, 32, 1 << 18, 128, 1),
+        (1, 1, 64, 4096, -1, 1, 1), (4, 1, 4, 32, 8, 1, 1), (0, -1, 4, 32, 8, 1, 1), (0, 1, -4, 32, 8, 1, 1), (0, 1, 4, 1 << 19, 8, 1, 1),
+        (0, 1 << 12, 1 << 13, 32, 8, 1, 1), (2, 1, 1 << 24, 1 << 18, 8, 1, 1), (3, 1, 1 << 24, 32, 1 << 18, 1, 1), (0, 1, 1 << 24, 32, 1 << 18, 1, 1)]
+    for shape in shapes:
+        args = _lib.mxfp4_product_args(a, a, a, a, 0, a, 0, shape[3], *shape, 0, 0, 0)
+        assert lib.glv_mxfp4_product_workspace(args) == -1, shape
+        assert b"glv_mxfp4_product_workspace" in lib.glv_last_error()
+        assert lib.glv_mxfp4_product(args, a, 1 << 62, None) == -1, shape
+    assert lib.glv_mxfp4_product_workspace(None) == -1
+    for shape in ((0, 1, 0, 32, 8, 1, 1), (0, 1, 4, 32, 0, 1, 1), (3, 1, 1 << 24, 1 << 18, 1 << 7, 1, 1), (0, 1, 1 << 24, 32, 127 << 7, 1, 1),
+                  (0, 1, 64, 1 << 17, 1 << 18, 2, 1 << 24), (0, 1, 4, 32, 8, 1, (1 << 31) - 1)):
+        args = _lib.mxfp4_product_args(0, 0, 0, 0, 0, 0, 0, shape[3], *shape, 0, 0, 0)
+        assert lib.glv_mxfp4_product_workspace(args) >= 0, shape
+
+
+@gpu
+def test_a_large_refused_product_allocates_nothing():
+    one, w = torch.ones(1, 1, 8, device="cuda", dtype=torch.float16), mxfp4_quantize(torch.ones(64, 8, device="cuda"))
+    wide = MXFP4Tensor(((1 << 18) + 1, 8), torch.zeros(((1 << 18) + 1) * 68, dtype=torch.uint8, device="cuda"))
+    before, _ = torch.cuda.memory_allocated(), torch.cuda.reset_peak_memory_stats()
+    for call in (lambda: mxfp4_linear(one.expand(1 << 13, (1 << 12) + 1, 8), w), lambda: mxfp4_linear(one[0].expand(1 << 13, 8), wide)):
+        with pytest.raises(tts_amd._lib.GlvError, match="outside"):
+            call()
+        assert torch.cuda.max_memory_allocated() == before

@@ -26,6 +26,7 @@ _ACTIVATIONS = {None: 0, "relu": 1}
 _NORMS = {"layer": 1, "rms": 2}
 _GROUP = 128  # columns that share one dword of scales
 _INT = (1 << 31) - 1  # the library counts in ints; its own limits, which it names, are lower
+_LARGE = 1 << 27  # elements of an output from which on the library is asked whether it takes the call before allocating
 
 
 # The calls below take a few microseconds on the host, as much as a small launch on the device, so
@@ -240,6 +241,9 @@ def _product(x, weight, bias, taps, dilation, activation, out_dtype):
         bias_ptr = bias.data_ptr()
     lib = _lib.load()
     shape = (*shape[:-1], n)
+    if batch * rows * n > _LARGE and lib.glv_mxfp4_product_workspace(_lib.mxfp4_product_args(
+            0, 0, 0, 0, 0, 0, 0, 0, kind, batch, rows, cols, n, taps, dilation, 0, 0, 0)) < 0:
+        _lib.check(-1)
     y = like.new_empty(shape) if out_kind == kind else like.new_empty(shape, dtype=out_dtype)
     args = _lib.mxfp4_product_args(data, scales, *weight._pointers(), bias_ptr, y.data_ptr(), batch_stride, row_stride, kind,
                                    batch, rows, cols, n, taps, dilation, bias_kind, act, out_kind)

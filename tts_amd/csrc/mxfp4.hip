@@ -797,9 +797,7 @@ __global__ __launch_bounds__((Tiling<TM, TN, !std::is_void_v<X>>::kThreads * TEA
 template <int TM, int TN, int TEAMS = 1, typename X = void>
 int launch_tiled(const Product& p, hipStream_t st) {
     using L = Tiling<TM, TN, !std::is_void_v<X>>;
-    const int64_t count = (int64_t)((p.rows + TM - 1) / TM) * ((p.n + TN - 1) / TN);
-    if (too_large(count, L::kThreads * TEAMS)) return report(GLV_ERR_INVALID, "glv_mxfp4_product: rows x n_out too large for one call");
-    const unsigned tiles = (unsigned)count;
+    const unsigned tiles = (unsigned)((p.rows + TM - 1) / TM) * (unsigned)((p.n + TN - 1) / TN);
     if (p.taps > 1)
         hipLaunchKernelGGL((product_tiled_kernel<X, true, TM, TN, TEAMS>), dim3(tiles), dim3(L::kThreads * TEAMS), 0, st, p);
     else
@@ -939,10 +937,30 @@ extern "C" int glv_mxfp4_dequantize(const glv_mxfp4_array* a, void* stream) {
     return launch_status("dequantise_kernel");
 }
 
+// The sizes and the type of x; GLV_OK with *all rows.
+static int check_product(const char* what, const glv_mxfp4_product_args& a, int64_t* all) {
+    if (a.batch < 0 || a.rows < 0) return report(GLV_ERR_INVALID, "%s: negative batch or rows", what);
+    *all = (int64_t)a.batch * a.rows;
+    const int rc = check_shape(what, *all, a.cols);
+    if (rc != GLV_OK) return rc;
+    if (a.n_out < 0 || a.n_out > kMaxCols) return report(GLV_ERR_INVALID, "%s: n_out %d outside [0, %d]", what, a.n_out, kMaxCols);
+    if (a.taps < 1 || a.dilation < 1 || (int64_t)a.taps * a.cols > kMaxCols || (int64_t)a.n_out * a.taps > kMaxRows ||
+        (int64_t)(a.taps - 1) * a.dilation > kMaxRows)
+        return report(GLV_ERR_INVALID, "%s: taps %d and dilation %d must be positive, taps x columns at most %d, "
+                      "n_out x taps and (taps - 1) x dilation at most %lld", what, a.taps, a.dilation, kMaxCols, (long long)kMaxRows);
+    if (!float_type(a.x_type) && a.x_type != GLV_MXFP4) return report(GLV_ERR_INVALID, "%s: unknown element type %d of x", what, a.x_type);
+    // what a launch holds: the quantiser's rows, and tiles of 128 x 128 by 256 threads (the larger ones are fewer, by more)
+    if ((a.x_type != GLV_MXFP4 && too_large(span_blocks((int)*all, (a.cols + kGroup - 1) / kGroup), 256)) ||
+        too_large(((*all + 127) / 128) * ((a.n_out + 127) / 128), 256))
+        return report(GLV_ERR_INVALID, "%s: rows x columns or rows x n_out too large for one call", what);
+    return GLV_OK;
+}
+
 extern "C" int64_t glv_mxfp4_product_workspace(const glv_mxfp4_product_args* a) {
-    if (!a || a->batch < 0 || a->rows < 0 || a->n_out < 0 || a->taps < 1 || a->dilation < 1 || a->cols < 1 || a->cols > kMaxCols) return -1;
-    const int64_t all = (int64_t)a->batch * a->rows;
-    if (all > kMaxRows || !(float_type(a->x_type) || a->x_type == GLV_MXFP4)) return -1;
+    const char* what = "glv_mxfp4_product_workspace";
+    if (!a) return report(GLV_ERR_INVALID, "%s: null argument", what);
+    int64_t all = 0;
+    if (check_product(what, *a, &all) != GLV_OK) return -1;
     if (a->x_type == GLV_MXFP4 || own_tile(all, a->cols, a->n_out, a->taps, a->dilation)) return 0;
     return quantised_bytes(all, (a->cols + kGroup - 1) / kGroup);
 }
@@ -952,16 +970,9 @@ extern "C" int glv_mxfp4_product(const glv_mxfp4_product_args* a, void* workspac
     if (!a) return report(GLV_ERR_INVALID, "%s: null argument", what);
     const auto [x_dev, x_scales_dev, w_codes_dev, w_scales_dev, bias_dev, y_dev, x_batch_stride, x_row_stride, x_type, batch, rows, cols,
                 n_out, taps, dilation, bias_type, activation, y_type] = *a;
-    if (batch < 0 || rows < 0) return report(GLV_ERR_INVALID, "%s: negative batch or rows", what);
-    const int64_t all = (int64_t)batch * rows;
-    int rc = check_shape(what, all, cols);
+    int64_t all = 0;
+    int rc = check_product(what, *a, &all);
     if (rc != GLV_OK) return rc;
-    if (n_out < 0 || n_out > kMaxCols) return report(GLV_ERR_INVALID, "%s: n_out %d outside [0, %d]", what, n_out, kMaxCols);
-    if (taps < 1 || dilation < 1 || (int64_t)taps * cols > kMaxCols || (int64_t)n_out * taps > kMaxRows ||
-        (int64_t)(taps - 1) * dilation > kMaxRows)
-        return report(GLV_ERR_INVALID, "%s: taps %d and dilation %d must be positive, taps x columns at most %d, "
-                      "n_out x taps and (taps - 1) x dilation at most %lld", what, taps, dilation, kMaxCols, (long long)kMaxRows);
-    if (!float_type(x_type) && x_type != GLV_MXFP4) return report(GLV_ERR_INVALID, "%s: unknown element type %d of x", what, x_type);
     if (!float_type(y_type)) return report(GLV_ERR_INVALID, "%s: unknown element type %d of y", what, y_type);
     if (activation != GLV_ACT_NONE && activation != GLV_ACT_RELU) return report(GLV_ERR_INVALID, "%s: unknown activation %d", what, activation);
     if (bias_dev && !float_type(bias_type)) return report(GLV_ERR_INVALID, "%s: unknown element type %d of the bias", what, bias_type);
