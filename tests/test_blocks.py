@@ -880,3 +880,29 @@ def test_a_large_refused_product_allocates_nothing():
         with pytest.raises(tts_amd._lib.GlvError, match="outside"):
             call()
         assert torch.cuda.max_memory_allocated() == before
+
+
+@gpu
+def test_an_earlier_error_of_another_call_is_not_this_ones():
+    """An error that its caller has dealt with (here: a device that does not exist) waits in the runtime."""
+    from tts_amd import _lib
+    lib, stream = _lib.load(), torch.cuda.current_stream().cuda_stream
+    x, w, out = torch.ones(40, 64, device="cuda"), torch.ones(8, 64, device="cuda"), torch.empty(40, 64, device="cuda")
+    q, y = mxfp4_quantize(w), torch.empty(40, 8, device="cuda")
+    again = MXFP4Tensor((8, 64), torch.zeros_like(q.data))
+    calls = [
+        lambda: lib.glv_mxfp4_quantize(_lib.mxfp4_array(w.data_ptr(), *again._pointers(), 0, 64, 0, 1, 8, 64), stream),
+        lambda: lib.glv_mxfp4_dequantize(_lib.mxfp4_array(out.data_ptr(), *q._pointers(), 0, 0, 0, 1, 8, 64), stream),
+        lambda: lib.glv_mxfp4_product(_lib.mxfp4_product_args(x.data_ptr(), 0, *q._pointers(), 0, y.data_ptr(), 0, 64, 0, 1, 40, 64, 8,
+                                                              1, 1, 0, 0, 0), None, 0, stream),
+        lambda: lib.glv_block_norm(_lib.block_norm_args(x.data_ptr(), 0, 0, 0, 0, 0, 0, 0, out.data_ptr(), 0, 0, 64, 0, 0, 0, 0, 0, 1, 40,
+                                                        64, 0, 2, 0, 1, 0.0, 0.0, 1.0), stream)]
+    torch.cuda.synchronize()
+    rcs = []
+    for call in calls:
+        refused = lib.hipSetDevice(1000)
+        rcs.append((refused != 0, call()))
+        lib.hipGetLastError()
+    torch.cuda.synchronize()
+    assert rcs == [(True, 0)] * 4, lib.glv_last_error()
+    assert torch.equal(again.data, q.data) and (y == 64).all() and (out == 1).all()

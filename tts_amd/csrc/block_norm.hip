@@ -250,26 +250,20 @@ __global__ __launch_bounds__(LANES > 0 ? 256 : 1024) void block_norm_kernel(Bloc
 // 8.8, with four eights 11.3; 4000 x 9000 94 and 113) up to twelve, of which a CU holds two workgroups (4000 x 12200 125
 // and 141), then four eights (4000 x 12400 137, with two 153).
 template <typename T, typename W>
-int launch(const BlockNorm& p, hipStream_t st) {
+int run(const BlockNorm& p, hipStream_t st) {
     const int pieces = (p.cols + 7) / 8;  // a lane holds one, two or four of them
     const int threads = (pieces <= 1536 ? (pieces + 127) / 128 : (pieces + 255) / 256) * 64;  // of a workgroup to itself
     if (pieces > 128 && too_large(p.rows, threads)) return report(GLV_ERR_INVALID, "glv_block_norm: rows x columns too large for one call");
-    auto rows_a_wave = [&](int lanes) { return dim3((unsigned)(((int64_t)p.rows * lanes + 255) / 256)); };
-    if (p.cols < 16 / (int)sizeof(T))
-        hipLaunchKernelGGL((block_norm_kernel<T, W, 16, 1, true>), rows_a_wave(16), dim3(256), 0, st, p);
-    else if (pieces <= 16)
-        hipLaunchKernelGGL((block_norm_kernel<T, W, 16, 1>), rows_a_wave(16), dim3(256), 0, st, p);
-    else if (pieces <= 32)
-        hipLaunchKernelGGL((block_norm_kernel<T, W, 32, 1>), rows_a_wave(32), dim3(256), 0, st, p);
-    else if (pieces <= 64)
-        hipLaunchKernelGGL((block_norm_kernel<T, W, 64, 1>), rows_a_wave(64), dim3(256), 0, st, p);
-    else if (pieces <= 128)
-        hipLaunchKernelGGL((block_norm_kernel<T, W, 64, 2>), rows_a_wave(64), dim3(256), 0, st, p);
-    else if (pieces <= 1536)
-        hipLaunchKernelGGL((block_norm_kernel<T, W, 0, 2>), dim3(p.rows), dim3(threads), 0, st, p);
-    else
-        hipLaunchKernelGGL((block_norm_kernel<T, W, 0, 4>), dim3(p.rows), dim3(threads), 0, st, p);
-    return launch_status("block_norm_kernel");
+    auto rows_a_wave = [&](auto kernel, int lanes) {
+        return launch("block_norm_kernel", kernel, dim3((unsigned)(((int64_t)p.rows * lanes + 255) / 256)), dim3(256), 0, st, p);
+    };
+    if (p.cols < 16 / (int)sizeof(T)) return rows_a_wave(block_norm_kernel<T, W, 16, 1, true>, 16);
+    if (pieces <= 16) return rows_a_wave(block_norm_kernel<T, W, 16, 1>, 16);
+    if (pieces <= 32) return rows_a_wave(block_norm_kernel<T, W, 32, 1>, 32);
+    if (pieces <= 64) return rows_a_wave(block_norm_kernel<T, W, 64, 1>, 64);
+    if (pieces <= 128) return rows_a_wave(block_norm_kernel<T, W, 64, 2>, 64);
+    return launch("block_norm_kernel", pieces <= 1536 ? block_norm_kernel<T, W, 0, 2> : block_norm_kernel<T, W, 0, 4>, dim3(p.rows),
+                  dim3(threads), 0, st, p);
 }
 
 constexpr int kMaxCols = 32768;         // 1024 threads of 32 columns
@@ -314,7 +308,7 @@ extern "C" int glv_block_norm(const glv_block_norm_args* a, void* stream) {
     p.y = y_dev, p.z = z_dev;
     p.rows = batch * rows, p.T = rows, p.cols = cols;
     hipStream_t st = (hipStream_t)stream;
-    if (type == GLV_F32) return launch<float, float>(p, st);
-    if (type == GLV_BF16) return vector_type == GLV_F32 ? launch<bf16, float>(p, st) : launch<bf16, bf16>(p, st);
-    return vector_type == GLV_F32 ? launch<f16, float>(p, st) : launch<f16, f16>(p, st);
+    if (type == GLV_F32) return run<float, float>(p, st);
+    if (type == GLV_BF16) return vector_type == GLV_F32 ? run<bf16, float>(p, st) : run<bf16, bf16>(p, st);
+    return vector_type == GLV_F32 ? run<f16, float>(p, st) : run<f16, f16>(p, st);
 }

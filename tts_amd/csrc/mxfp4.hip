@@ -798,11 +798,8 @@ template <int TM, int TN, int TEAMS = 1, typename X = void>
 int launch_tiled(const Product& p, hipStream_t st) {
     using L = Tiling<TM, TN, !std::is_void_v<X>>;
     const unsigned tiles = (unsigned)((p.rows + TM - 1) / TM) * (unsigned)((p.n + TN - 1) / TN);
-    if (p.taps > 1)
-        hipLaunchKernelGGL((product_tiled_kernel<X, true, TM, TN, TEAMS>), dim3(tiles), dim3(L::kThreads * TEAMS), 0, st, p);
-    else
-        hipLaunchKernelGGL((product_tiled_kernel<X, false, TM, TN, TEAMS>), dim3(tiles), dim3(L::kThreads * TEAMS), 0, st, p);
-    return launch_status("product_tiled_kernel");
+    return launch("product_tiled_kernel", p.taps > 1 ? product_tiled_kernel<X, true, TM, TN, TEAMS> : product_tiled_kernel<X, false, TM, TN, TEAMS>,
+                  dim3(tiles), dim3(L::kThreads * TEAMS), 0, st, p);
 }
 
 // rows sixteen at a time by groups four at a time
@@ -813,20 +810,13 @@ int quantise(const char* what, const void* x, int type, Rows xr, int rows, int c
     const int64_t blocks = span_blocks(rows, groups);
     if (too_large(blocks, 256)) return report(GLV_ERR_INVALID, "%s: rows x columns too large for one call", what);
     const dim3 grid((unsigned)blocks), block(256);
-    auto launch = [&](auto* typed) {
+    auto run = [&](auto* typed) {
         using T = std::remove_const_t<std::remove_pointer_t<decltype(typed)>>;
-        if (cols < 8)
-            hipLaunchKernelGGL((quantise_kernel<T, true>), grid, block, 0, st, typed, xr, rows, cols, groups, codes, scales);
-        else
-            hipLaunchKernelGGL((quantise_kernel<T, false>), grid, block, 0, st, typed, xr, rows, cols, groups, codes, scales);
+        return launch("quantise_kernel", cols < 8 ? quantise_kernel<T, true> : quantise_kernel<T, false>, grid, block, 0, st, typed, xr, rows,
+                      cols, groups, codes, scales);
     };
-    if (type == GLV_F32)
-        launch(static_cast<const float*>(x));
-    else if (type == GLV_BF16)
-        launch(static_cast<const bf16*>(x));
-    else
-        launch(static_cast<const f16*>(x));
-    return launch_status("quantise_kernel");
+    if (type == GLV_F32) return run(static_cast<const float*>(x));
+    return type == GLV_BF16 ? run(static_cast<const bf16*>(x)) : run(static_cast<const f16*>(x));
 }
 
 // Rows of x that one tile of `tile` rows of y reaches, at most.
@@ -839,11 +829,9 @@ int64_t reached_rows(int64_t rows, int tile, int taps, int dilation) {
 template <typename X>
 int launch_direct(const Product& p, unsigned tiles, hipStream_t st) {
     const size_t held = std::is_void_v<X> ? 0 : reached_rows(p.rows, 32, p.taps, p.dilation) * p.groups * (kGroupBytes + 4);
-    if (p.taps * p.groups <= 4)
-        hipLaunchKernelGGL((product_direct_kernel<X, 4>), dim3(tiles), dim3(256), held, st, p);
-    else
-        hipLaunchKernelGGL((product_direct_kernel<X, 8>), dim3(tiles), dim3(512), held, st, p);
-    return launch_status("product_direct_kernel");
+    const bool few = p.taps * p.groups <= 4;
+    return launch("product_direct_kernel", few ? product_direct_kernel<X, 4> : product_direct_kernel<X, 8>, dim3(tiles), dim3(few ? 256 : 512),
+                  held, st, p);
 }
 
 // The tile in which a product quantises its activations itself (columns of y; 0: it does not): every tile
@@ -928,13 +916,12 @@ extern "C" int glv_mxfp4_dequantize(const glv_mxfp4_array* a, void* stream) {
     if (too_large(blocks, 256)) return report(GLV_ERR_INVALID, "%s: rows x columns too large for one call", what);
     const dim3 grid((unsigned)blocks), block(256);
     hipStream_t st = (hipStream_t)stream;
-    if (out_type == GLV_F32)
-        hipLaunchKernelGGL(dequantise_kernel<float>, grid, block, 0, st, codes_dev, scales_dev, rows, cols, groups, (float*)out_dev);
-    else if (out_type == GLV_BF16)
-        hipLaunchKernelGGL(dequantise_kernel<bf16>, grid, block, 0, st, codes_dev, scales_dev, rows, cols, groups, (bf16*)out_dev);
-    else
-        hipLaunchKernelGGL(dequantise_kernel<f16>, grid, block, 0, st, codes_dev, scales_dev, rows, cols, groups, (f16*)out_dev);
-    return launch_status("dequantise_kernel");
+    auto run = [&](auto* typed) {
+        using T = std::remove_pointer_t<decltype(typed)>;
+        return launch("dequantise_kernel", dequantise_kernel<T>, grid, block, 0, st, codes_dev, scales_dev, rows, cols, groups, typed);
+    };
+    if (out_type == GLV_F32) return run((float*)out_dev);
+    return out_type == GLV_BF16 ? run((bf16*)out_dev) : run((f16*)out_dev);
 }
 
 // The sizes and the type of x; GLV_OK with *all rows.
@@ -1000,14 +987,14 @@ extern "C" int glv_mxfp4_product(const glv_mxfp4_product_args* a, void* workspac
         p.xc = static_cast<const uint8_t*>(x_dev), p.xs = x_scales_dev;
     } else if (const int tile = own_tile(all, cols, n_out, taps, dilation)) {
         p.x = x_dev, p.xr = Rows{x_batch_stride, x_row_stride, rows, batch == 1}, p.cols = cols;
-        auto launch = [&](auto* typed) {
+        auto run = [&](auto* typed) {
             using X = std::remove_pointer_t<decltype(typed)>;
             if (tile == 256) return launch_tiled<128, 256, 1, X>(p, st);
             if (tile == 128) return launch_tiled<128, 128, 1, X>(p, st);
             return launch_direct<X>(p, (unsigned)tiles, st);
         };
-        if (x_type == GLV_F32) return launch((float*)nullptr);
-        return x_type == GLV_BF16 ? launch((bf16*)nullptr) : launch((f16*)nullptr);
+        if (x_type == GLV_F32) return run((float*)nullptr);
+        return x_type == GLV_BF16 ? run((bf16*)nullptr) : run((f16*)nullptr);
     } else {
         const int64_t need = quantised_bytes(all, p.groups);
         if (!workspace_dev || workspace_bytes < need)

@@ -21,9 +21,18 @@ inline int report(int code, const char* fmt, ...) {
     return code;
 }
 
-inline int launch_status(const char* what) {
-    const hipError_t e = hipGetLastError();
-    return e == hipSuccess ? GLV_OK : report(GLV_ERR_HIP, "%s: launch failed: %s", what, hipGetErrorString(e));
+// Launches `kernel` and reports that launch's own error: an earlier one, of another library's call that its caller has
+// dealt with, stays in hipGetLastError() and is none of this call's.
+template <typename... P, typename... A>
+int launch(const char* what, void (*kernel)(P...), dim3 grid, dim3 block, size_t lds, hipStream_t stream, A... args) {
+    static_assert(sizeof...(P) == sizeof...(A), "an argument for every parameter");
+    return [&](P... values) {
+        void* pointers[] = {const_cast<void*>(static_cast<const void*>(&values))...};
+        const hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, block, pointers, lds, stream);
+        if (e == hipSuccess) return (int)GLV_OK;
+        (void)hipGetLastError();  // it is reported here, and not once more by whoever looks next
+        return report(GLV_ERR_HIP, "%s: launch failed: %s", what, hipGetErrorString(e));
+    }(args...);
 }
 
 // A launch counts its threads in 32 bits.
