@@ -906,3 +906,17 @@ def test_an_earlier_error_of_another_call_is_not_this_ones():
     torch.cuda.synchronize()
     assert rcs == [(True, 0)] * 4, lib.glv_last_error()
     assert torch.equal(again.data, q.data) and (y == 64).all() and (out == 1).all()
+
+
+def test_inline_assembly_names_the_registers_that_it_writes():
+    """Every statement that writes M0 lists it, so that the compiler keeps its own uses of it away."""
+    import re
+    here = os.path.join(os.path.dirname(os.path.abspath(tts_amd.__file__)), "csrc")
+    found = 0
+    for name in ("mxfp4.hip", "block_norm.hip", "lowp.h"):
+        with open(os.path.join(here, name)) as f:
+            statements = re.findall(r"asm volatile\((.*?)\);", f.read(), re.S)
+        for statement in (s for s in statements if "s_mov_b32 m0" in s):
+            found += 1
+            assert '"m0"' in statement.rsplit(":", 1)[1], (name, statement)
+    assert found == 4

@@ -428,21 +428,24 @@ __device__ __align__(64) const uint32_t g_zeros[16] = {};
 
 // 16 (or 4) bytes a lane from memory to LDS, lane after lane from the uniform address `dst` on.  Nothing
 // waits for these loads but the explicit s_waitcnt before the barrier that hands a stage over.  M0
-// holds the LDS address (one wait state before its use); the compiler uses that register for nothing
-// in these kernels.
+// holds the LDS address (one wait state before its use).  It is a register that the compiler reserves and warns of in a
+// list of clobbers; there it keeps a use of its own, of which these kernels have none now, from spanning a load.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ inline void to_lds(const uint8_t* base, uint32_t offset, uint32_t dst) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst), "v"(offset), "s"(base) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst), "v"(offset), "s"(base) : "m0", "memory");
 }
 __device__ inline void to_lds(const uint8_t* src, uint32_t dst) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(dst), "v"(src) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(dst), "v"(src) : "m0", "memory");
 }
 
 __device__ inline void dword_to_lds(const uint8_t* base, uint32_t offset, uint32_t dst) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(dst), "v"(offset), "s"(base) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(dst), "v"(offset), "s"(base) : "m0", "memory");
 }
 __device__ inline void dword_to_lds(const uint8_t* src, uint32_t dst) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(dst), "v"(src) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(dst), "v"(src) : "m0", "memory");
 }
+#pragma clang diagnostic pop
 
 template <int WT>
 struct Fragments {
