@@ -416,3 +416,49 @@ def test_norms_are_called_as_modules_with_their_own_eps(monkeypatch):
     calls.clear()
     model.use_mxfp4(False)(inputs)
     assert not calls
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_mxfp4_layers_against_the_oracle_before_and_after_a_reload(dtype):
+    """Every convolution, norm and the mel head on an input of its own, without the LSTMs of a library between them."""
+    import copy
+    from oracle import blocks_oracle as O
+    from test_blocks import check_block_norm, check_product
+    from tts_amd import Norm
+    w, other = random_weights(np.random.default_rng(21)), random_weights(np.random.default_rng(22))
+    rng = np.random.default_rng(23)
+
+    def check(model, weights):
+        layers = {"enc_conv1": model.encoder.block1, "enc_conv2": model.encoder.block2, "mel_out": model.mel_out,
+                  **{f"dur_conv{n}": b for n, b in enumerate(model.duration_predictor.blocks, 1)}}
+        for name, layer in layers.items():
+            conv, norm = (layer, None) if name == "mel_out" else (layer.conv, layer.norm)
+            x = torch.from_numpy(rng.normal(0, 1, (2, 21, 256))).to(dtype).cuda()
+            xv = O.mxfp4_round(x.cpu().double().numpy())
+
+            def held(key):  # what the layer keeps of a loaded array
+                return torch.from_numpy(weights[name + key]).float().to(dtype).double().numpy()
+
+            wv = O.mxfp4_round(held("_kernel").transpose(2, 0, 1))
+            want, size = O.conv1d(xv, wv, held("_bias"), conv.dilation[0])
+            k = wv.shape[1] * wv.shape[2]
+            if norm is None:
+                check_product(conv(x.transpose(1, 2)).transpose(1, 2), want, size, k, dtype)
+                continue
+            out, [(_, y), (u, _)] = through(layer, [conv, norm], lambda: layer(x))
+            check_product(y.transpose(1, 2), want, size, k, dtype)
+            assert torch.equal(u, torch.relu(y.transpose(1, 2)))
+            check_block_norm(u, Norm(norm.weight, norm.bias, norm.eps), None, None, None, None, out)
+            assert torch.equal(layer(x), out)  # the rectifier within the product
+
+    with torch.no_grad():
+        model = FastSpeechAcousticModel(VOCAB).load_keras_weights(w).cuda().to(dtype).use_mxfp4()
+        check(model, w)
+        twin = copy.deepcopy(model)
+        check(model.load_keras_weights(other), other)
+        check(twin, w)
+        model.load_state_dict(twin.state_dict())
+        check(model, w)
+        twin.cpu().load_state_dict(FastSpeechAcousticModel(VOCAB).load_keras_weights(other).state_dict())
+        check(twin.cuda(), other)

@@ -920,3 +920,48 @@ def test_inline_assembly_names_the_registers_that_it_writes():
             found += 1
             assert '"m0"' in statement.rsplit(":", 1)[1], (name, statement)
     assert found == 4
+
+
+# shapes whose activations the tiled convolutions quantise themselves: of up to 128 columns of y and of more, channels
+# that end inside a block, entries of one row and of many
+@gpu
+@pytest.mark.parametrize("batch,time,c,n,taps,dilation", [
+    (330, 100, 8, 80, 5, 7), (65, 505, 300, 128, 3, 1), (25001, 2, 40, 33, 7, 2), (72, 700, 130, 200, 3, 2), (70, 705, 256, 250, 4, 5),
+    (50001, 1, 384, 256, 1, 1), (64, 865, 256, 256, 3, 1), (71, 700, 101, 140, 2, 9)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_conv1d_quantising_in_its_tiles(dtype, batch, time, c, n, taps, dilation):
+    rng = np.random.default_rng(batch + time + c + n)
+    x, w, bias = draw(rng, batch, time, c, dtype=dtype), draw(rng, n, taps, c, scale=(taps * c) ** -0.5), draw(rng, n)
+    x[batch // 2] = 0
+    q = mxfp4_quantize(w)
+    rows, wv = gathered(mxfp4_quantize(x).dequantize().double(), taps, dilation), q.dequantize().double().reshape(n, -1)
+    y = mxfp4_conv1d(x, q, bias, dilation=dilation, activation="relu")
+    check_product_on_device(y, rows, wv, bias, True)
+    # the same rows between others, and 2 bytes off any alignment
+    wide = torch.full((batch, time + 3, c + 5), float("nan"), dtype=dtype, device="cuda")
+    wide[:, 2:2 + time, 1:1 + c] = x
+    assert torch.equal(mxfp4_conv1d(wide[:, 2:2 + time, 1:1 + c], q, bias, dilation=dilation, activation="relu"), y)
+
+
+@gpu
+@pytest.mark.parametrize("m,n,k", [(2100, 1000, 100), (4000, 1000, 1), (2100, 1000, 300), (1900, 1100, 500)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_two_teams_share_out_one_group_and_odd_ones(dtype, m, n, k):
+    rng = np.random.default_rng(m + n + k)
+    x, w, bias = draw(rng, m, k, dtype=dtype), draw(rng, n, k, scale=k ** -0.5), draw(rng, n)
+    q, xq = mxfp4_quantize(w), mxfp4_quantize(x)
+    xv, wv = xq.dequantize().double(), q.dequantize().double()
+    check_product_on_device(mxfp4_linear(x, q, bias), xv, wv, bias, False)
+    check_product_on_device(mxfp4_linear(xq, q, bias, activation="relu", out_dtype=dtype), xv, wv, bias, True)
+
+
+@gpu
+@pytest.mark.parametrize("c", [12280, 12289, 16385, 20001, 32761])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_block_norm_of_wide_ragged_rows(dtype, c):
+    rng = np.random.default_rng(c)
+    u, gate, residual = (draw(rng, 1, 3, c, dtype=dtype) for _ in range(3))
+    scale = torch.from_numpy(rng.normal(0.5, 0.1, c)).to(dtype).cuda()
+    for kind in ("layer", "rms"):
+        post, pre = norm_vectors(rng, kind, c, dtype), norm_vectors(rng, kind, c, dtype)
+        check_block_norm(u, post, gate, scale, residual, pre, block_norm(u, post=post, gate=gate, scale=scale, residual=residual, pre=pre))
