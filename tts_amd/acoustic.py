@@ -99,31 +99,33 @@ class _SequenceConv(nn.Conv1d):
             self.mxfp4_data = old.copy_(self.mxfp4_data)
         self.stale = False
 
-    def forward(self, x, relu=False):  # (B, C, T)
-        if self.mxfp4_data is None:
-            y = super().forward(x)
-            return F.relu(y) if relu else y
+    def forward(self, x):  # (B, C, T)
+        if self._buffers["mxfp4_data"] is None:
+            return super().forward(x)
+        return self.product(x.transpose(-1, -2)).transpose(-1, -2)
+
+    def product(self, x, relu=False):  # (B, T, C), in MXFP4
         if self.stale:
             raise ValueError("the weights were loaded where they cannot be quantised: move the module to a ROCm GPU "
                              "in float32, bfloat16 or float16 and call use_mxfp4() again")
         n, c, taps = self.weight.shape
         weight = MXFP4Tensor((n, taps, c) if taps > 1 else (n, c), self.mxfp4_data)
-        x, activation = x.transpose(-1, -2), "relu" if relu else None
+        activation = "relu" if relu else None
         if taps == 1:
-            y = mxfp4_linear(x, weight, self.bias, activation=activation)
-        else:
-            y = mxfp4_conv1d(x, weight, self.bias, dilation=self.dilation[0], activation=activation)
-        return y.transpose(-1, -2)
+            return mxfp4_linear(x, weight, self.bias, activation=activation)
+        return mxfp4_conv1d(x, weight, self.bias, dilation=self.dilation[0], activation=activation)
 
-    def joins_relu(self):
-        """Whether the product may rectify its own output: a hook sees the layer's output before that."""
-        return self.mxfp4_data is not None and not self._forward_hooks and not nn.modules.module._global_forward_hooks
+    def is_bare(self):
+        """Whether nothing would notice that the product is called past the module, with the rectifier in it: no hook and no
+        forward that was put in the place of the class's (a call and its views cost 5 us of a block's 24)."""
+        return not (self._forward_hooks or self._forward_pre_hooks or self._backward_hooks or self._backward_pre_hooks
+                    or "forward" in self.__dict__ or nn.modules.module._has_any_global_hook())
 
 
 def _along_time(layer, x, relu=False):
     """`layer`, a convolution of (B, C, T), over (B, T, C)."""
-    if relu and isinstance(layer, _SequenceConv) and layer.joins_relu():
-        return layer(x.transpose(1, 2), relu=True).transpose(1, 2)
+    if isinstance(layer, _SequenceConv) and layer._buffers["mxfp4_data"] is not None and layer.is_bare():
+        return layer.product(x, relu)
     y = layer(x.transpose(1, 2))
     return (F.relu(y) if relu else y).transpose(1, 2)
 
