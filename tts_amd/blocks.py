@@ -176,7 +176,7 @@ def mxfp4_quantize(x):
     """(..., K) float tensor -> `MXFP4Tensor`.  The scale of 32 elements is 2 ** (floor(log2 max|x|) - 2),
     at least 2 ** -127; an element goes to the nearest code, ties to the even one, beyond 6 to 6.  A block
     that holds an infinity or a NaN reads back as NaN.  Any strides; a last dimension that is not
-    contiguous is copied first."""
+    contiguous is copied first.  At most 2 ** 24 rows (all dimensions but the last) and 2 ** 18 columns."""
     _no_trace()
     kind, shape = _check(x, "x"), x.shape
     if len(shape) < 1 or shape[-1] < 1:
@@ -273,6 +273,8 @@ def mxfp4_linear(x, weight, bias=None, *, activation=None, out_dtype=None):
     bias        (N,) float tensor or None
     activation  None or "relu"
     out_dtype   default: the type of x; float32 for an `MXFP4Tensor`
+
+    At most 2 ** 24 rows of x, and K and N at most 2 ** 18.
     """
     _check_weight(weight, 2, "(N, K)")
     return _product(x, weight, bias, 1, 1, activation, out_dtype)
@@ -284,7 +286,8 @@ def mxfp4_conv1d(x, weight, bias=None, *, dilation=1, activation=None, out_dtype
     left = dilation * (taps - 1) // 2 (Keras Conv1D(padding='same'), torch padding='same').
 
     weight is an `MXFP4Tensor` of shape (N, taps, C): a torch.nn.Conv1d weight is
-    ``mxfp4_quantize(conv.weight.permute(0, 2, 1))``.  The other arguments are `mxfp4_linear`'s."""
+    ``mxfp4_quantize(conv.weight.permute(0, 2, 1))``.  The other arguments are `mxfp4_linear`'s.
+    taps * C and N are at most 2 ** 18, B * T, N * taps and (taps - 1) * dilation at most 2 ** 24."""
     _check_weight(weight, 3, "(N, taps, C)")
     if not isinstance(x, (torch.Tensor, MXFP4Tensor)):
         raise ValueError(f"x must be a tensor, got {type(x).__name__}")
@@ -357,7 +360,8 @@ def block_norm(u, *, post=None, gate=None, scale=None, residual=None, pre=None):
     residual  tensor of u's shape and type, or None
     pre       `Norm` the next block starts with, or None
 
-    Statistics are 32 bits; y enters `pre` before it is rounded to u's type.  C is at most 32768."""
+    Statistics are 32 bits; y enters `pre` before it is rounded to u's type.  C is at most
+    32768, and there are at most 2 ** 24 rows."""
     _no_trace()
     kind, shape, index = _check(u, "u"), u.shape, u.get_device()
     if len(shape) < 1 or shape[-1] < 1:
