@@ -1028,9 +1028,12 @@ extern "C" int glv_mxfp4_product(const glv_mxfp4_product_args* a, void* workspac
     // workgroup of 128 x 128 and two teams alone on its CU 5 and 0.2 a group: the rule below fits where the two meet
     // (1700 tiles of 32 x 32 for two groups, 1300 for seven, 1100 for 19, 1000 for 64: 283 x 4812 x 2061, 1359 tiles,
     // 9.8 us against 8.7; 960 tiles, 158 x 6144 x 1749, 6.8 against 7.6; 1163 x 1807 x 160, 2109 tiles, 6.6 against 6.1).
+    // The hyperbola through those four points stands for no law of the card: near it the two forms are within about a tenth of each
+    // other, so that a card with another clock moves the border and costs no more than that.
     // Two teams a tile, while there is a CU for every tile: a wave a SIMD alone reaches half the rate (340 x 7567 x
     // 5126, 180 tiles: 16.4 us against 19.2 with one team, 15164 x 151 x 490, 238 tiles, 6.9 against 7.6; 18227 x 187 x
-    // 1375, 286 tiles, 13.7 against 11.3).
+    // 1375, 286 tiles, 13.7 against 11.3).  So too for a single group, of which the second team multiplies none: twice the
+    // waves convert and store y (2100 x 1000 x 128 7.4 against 7.8, 8000 x 500 x 128 8.8 and 9.1, 4096 x 1024 x 64 8.0 and 7.8).
     // 128 x 128 has three workgroups on a CU to hide each other's ends, but reads twice the LDS bytes of the larger
     // tiles for a product, and where it follows a kernel bound by memory its draw makes the card lower its clock
     // (10560 x 4096 x 1024: 38 us of zeros, 64 of random values; 41 and 47 for 128 x 256).  So sums of some length take
