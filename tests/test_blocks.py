@@ -965,3 +965,41 @@ def test_block_norm_of_wide_ragged_rows(dtype, c):
     for kind in ("layer", "rms"):
         post, pre = norm_vectors(rng, kind, c, dtype), norm_vectors(rng, kind, c, dtype)
         check_block_norm(u, post, gate, scale, residual, pre, block_norm(u, post=post, gate=gate, scale=scale, residual=residual, pre=pre))
+
+
+def freed(t):
+    t.untyped_storage().resize_(0)
+    return t
+
+
+def test_a_tensor_without_memory_is_not_none():
+    from tts_amd import blocks
+    with pytest.raises(ValueError, match="gate has no memory"):
+        blocks._pointer(freed(torch.ones(3, 4)), "gate")
+    assert blocks._pointer(torch.ones(0, 4), "gate") == 0
+    q = packed((5, 40))
+    freed(q.data)
+    with pytest.raises(ValueError, match="no memory"):
+        q._pointers()
+    assert packed((0, 40))._pointers() == (0, 0)
+
+
+@gpu
+def test_freed_arguments_are_refused_by_name():
+    def one(*shape):
+        return torch.ones(shape, device="cuda")
+
+    x, w = one(3, 40), mxfp4_quantize(one(5, 40))
+    for call, name in ((lambda: block_norm(x, gate=freed(one(3, 40))), "gate"), (lambda: block_norm(x, gate=freed(one(3, 1))), "gate"),
+                       (lambda: block_norm(x, residual=freed(one(3, 40))), "residual"), (lambda: block_norm(x, scale=freed(one(40))), "scale"),
+                       (lambda: block_norm(x, post=Norm(freed(one(40)))), "post.weight"), (lambda: block_norm(x, pre=Norm(None, freed(one(40)))), "pre.bias"),
+                       (lambda: mxfp4_linear(x, w, freed(one(5))), "bias")):
+        with pytest.raises(ValueError, match=f"{name} has no memory"):
+            call()
+    for call in (lambda: block_norm(freed(one(3, 40)), post=Norm()), lambda: mxfp4_linear(freed(one(3, 40)), w), lambda: mxfp4_quantize(freed(one(3, 40)))):
+        with pytest.raises(tts_amd._lib.GlvError, match="null argument"):
+            call()
+    freed(w.data)
+    for call in (lambda: mxfp4_linear(x, w), lambda: w.dequantize()):
+        with pytest.raises(ValueError, match="MXFP4 tensor has no memory"):
+            call()

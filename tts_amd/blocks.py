@@ -65,6 +65,15 @@ def _check(t, name, index=None):
     return kind
 
 
+def _pointer(t, name):
+    """The address of an argument that the library takes for absent where it is null: a tensor whose storage was given
+    back (as sharded parameters' are between their uses) must not pass for none."""
+    at = t.data_ptr()
+    if not at and t.numel():
+        raise ValueError(f"{name} has no memory: its storage was freed")
+    return at
+
+
 def _vector(t, name, n, index):
     """(n,) vector as (contiguous tensor, number of its type)."""
     kind = _check(t, name, index)
@@ -141,7 +150,7 @@ class MXFP4Tensor:
         return self.data[self.groups * self.rows * 64:].view(self.groups, self.rows, 4)
 
     def _pointers(self):
-        at = self.data.data_ptr()
+        at = _pointer(self.data, "the MXFP4 tensor")
         return at, at + self.groups * self.rows * 64
 
     def to(self, device):
@@ -238,7 +247,7 @@ def _product(x, weight, bias, taps, dilation, activation, out_dtype):
     bias_ptr, bias_kind = 0, 0
     if bias is not None:
         bias, bias_kind = _vector(bias, "bias", n, index)
-        bias_ptr = bias.data_ptr()
+        bias_ptr = _pointer(bias, "bias")
     lib = _lib.load()
     shape = (*shape[:-1], n)
     if batch * rows * n > _LARGE and lib.glv_mxfp4_product_workspace(_lib.mxfp4_product_args(
@@ -324,7 +333,7 @@ def _norm_vector(t, name, cols, index, kind, seen, held):
     if t.stride(0) != 1 or cols == 1:
         t = t.resolve_neg().contiguous()
         held.append(t)
-    return t.data_ptr(), k
+    return _pointer(t, name), k
 
 
 def _broadcast(gate, shape, batch, rows, cols):
@@ -399,7 +408,7 @@ def block_norm(u, *, post=None, gate=None, scale=None, residual=None, pre=None):
             gate_strides.append(1)
         else:
             g, gate_strides = _broadcast(gate, shape, batch, rows, cols)
-        gate_ptr = g.data_ptr()
+        gate_ptr = _pointer(g, "gate")
         held.append(g)
     res_ptr, res_batch, res_row = 0, 0, 0
     if residual is not None:
@@ -407,7 +416,7 @@ def block_norm(u, *, post=None, gate=None, scale=None, residual=None, pre=None):
             raise ValueError(f"residual must be {u.dtype} {tuple(shape)} like u, got {residual.dtype} "
                              f"{tuple(residual.shape)}")
         r, _, _, res_batch, res_row = _rows(residual, shape)
-        res_ptr = r.data_ptr()
+        res_ptr = _pointer(r, "residual")
         held.append(r)
     if u.is_contiguous():  # the shorter call, which would keep other strides
         y = torch.empty_like(u)
