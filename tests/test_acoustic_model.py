@@ -471,3 +471,18 @@ def test_a_forward_put_in_place_of_the_layers_runs_in_mxfp4():
     inputs = np.array([[3, 4, 5]]), np.ones((1, 3), np.float32)
     got = model(inputs)
     assert torch.equal(got, model.use_mxfp4(False)(inputs))
+
+
+def test_mxfp4_weights_quantised_in_inference_mode_stay_in_place(monkeypatch):
+    from types import SimpleNamespace
+    from tts_amd import acoustic
+    made = iter((1, 2, 3))
+    monkeypatch.setattr(acoustic, "mxfp4_quantize", lambda w: SimpleNamespace(data=torch.full((68,), next(made), dtype=torch.uint8)))
+    layer = FastSpeechAcousticModel(VOCAB).mel_out
+    with torch.inference_mode():
+        layer.quantize(True)
+        kept = layer.mxfp4_data
+        layer.quantize(True)
+        assert layer.mxfp4_data is kept
+    layer.quantize(True)
+    assert layer.mxfp4_data is kept and (kept == 3).all()

@@ -93,11 +93,15 @@ class _SequenceConv(nn.Conv1d):
 
     def quantize(self, on):
         old = self.mxfp4_data
-        self.mxfp4_data = mxfp4_quantize(self.weight.detach().permute(0, 2, 1)).data if on else None
-        if on and old is not None and old.device == self.mxfp4_data.device and not old.is_inference():
+        if not on:
+            self.mxfp4_data, self.stale = None, False
+            return
+        with torch.inference_mode(False):  # a buffer of inference mode could not be written outside it
+            self.mxfp4_data = mxfp4_quantize(self.weight.detach().permute(0, 2, 1)).data
+        self.stale = False
+        if old is not None and old.device == self.mxfp4_data.device and not old.is_inference():
             # where it was: a graph that was captured with the old weights reads the new ones, as of the float weights
             self.mxfp4_data = old.copy_(self.mxfp4_data)
-        self.stale = False
 
     def forward(self, x):  # (B, C, T)
         if self._buffers["mxfp4_data"] is None:
